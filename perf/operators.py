@@ -161,8 +161,8 @@ def prepare(case, seed):
     s.update(logits=logits, index=index.to(_IDS[case["ids"]]), teacher=teacher.to(_TYPES[case["teacher"]]),
              labels=label.to(_IDS[case["ids"]]) if case["hard"] > 0 else None,
              dloss=torch.rand(n, device="cuda", generator=gen) * weight)
-    if case["kind"] == "distill_dx":  # the forward pass has left the log-sum-exps behind
-        s["lse"] = _plain_lse(s)
+    if case["kind"] == "distill_dx":  # the forward pass has left the softmax statistics behind
+        s["stats"] = _plain_stats(s)
     return s
 
 
@@ -197,20 +197,18 @@ def _present(s):
     return there, there.any(1), labelled
 
 
-def _plain_log_sum(z):
-    top = z.max(dim=1, keepdim=True).values
-    return ((z - top).exp().sum(dim=1, keepdim=True).log() + top).squeeze(1)
-
-
-def _plain_lse(s):
-    """[rows, 2]: log-sum-exp of z / T for the rows with a teacher, of z for the rows with a label."""
+def _plain_stats(s):
+    """[rows, 3]: the largest logit m, log sum exp((z - m) / T) for the rows with a teacher and
+    log sum exp(z - m) for the rows with a label, zero where a row has no use for it."""
     c = s["case"]
     _, soft, labelled = _present(s)
     z = s["logits"][:, :c["vocab"]].float()
-    none = torch.zeros(c["rows"], device=z.device)
-    first = torch.where(soft, _plain_log_sum(z / c["temperature"]), none)
-    second = torch.where(labelled, _plain_log_sum(z), none) if c["hard"] > 0 else none
-    return torch.stack([first, second], dim=1)
+    m = z.max(dim=1).values
+    none = torch.zeros_like(m)
+    d = z - m[:, None]
+    first = torch.where(soft, (d / c["temperature"]).exp().sum(dim=1).log(), none)
+    second = torch.where(labelled, d.exp().sum(dim=1).log(), none) if c["hard"] > 0 else none
+    return torch.stack([torch.where(soft | labelled, m, none), first, second], dim=1)
 
 
 def _plain_teacher(s):
@@ -223,33 +221,33 @@ def _plain_teacher(s):
     return torch.where(there, logp.exp(), torch.zeros_like(logp)), logp
 
 
-def _plain_loss(s, lse):
+def _plain_loss(s, stats):
     c = s["case"]
     there, soft, labelled = _present(s)
     p, logp = _plain_teacher(s)
     at = torch.where(there, s["index"].long(), torch.zeros_like(s["index"], dtype=torch.int64))
-    logq = s["logits"].gather(1, at).float() / c["temperature"] - lse[:, :1]
+    logq = (s["logits"].gather(1, at).float() - stats[:, :1]) / c["temperature"] - stats[:, 1:2]
     loss = (p * (logp - logq)).sum(dim=1) * c["temperature"] ** 2
     if c["hard"] > 0:
         at = torch.where(labelled, s["labels"].long(), torch.zeros_like(s["labels"], dtype=torch.int64))
-        ce = lse[:, 1] - s["logits"].gather(1, at[:, None]).float().squeeze(1)
+        ce = stats[:, 2] - (s["logits"].gather(1, at[:, None]).float().squeeze(1) - stats[:, 0])
         loss = loss + torch.where(labelled, ce, torch.zeros_like(ce)) * c["hard"]
     return loss
 
 
-def _plain_dlogits(s, lse):
+def _plain_dlogits(s, stats):
     c = s["case"]
     there, soft, labelled = _present(s)
     p, _ = _plain_teacher(s)
-    z = s["logits"][:, :c["vocab"]].float()
+    z = s["logits"][:, :c["vocab"]].float() - stats[:, :1]
     a = (s["dloss"] * c["temperature"])[:, None]
     d = torch.zeros(s["logits"].shape, device=z.device)
     inner = d[:, :c["vocab"]]
-    inner += (z / c["temperature"] - lse[:, :1]).exp() * torch.where(soft[:, None], a, torch.zeros_like(a))
+    inner += (z / c["temperature"] - stats[:, 1:2]).exp() * torch.where(soft[:, None], a, torch.zeros_like(a))
     d.scatter_add_(1, torch.where(there, s["index"].long(), torch.zeros_like(s["index"], dtype=torch.int64)), -p * a)
     if c["hard"] > 0:
         h = torch.where(labelled, s["dloss"] * c["hard"], torch.zeros_like(s["dloss"]))[:, None]
-        inner += (z - lse[:, 1:]).exp() * h
+        inner += (z - stats[:, 2:]).exp() * h
         d.scatter_add_(1, torch.where(labelled, s["labels"].long(), torch.zeros_like(s["labels"], dtype=torch.int64))[:, None], -h)
     return d.to(s["logits"].dtype)
 
@@ -262,12 +260,12 @@ def run(s):
         return _plain_embedding(s)
     if c["kind"] == "embedding_dx":
         return _plain_embedding_dx(s)
-    lse = s["lse"] if c["kind"] == "distill_dx" else _plain_lse(s)
+    stats = s["stats"] if c["kind"] == "distill_dx" else _plain_stats(s)
     if c["kind"] == "distill":
-        return {"loss": _plain_loss(s, lse), "lse": lse}
+        return {"loss": _plain_loss(s, stats), "stats": stats}
     if c["kind"] == "distill_dx":
-        return _plain_dlogits(s, lse)
-    return {"loss": _plain_loss(s, lse), "dlogits": _plain_dlogits(s, lse)}
+        return _plain_dlogits(s, stats)
+    return {"loss": _plain_loss(s, stats), "dlogits": _plain_dlogits(s, stats)}
 
 
 def _own(s):
@@ -281,10 +279,10 @@ def _own(s):
                                out_dtype=_TYPES[c["out"]], grad=s["grad"])
     more = dict(temperature=c["temperature"], labels=s["labels"], hard_weight=c["hard"], vocab_size=c["vocab"])
     if c["kind"] == "distill":
-        loss, lse = op.topk_distill(s["logits"], s["index"], s["teacher"], **more)
-        return {"loss": loss, "lse": lse}
+        loss, stats = op.topk_distill(s["logits"], s["index"], s["teacher"], **more)
+        return {"loss": loss, "stats": stats}
     if c["kind"] == "distill_dx":
-        return op.topk_distill_dx(s["dloss"], s["logits"], s["index"], s["teacher"], s["lse"], **more)
+        return op.topk_distill_dx(s["dloss"], s["logits"], s["index"], s["teacher"], s["stats"], **more)
     loss, dlogits = op.topk_distill_step(s["logits"], s["index"], s["teacher"], s["dloss"], **more)
     return {"loss": loss, "dlogits": dlogits}
 
@@ -317,7 +315,7 @@ def work(case):
     write = 0 if case["kind"] == "distill" else n * (v + case["padded"]) * _BYTES[case["logits"]]
     sums = 2 if case["hard"] > 0 and case["temperature"] != 1.0 else 1
     passes = 2 if case["kind"] == "distill_step" else 1
-    return {"bytes": targets + read + write + n * 8, "flops": live * v * 3 * sums * passes}
+    return {"bytes": targets + read + write + n * (16 if case["kind"] == "distill" else 4), "flops": live * v * 3 * sums * passes}
 
 
 # ------------------------------------------------------------------------------------------- exact
@@ -353,7 +351,7 @@ def exact(case, seed):
         return dx
     t, v = c["temperature"], c["vocab"]
     p, index, some, label, labelled = _exact_target(s)
-    loss, lses, grads = [], [], []
+    loss, stats, grads = [], [], []
     for at in range(0, c["rows"], 1024):  # 64 bits of everything at once would not leave room for the rest
         cut = slice(at, at + 1024)
         z = s["logits"][cut, :v].double()
@@ -361,8 +359,10 @@ def exact(case, seed):
         pi, ii, li = p[cut], index[cut], label[cut][:, None]
         kl = (torch.xlogy(pi, pi) - pi * logq.gather(1, ii)).sum(1)
         loss.append(t * t * kl - c["hard"] * labelled[cut] * logq1.gather(1, li).squeeze(1))
-        lses.append(torch.stack([torch.logsumexp(z / t, 1) * some[cut],
-                                 torch.logsumexp(z, 1) * labelled[cut] * (1.0 if c["hard"] > 0 else 0.0)], 1))
+        m = z.amax(1)
+        hard = labelled[cut] * (1.0 if c["hard"] > 0 else 0.0)
+        stats.append(torch.stack([m * torch.maximum(some[cut], hard), (torch.logsumexp(z / t, 1) - m / t) * some[cut],
+                                  (torch.logsumexp(z, 1) - m) * hard], 1))
         if c["kind"] == "distill":
             continue
         g = logq.exp_().mul_(t * some[cut][:, None]).scatter_add_(1, ii, -t * pi)
@@ -371,7 +371,7 @@ def exact(case, seed):
         grads.append(torch.nn.functional.pad(g, (0, c["padded"])))
         del z, logq, logq1, g
     if c["kind"] == "distill":
-        return {"loss": torch.cat(loss), "lse": torch.cat(lses)}
+        return {"loss": torch.cat(loss), "stats": torch.cat(stats)}
     if c["kind"] == "distill_dx":
         return torch.cat(grads)
     return {"loss": torch.cat(loss), "dlogits": torch.cat(grads)}
