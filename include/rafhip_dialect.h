@@ -138,6 +138,30 @@ int rafhip_raf_defuse_tensor_make(const rafhip_tensor_desc* data, int32_t n_size
 int rafhip_raf_defuse_tensor_execute(rafhip_raf_env* env, const rafhip_tensor_desc* data,
                                      int32_t n_out, const rafhip_tensor_desc* outs, void* stream);
 
+/* raf.op.embedding(x, indices) -> a row of x per index, and raf.op.embedding_dx(dy, indices,
+ * num_weight) -> its gradient; see rafhip_vocab.h for the extension arguments.  out_code / out_bits:
+ * dtype of the output.  grad: a gradient to add to, the op's output then, or NULL. */
+int rafhip_raf_embedding_make(const rafhip_tensor_desc* x, const rafhip_tensor_desc* indices, double scale,
+                              int64_t first_row, int32_t out_code, int32_t out_bits, rafhip_raf_env** env_out);
+int rafhip_raf_embedding_dx_make(const rafhip_tensor_desc* dy, const rafhip_tensor_desc* indices,
+                                 const rafhip_tensor_desc* grad, int64_t num_weight, double scale, int64_t first_row,
+                                 int32_t has_padding, int64_t padding_index, int32_t out_code, int32_t out_bits,
+                                 rafhip_raf_env** env_out);
+
+/* Extension ops raf.op.topk_distill (kind 0; -> loss, stats), raf.op.topk_distill_dx (1; -> dlogits) and
+ * raf.op.topk_distill_step (2; -> loss, dlogits); see rafhip_vocab.h.  The logits' last dimension may
+ * be wider than vocab_size.  labels, dloss (kinds 1 and 2) and stats (kind 1) may be NULL where
+ * they have no part. */
+int rafhip_raf_topk_distill_make(int32_t kind, const rafhip_tensor_desc* logits, const rafhip_tensor_desc* topk_indices,
+                                 const rafhip_tensor_desc* topk_logits, const rafhip_tensor_desc* labels,
+                                 const rafhip_tensor_desc* dloss, const rafhip_tensor_desc* stats, double temperature,
+                                 double soft_weight, double hard_weight, int64_t vocab_size, rafhip_raf_env** env_out);
+
+/* Execute of the five ops above: the tensors in schema order (an absent one as a descriptor of
+ * negative rank) and the outputs.  Calls on one env may come from several threads. */
+int rafhip_raf_execute(rafhip_raf_env* env, int32_t n_in, const rafhip_tensor_desc* inputs, int32_t n_out,
+                       const rafhip_tensor_desc* outputs, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* OpEnv::RequestStream (include/raf/op.h:87).  The fuse_tensor and defuse_tensor OpEnvs request a
  * copy stream the way the reference's do (src/op/dialect/cuda/memory.cc:34, :89).  By default this
  * window leaves such requests unserved and the OpEnv launches on the `stream` argument.  With

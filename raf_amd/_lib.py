@@ -199,6 +199,14 @@ DIALECT_SYMBOLS = {
                                               POINTER(c_int64), c_int32, POINTER(c_int64), POINTER(c_void_p)]),
     "rafhip_raf_defuse_tensor_execute": (c_int, [c_void_p, POINTER(TensorDesc), c_int32, POINTER(TensorDesc),
                                                  c_void_p]),
+    "rafhip_raf_embedding_make": (c_int, [POINTER(TensorDesc), POINTER(TensorDesc), c_double, c_int64, c_int32, c_int32,
+                                          POINTER(c_void_p)]),
+    "rafhip_raf_embedding_dx_make": (c_int, [POINTER(TensorDesc)] * 3 + [c_int64, c_double, c_int64, c_int32, c_int64,
+                                                                         c_int32, c_int32, POINTER(c_void_p)]),
+    "rafhip_raf_topk_distill_make": (c_int, [c_int32] + [POINTER(TensorDesc)] * 6 + [c_double, c_double, c_double,
+                                                                                   c_int64, POINTER(c_void_p)]),
+    "rafhip_raf_execute": (c_int, [c_void_p, c_int32, POINTER(TensorDesc), c_int32, POINTER(TensorDesc), c_void_p, c_int64,
+                                   c_void_p]),
     "rafhip_raf_serve_stream_requests": (c_int, [c_int32]),
     "rafhip_raf_env_num_outputs": (c_int32, [c_void_p]),
     "rafhip_raf_env_output": (c_int, [c_void_p, c_int32, POINTER(c_int32), POINTER(c_int32), POINTER(c_int32),
@@ -237,6 +245,44 @@ DIALECT_SYMBOLS = {
     "rafhip_raf_env_name": (c_char_p, [c_void_p]),
     "rafhip_raf_env_op": (c_char_p, [c_void_p]),
     "rafhip_raf_env_destroy": (c_int, [c_void_p]),
+}
+
+class TopkDistillArgs(Structure):
+    """``rafhip_topk_distill_args`` of include/rafhip_vocab.h."""
+
+    _fields_ = [
+        ("logits", c_void_p),
+        ("topk_indices", c_void_p),
+        ("topk_logits", c_void_p),
+        ("labels", c_void_p),
+        ("rows", c_int64),
+        ("vocab", c_int64),
+        ("row_stride", c_int64),
+        ("topk", c_int32),
+        ("logits_dtype", c_int32),
+        ("topk_dtype", c_int32),
+        ("index_bits", c_int32),
+        ("temperature", c_float),
+        ("soft_weight", c_float),
+        ("hard_weight", c_float),
+    ]
+
+
+RAFHIP_MAX_TOPK = 1024
+
+# include/rafhip_vocab.h: the operators at the vocabulary (same library as the optimizer steps)
+VOCAB_SYMBOLS = {
+    "rafhip_embedding": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64, c_float,
+                                 c_void_p, c_int32, c_void_p]),
+    "rafhip_embedding_dx_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "rafhip_embedding_dx": (c_int, [c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int32,
+                                    c_int64, c_float, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p]),
+    "rafhip_topk_distill_workspace_bytes": (c_int64, [POINTER(TopkDistillArgs)]),
+    "rafhip_topk_distill": (c_int, [POINTER(TopkDistillArgs), c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "rafhip_topk_distill_dx": (c_int, [POINTER(TopkDistillArgs), c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                       c_void_p]),
+    "rafhip_topk_distill_step": (c_int, [POINTER(TopkDistillArgs), c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                         c_void_p, c_int64, c_void_p]),
 }
 
 # include/rafhip_device.h: the HIP runtime calls behind the rocm DeviceAPI (same library)
@@ -284,6 +330,7 @@ def optim():
         lib = ctypes.CDLL(str(OPTIM_LIB), mode=ctypes.RTLD_GLOBAL)
         _bind(lib, OPTIM_SYMBOLS)
         _bind(lib, DEVICE_SYMBOLS)
+        _bind(lib, VOCAB_SYMBOLS)
         _optim = lib
     return _optim
 

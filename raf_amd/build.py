@@ -30,9 +30,9 @@ HIP_FLAGS = [
 ]
 
 OPTIM_SOURCES = ["status.hip", "sgd.hip", "lans_kernels.hip", "lans_plan.hip", "l2norm.hip", "fuse_tensor.hip",
-                 "device_rt.hip"]
+                 "device_rt.hip", "embedding.hip", "topk_distill.hip"]
 DIALECT_SOURCES = ["dialect/registry.cc", "dialect/device_api.cc", "dialect/memory_pool.cc", "dialect/hip_dialect.cc",
-                   "dialect/raf_ir.cc", "dialect/hip_fusion.cc", "dialect/c_api.cc"]
+                   "dialect/hip_vocab.cc", "dialect/raf_ir.cc", "dialect/hip_fusion.cc", "dialect/c_api.cc"]
 
 
 def hipcc() -> str:
@@ -80,7 +80,8 @@ def glue_lib() -> Path:
 
 def build_glue() -> Path:
     """The only piece that sees torch's headers: host C++ built with the host compiler against the
-    installed torch (its C++ ABI setting included) and this interpreter's headers."""
+    installed torch (its C++ ABI setting included) and this interpreter's headers.  Linked with the
+    host layer, whose execute entry it calls."""
     import sysconfig
 
     import torch
@@ -93,7 +94,7 @@ def build_glue() -> Path:
     _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *incs,
           "-o", out, CSRC / "torch_glue.cpp", f"-L{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-lc10",
-          f"-Wl,-rpath,{torch_lib}"])
+          f"-Wl,-rpath,{torch_lib}", f"-L{LIB}", "-lraf_hip_dialect", "-Wl,-rpath,$ORIGIN"])
     return out
 
 

@@ -51,6 +51,7 @@ struct rafhip_raf_env {
   std::vector<GraphCall> graph_calls;
   std::vector<size_t> var_counts;  // how many variables each descriptor list of the make call bound
   int kind = -1;                   // 0 SGD, 1 LANS
+  std::mutex executing;            // rafhip_raf_execute: the workspace bound to the OpEnv is one call's
 };
 
 namespace {
@@ -775,6 +776,92 @@ int rafhip_raf_defuse_tensor_execute(rafhip_raf_env* env, const rafhip_tensor_de
     StreamBinding streams(env->env.get(), env->call->device, stream);
     env->env->Execute(inputs, value::MakeTuple(std::move(fields)));
     streams.Finish();
+  });
+}
+
+// An argument that may be absent: a descriptor of negative rank, or none.
+static value::TensorValue Optional(const rafhip_tensor_desc* d, const char* what) {
+  return d && d->ndim >= 0 ? FromDesc(d, what) : nullptr;
+}
+static DType MakeDType(int32_t code, int32_t bits) {
+  DType t;
+  t.code = code;
+  t.bits = bits;
+  return t;
+}
+
+int rafhip_raf_embedding_make(const rafhip_tensor_desc* x, const rafhip_tensor_desc* indices, double scale,
+                              int64_t first_row, int32_t out_code, int32_t out_bits, rafhip_raf_env** env_out) {
+  return Guard([&] {
+    if (!env_out) throw Error("rafhip_raf_embedding_make: env_out is NULL");
+    *env_out = nullptr;
+    auto args = std::make_shared<schema::EmbeddingArgs>();
+    args->x = FromDesc(x, "x");
+    args->indices = FromDesc(indices, "indices");
+    args->scale = scale;
+    args->first_row = first_row;
+    args->out_dtype = MakeDType(out_code, out_bits);
+    *env_out = Finish(MakeCall("raf.op.embedding", args));
+  });
+}
+
+int rafhip_raf_embedding_dx_make(const rafhip_tensor_desc* dy, const rafhip_tensor_desc* indices,
+                                 const rafhip_tensor_desc* grad, int64_t num_weight, double scale, int64_t first_row,
+                                 int32_t has_padding, int64_t padding_index, int32_t out_code, int32_t out_bits,
+                                 rafhip_raf_env** env_out) {
+  return Guard([&] {
+    if (!env_out) throw Error("rafhip_raf_embedding_dx_make: env_out is NULL");
+    *env_out = nullptr;
+    auto args = std::make_shared<schema::EmbeddingDxArgs>();
+    args->dy = FromDesc(dy, "dy");
+    args->indices = FromDesc(indices, "indices");
+    args->grad = Optional(grad, "grad");
+    args->num_weight = num_weight;
+    args->scale = scale;
+    args->first_row = first_row;
+    args->has_padding = has_padding != 0;
+    args->padding_index = padding_index;
+    args->out_dtype = MakeDType(out_code, out_bits);
+    *env_out = Finish(MakeCall("raf.op.embedding_dx", args));
+  });
+}
+
+int rafhip_raf_topk_distill_make(int32_t kind, const rafhip_tensor_desc* logits, const rafhip_tensor_desc* topk_indices,
+                                 const rafhip_tensor_desc* topk_logits, const rafhip_tensor_desc* labels,
+                                 const rafhip_tensor_desc* dloss, const rafhip_tensor_desc* stats, double temperature,
+                                 double soft_weight, double hard_weight, int64_t vocab_size, rafhip_raf_env** env_out) {
+  return Guard([&] {
+    if (!env_out) throw Error("rafhip_raf_topk_distill_make: env_out is NULL");
+    *env_out = nullptr;
+    if (kind < 0 || kind > 2) throw Error("rafhip_raf_topk_distill_make: kind must be 0, 1 or 2");
+    auto args = std::make_shared<schema::TopkDistillArgs>();
+    args->logits = FromDesc(logits, "logits");
+    args->topk_indices = FromDesc(topk_indices, "topk_indices");
+    args->topk_logits = FromDesc(topk_logits, "topk_logits");
+    args->labels = Optional(labels, "labels");
+    args->dloss = Optional(dloss, "dloss");
+    args->stats = Optional(stats, "stats");
+    args->temperature = temperature;
+    args->soft_weight = soft_weight;
+    args->hard_weight = hard_weight;
+    args->vocab_size = vocab_size;
+    static const char* const kOps[] = {"raf.op.topk_distill", "raf.op.topk_distill_dx", "raf.op.topk_distill_step"};
+    *env_out = Finish(MakeCall(kOps[kind], args));
+  });
+}
+
+int rafhip_raf_execute(rafhip_raf_env* env, int32_t n_in, const rafhip_tensor_desc* inputs, int32_t n_out,
+                       const rafhip_tensor_desc* outputs, void* workspace, int64_t workspace_bytes, void* stream) {
+  return Guard([&] {
+    if (!env || !env->env) throw Error("rafhip_raf_execute: env is NULL");
+    if (n_in < 0 || n_out < 1 || (n_in > 0 && !inputs) || !outputs) throw Error("rafhip_raf_execute: bad tensor list");
+    std::vector<value::Value> in, out;
+    for (int32_t i = 0; i < n_in; ++i) in.push_back(Optional(&inputs[i], "input"));
+    for (int32_t i = 0; i < n_out; ++i) out.push_back(FromDesc(&outputs[i], "output"));
+    std::lock_guard<std::mutex> lock(env->executing);
+    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    WorkspaceBinding bind(env->env.get(), workspace, workspace_bytes);
+    env->env->Execute(in, n_out == 1 ? out[0] : value::MakeTuple(out));
   });
 }
 

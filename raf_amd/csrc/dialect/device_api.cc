@@ -192,7 +192,9 @@ class ROCMDeviceAPI final : public DeviceAPI {
 
  private:
   int device_id_ = 0;
-  void* stream_ = nullptr;  // the default stream unless the executor sets one
+  // The default stream unless the executor sets one; per thread, so that two threads' calls cannot
+  // exchange their streams between SetStream and Execute.
+  inline static thread_local void* stream_ = nullptr;
 };
 
 const bool kCpuRegistered = DeviceAPI::RegisterMaker("cpu", CPUDeviceAPI::make);

@@ -73,6 +73,7 @@ struct Device {
 };
 
 // DLPack-style dtype codes (kDLInt = 0, kDLUInt = 1, kDLFloat = 2, kDLBfloat = 4).
+constexpr int kDLInt = 0;
 constexpr int kDLFloat = 2;
 constexpr int kDLBfloat = 4;
 struct DType {
@@ -219,6 +220,40 @@ struct DefuseTensorArgs : ArgsBase {  // def_schema.py:836-841
   std::vector<int64_t> sizes;          // element count of every output
   std::vector<int64_t> shapes;         // all outputs' dimensions, concatenated
   std::vector<int64_t> shape_indices;  // end of every output's dimensions in `shapes`
+  int FieldIndex(const std::string& name) const override;
+};
+
+// raf.op.embedding(x, indices), with the extension fields scale (1), first_row (0) and the output's
+// dtype (x's).
+struct EmbeddingArgs : ArgsBase {
+  value::TensorValue x, indices;
+  double scale = 1.0;
+  int64_t first_row = 0;
+  DType out_dtype;
+  int FieldIndex(const std::string& name) const override;
+};
+
+// raf.op.embedding_dx(dy, indices, num_weight), with the extension fields grad (a gradient to add
+// to, in place, or null), scale, first_row, the padding index and the output's dtype.
+struct EmbeddingDxArgs : ArgsBase {
+  value::TensorValue dy, indices, grad;
+  int64_t num_weight = 0;
+  double scale = 1.0;
+  int64_t first_row = 0;
+  bool has_padding = false;
+  int64_t padding_index = 0;
+  DType out_dtype;
+  int FieldIndex(const std::string& name) const override;
+};
+
+// Extension ops raf.op.topk_distill, raf.op.topk_distill_dx and raf.op.topk_distill_step.  labels may
+// be null; dloss belongs to the last two, stats to topk_distill_dx.
+struct TopkDistillArgs : ArgsBase {
+  value::TensorValue logits, topk_indices, topk_logits, labels, dloss, stats;
+  double temperature = 1.0;
+  double soft_weight = 1.0;
+  double hard_weight = 0.0;
+  int64_t vocab_size = 0;
   int FieldIndex(const std::string& name) const override;
 };
 

@@ -91,6 +91,23 @@ int DefuseTensorArgs::FieldIndex(const std::string& name) const {
   return IndexIn(kNames, 4, name);
 }
 
+int EmbeddingArgs::FieldIndex(const std::string& name) const {
+  static const char* const kNames[] = {"x", "indices", "scale", "first_row", "out_dtype"};
+  return IndexIn(kNames, 5, name);
+}
+
+int EmbeddingDxArgs::FieldIndex(const std::string& name) const {
+  static const char* const kNames[] = {"dy",        "indices",     "grad",          "num_weight", "scale",
+                                       "first_row", "has_padding", "padding_index", "out_dtype"};
+  return IndexIn(kNames, 9, name);
+}
+
+int TopkDistillArgs::FieldIndex(const std::string& name) const {
+  static const char* const kNames[] = {"logits", "topk_indices", "topk_logits", "labels",      "dloss",
+                                       "stats",  "temperature",  "soft_weight", "hard_weight", "vocab_size"};
+  return IndexIn(kNames, 10, name);
+}
+
 }  // namespace schema
 
 CallValues MakeCall(const std::string& op_name, std::shared_ptr<schema::ArgsBase> args) {
@@ -241,6 +258,115 @@ void DefuseTensorDecl(const CallValues& call) {
   call->out = value::MakeTuple(std::move(outs));
 }
 
+bool IsIndex(const TensorView& t) { return t.dtype.code == kDLInt && (t.dtype.bits == 32 || t.dtype.bits == 64); }
+bool SameDevice(const TensorView& a, const TensorView& b) {
+  return a.device.device_type() == b.device.device_type() && a.device.device_id() == b.device.device_id();
+}
+bool SameDType(const DType& a, const DType& b) { return a.code == b.code && a.bits == b.bits; }
+
+// raf.op.embedding: one row of x per index, in the indices' shape.
+void EmbeddingDecl(const CallValues& call) {
+  const auto* args = call->args_as<schema::EmbeddingArgs>();
+  RAF_CHECK(args != nullptr && args->x && args->indices, "raf.op.embedding expects x and indices");
+  const TensorView& x = args->x->tensor;
+  const TensorView& ids = args->indices->tensor;
+  RAF_CHECK(x.ndim() == 2, "raf.op.embedding: x must be a table of rows");
+  RAF_CHECK(IsIndex(ids), "raf.op.embedding: indices must be int32 or int64");
+  RAF_CHECK(SameDevice(x, ids), "raf.op.embedding: x and indices are on different devices");
+  RAF_CHECK(args->first_row >= 0, "raf.op.embedding: first_row must not be negative");
+  TensorView out;
+  out.device = x.device;
+  out.dtype = args->out_dtype;
+  out.shape = ids.shape;
+  out.shape.push_back(x.shape[1]);
+  call->out = value::MakeTensor(out);
+  call->device = x.device;
+}
+
+// raf.op.embedding_dx: num_weight rows of dy's width; with grad the output is grad itself.
+void EmbeddingDxDecl(const CallValues& call) {
+  const auto* args = call->args_as<schema::EmbeddingDxArgs>();
+  RAF_CHECK(args != nullptr && args->dy && args->indices, "raf.op.embedding_dx expects dy and indices");
+  const TensorView& dy = args->dy->tensor;
+  const TensorView& ids = args->indices->tensor;
+  RAF_CHECK(IsIndex(ids), "raf.op.embedding_dx: indices must be int32 or int64");
+  RAF_CHECK(dy.ndim() == ids.ndim() + 1, "raf.op.embedding_dx: dy must have one dimension more than indices");
+  for (int i = 0; i < ids.ndim(); ++i)
+    RAF_CHECK(dy.shape[i] == ids.shape[i], "raf.op.embedding_dx: dy and indices differ in shape");
+  RAF_CHECK(SameDevice(dy, ids), "raf.op.embedding_dx: dy and indices are on different devices");
+  RAF_CHECK(args->num_weight >= 0, "raf.op.embedding_dx: num_weight must not be negative");
+  RAF_CHECK(args->first_row >= 0, "raf.op.embedding_dx: first_row must not be negative");
+  call->device = dy.device;
+  const std::vector<int64_t> shape = {args->num_weight, dy.shape.back()};
+  if (args->grad) {
+    const TensorView& grad = args->grad->tensor;
+    RAF_CHECK(grad.shape == shape, "raf.op.embedding_dx: grad must have num_weight rows of dy's width");
+    RAF_CHECK(SameDType(grad.dtype, args->out_dtype), "raf.op.embedding_dx: grad is not of the output's dtype");
+    RAF_CHECK(SameDevice(dy, grad), "raf.op.embedding_dx: dy and grad are on different devices");
+    call->out = args->grad;
+    return;
+  }
+  TensorView out;
+  out.device = dy.device;
+  out.dtype = args->out_dtype;
+  out.shape = shape;
+  call->out = value::MakeTensor(out);
+}
+
+// raf.op.topk_distill -> (loss, stats), raf.op.topk_distill_dx -> dlogits and
+// raf.op.topk_distill_step -> (loss, dlogits).
+void TopkDistillDecl(const CallValues& call, const std::string& op, bool gradient, bool needs_stats) {
+  const auto* args = call->args_as<schema::TopkDistillArgs>();
+  RAF_CHECK(args != nullptr && args->logits && args->topk_indices && args->topk_logits,
+            op + " expects logits, topk_indices and topk_logits");
+  const TensorView& z = args->logits->tensor;
+  const TensorView& index = args->topk_indices->tensor;
+  RAF_CHECK(z.ndim() >= 1, op + ": logits must have a vocabulary dimension");
+  const std::vector<int64_t> rows(z.shape.begin(), z.shape.end() - 1);
+  RAF_CHECK(index.ndim() == z.ndim() && std::equal(rows.begin(), rows.end(), index.shape.begin()),
+            op + ": topk_indices must have the logits' rows");
+  RAF_CHECK(args->topk_logits->tensor.shape == index.shape, op + ": topk_indices and topk_logits differ in shape");
+  RAF_CHECK(IsIndex(index), op + ": topk_indices must be int32 or int64");
+  RAF_CHECK(args->vocab_size >= 0 && args->vocab_size <= z.shape.back(), op + ": vocab_size exceeds the logits' width");
+  RAF_CHECK(SameDevice(z, index) && SameDevice(z, args->topk_logits->tensor), op + ": tensors are on different devices");
+  if (args->labels) {
+    const TensorView& labels = args->labels->tensor;
+    RAF_CHECK(labels.shape == rows, op + ": labels must have the logits' rows");
+    RAF_CHECK(SameDType(labels.dtype, index.dtype), op + ": labels must have the dtype of topk_indices");
+    RAF_CHECK(SameDevice(z, labels), op + ": tensors are on different devices");
+  }
+  const DType f32;
+  if (gradient) {
+    RAF_CHECK(args->dloss != nullptr, op + " expects dloss");
+    const TensorView& dloss = args->dloss->tensor;
+    RAF_CHECK(dloss.shape == rows || dloss.numel() == 1, op + ": dloss must have the logits' rows or one element");
+    RAF_CHECK(SameDType(dloss.dtype, f32), op + ": dloss must be float32");
+    RAF_CHECK(SameDevice(z, dloss), op + ": tensors are on different devices");
+  }
+  std::vector<int64_t> stats = rows;
+  stats.push_back(3);
+  if (needs_stats) {
+    RAF_CHECK(args->stats != nullptr, op + " expects stats");
+    RAF_CHECK(args->stats->tensor.shape == stats && SameDType(args->stats->tensor.dtype, f32),
+              op + ": stats must be float32, three for each row");
+    RAF_CHECK(SameDevice(z, args->stats->tensor), op + ": tensors are on different devices");
+  }
+  auto output = [&](const std::vector<int64_t>& shape, const DType& dtype) {
+    TensorView out;
+    out.device = z.device;
+    out.dtype = dtype;
+    out.shape = shape;
+    return value::MakeTensor(out);
+  };
+  if (!gradient)
+    call->out = value::MakeTuple({output(rows, f32), output(stats, f32)});
+  else if (needs_stats)
+    call->out = output(z.shape, z.dtype);
+  else
+    call->out = value::MakeTuple({output(rows, f32), output(z.shape, z.dtype)});
+  call->device = z.device;
+}
+
 }  // namespace
 
 void RunDeclare(const CallValues& call) {
@@ -254,6 +380,11 @@ void RunDeclare(const CallValues& call) {
   if (op == "raf.op.l2norm") return L2NormDecl(call);
   if (op == "raf.op.fuse_tensor") return FuseTensorDecl(call);
   if (op == "raf.op.defuse_tensor") return DefuseTensorDecl(call);
+  if (op == "raf.op.embedding") return EmbeddingDecl(call);
+  if (op == "raf.op.embedding_dx") return EmbeddingDxDecl(call);
+  if (op == "raf.op.topk_distill") return TopkDistillDecl(call, op, false, false);
+  if (op == "raf.op.topk_distill_dx") return TopkDistillDecl(call, op, true, true);
+  if (op == "raf.op.topk_distill_step") return TopkDistillDecl(call, op, true, false);
   throw Error("no declare function registered for op " + op);
 }
 

@@ -1,0 +1,882 @@
+// Distillation loss against a teacher's top logits, and its gradient, for gfx950.
+//
+//   loss = soft T^2 KL(p || softmax(z/T)) + hard CE(label, softmax(z)),  p = softmax over k entries
+//   dz   = dloss (soft T (softmax(z/T) - p) + hard (softmax(z) - onehot(label)))
+//
+// With m = max z and the two sums S_T = sum exp((z-m)/T), S_1 = sum exp(z-m) a row's loss needs its
+// k + 1 picked logits only:
+//   KL = sum p_j ((t_j - m_t) - (z_j - m))/T - log S_t + log S_T,  CE = log S_1 - (z_label - m),
+// and its gradient is an element-wise function of z with k + 1 corrections.  Keeping m and log S
+// apart (not their sum) keeps softmax exact to fp32 for logits of any magnitude, rows of the
+// type's lowest value included.
+//
+// What bounds it is memory: n V s bytes to read and, for the gradient, n V s to write.
+//   row_loss      forward, a workgroup per row, one pass with a running maximum and sums
+//   row_part      the same for few rows: several workgroups per row leave partial sums,
+//   join_loss     a wavefront per row joins them
+//   row_grad      gradient, workgroups over (row, columns)
+//   row_step      both: the row stays in the registers of one workgroup between its sums and its
+//                 gradient, so each logit is read once
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "rafhip_vocab.h"
+#include "status.h"
+#include "vocab_io.h"
+
+namespace rafhip {
+namespace {
+
+constexpr int kLanes = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxTop = RAFHIP_MAX_TOPK;
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What the kernels know about a call.
+struct Task {
+  const void* logits;
+  const void* indices;
+  const void* teacher;
+  const void* labels;
+  int64_t rows, row_stride;
+  int vocab, topk;
+  int teacher_dtype, index_bits;
+  float temperature, soft, hard;
+  float c_soft;  // log2(e) / T
+
+  __device__ __forceinline__ int64_t index_at(const void* p, int64_t i) const {
+    return index_bits == 32 ? (int64_t)((const RAFHIP_GLOBAL int32_t*)p)[i] : ((const RAFHIP_GLOBAL int64_t*)p)[i];
+  }
+  __device__ __forceinline__ float teacher_at(int64_t i) const {
+    if (teacher_dtype == RAFHIP_F32) return ((const RAFHIP_GLOBAL float*)teacher)[i];
+    if (teacher_dtype == RAFHIP_F16) return (float)((const RAFHIP_GLOBAL _Float16*)teacher)[i];
+    return bf16_widen(((const RAFHIP_GLOBAL unsigned short*)teacher)[i]);
+  }
+  // Column of teacher entry j of a row, -1 if it is absent; *t is its logit.
+  __device__ __forceinline__ int entry(int64_t row, int j, float* t) const {
+    const int64_t i = index_at(indices, row * topk + j);
+    *t = teacher_at(row * topk + j);
+    return i >= 0 && i < vocab && *t != -INFINITY ? (int)i : -1;
+  }
+  __device__ __forceinline__ int label(int64_t row) const {
+    if (!labels) return -1;
+    const int64_t i = index_at(labels, row);
+    return i >= 0 && i < vocab ? (int)i : -1;
+  }
+};
+
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float x, F&& f) {
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) x = f(x, __shfl_xor(x, d, kLanes));
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_add(float x) {
+  return wave_reduce(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ double wave_add(double x) {
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) x += __shfl_xor(x, d, kLanes);
+  return x;
+}
+
+// The teacher's softmax of one row, computed by a whole wavefront: p_j = exp2((t_j - top) c) / sum.
+struct Teacher {
+  float top, sum;
+  bool any;
+};
+__device__ __forceinline__ Teacher teacher_of(const Task& a, int64_t row) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  Teacher r;
+  float top = -INFINITY;
+  bool any = false;
+  for (int j = lane; j < a.topk; j += kLanes) {
+    float t;
+    if (a.entry(row, j, &t) >= 0) {
+      top = fmaxf(top, t);
+      any = true;
+    }
+  }
+  r.any = __any(any);
+  r.top = wave_max(top);
+  float sum = 0.f;
+  for (int j = lane; j < a.topk; j += kLanes) {
+    float t;
+    if (a.entry(row, j, &t) >= 0) sum += exp2_hw((t - r.top) * a.c_soft);
+  }
+  r.sum = wave_add(sum);
+  return r;
+}
+
+// Running maximum and sums of exp((z - m)/T) and, kTwo, exp(z - m) over the columns a lane has seen.
+// With one sum the factor is c_soft, or log2(e) if only the hard term is wanted.
+template <bool kTwo>
+struct Sums {
+  float m = -INFINITY;
+  float s0 = 0.f, s1 = 0.f;
+
+  // A maximum of -inf stands for "nothing yet": exponents are then taken against zero, so that
+  // -inf - -inf does not arise.
+  static __device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.f : m; }
+
+  __device__ __forceinline__ void rescale(float m2, float c0) {
+    const float d = m - base(m2);
+    s0 *= exp2_hw(d * c0);
+    if constexpr (kTwo) s1 *= exp2_hw(d * kLog2e);
+    m = m2;
+  }
+  __device__ __forceinline__ void term(float z, float b, float c0) {
+    const float d = z - b;
+    s0 += exp2_hw(d * c0);
+    if constexpr (kTwo) s1 += exp2_hw(d * kLog2e);
+  }
+  __device__ __forceinline__ void merge(float om, float o0, float o1, float c0) {
+    rescale(fmaxf(m, om), c0);
+    const float d = om - base(m);
+    s0 += o0 * exp2_hw(d * c0);
+    if constexpr (kTwo) s1 += o1 * exp2_hw(d * kLog2e);
+  }
+  __device__ __forceinline__ void wave_merge(float c0) {
+    rescale(wave_max(m), c0);
+    s0 = wave_add(s0);
+    if constexpr (kTwo) s1 = wave_add(s1);
+  }
+};
+
+// Joined over the workgroup, the same in every thread; `red` holds three floats per wavefront.
+template <int kWaves, bool kTwo>
+__device__ __forceinline__ void block_merge(Sums<kTwo>& a, float (*red)[3], float c0) {
+  a.wave_merge(c0);
+  if ((threadIdx.x & (kLanes - 1)) == 0) {
+    float* r = red[threadIdx.x / kLanes];
+    r[0] = a.m;
+    r[1] = a.s0;
+    r[2] = a.s1;
+  }
+  __syncthreads();
+  Sums<kTwo> all;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all.merge(red[w][0], red[w][1], red[w][2], c0);
+  a = all;
+}
+
+// A stretch of columns as up to `head` single elements, whole words and a tail: 16-bit rows of an
+// odd width start at an odd multiple of two bytes every other row, and words there would cost a
+// quarter of the bandwidth.
+struct Stretch {
+  int head, words, tail_at, tail;
+};
+template <typename T>
+__device__ __forceinline__ Stretch stretch_of(const T* at, int count) {
+  Stretch s;
+  s.head = sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(at) & 2) && count > 0 ? 1 : 0;
+  s.words = (count - s.head) / kWide;
+  s.tail_at = s.head + s.words * kWide;
+  s.tail = count - s.tail_at;
+  return s;
+}
+
+// The sums over `count` columns at z, by kBlock threads.
+template <typename T, bool kTwo, int kBlock>
+__device__ __forceinline__ void add_columns(Sums<kTwo>& a, const T* z, int count, float c0) {
+  constexpr int kInFlight = 4;
+  const Stretch s = stretch_of(z, count);
+  for (int w0 = threadIdx.x; w0 < s.words; w0 += kBlock * kInFlight) {
+    typename Wide<T>::Raw raw[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int w = w0 + u * kBlock;
+      raw[u] = w < s.words ? Wide<T>::load(z + s.head + (int64_t)w * kWide) : Wide<T>::fill(-INFINITY);
+    }
+    float top = a.m;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) top = fmaxf(top, Wide<T>::get(raw[u], j));
+    }
+    a.rescale(top, c0);
+    const float b = Sums<kTwo>::base(top);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (w0 + u * kBlock < s.words) {
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) a.term(Wide<T>::get(raw[u], j), b, c0);
+      }
+    }
+  }
+  // The single elements: the first and the last few, one per thread.
+  const int i = (int)threadIdx.x;
+  if (i < s.head + s.tail) {
+    const float x = Wide<T>::one(z + (i < s.head ? i : s.tail_at + i - s.head));
+    a.rescale(fmaxf(a.m, x), c0);
+    a.term(x, Sums<kTwo>::base(a.m), c0);
+  }
+}
+
+// Which sums a row's loss needs, and what they are called.
+struct RowSums {
+  float m;
+  double log_soft, log_hard;  // log S_T, log S_1
+};
+template <bool kTwo>
+__device__ __forceinline__ RowSums row_sums_of(const Sums<kTwo>& s) {
+  RowSums r;
+  r.m = s.s0 != s.s0 && s.m != INFINITY ? NAN : s.m;  // the running maximum passes over a NaN
+  r.log_soft = s.m == -INFINITY ? (double)NAN : log((double)s.s0);  // nothing but -inf has no softmax
+  r.log_hard = kTwo && s.m != -INFINITY ? log((double)s.s1) : r.log_soft;
+  return r;
+}
+
+// Loss and stats of a row, by one wavefront.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Task& a, int64_t row, const Teacher& t, int label, const RowSums& s,
+                                           float* loss, float* stats) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  const T* z = (const T*)a.logits + row * a.row_stride;
+  const double inv_t = 1.0 / (double)a.temperature;
+  double value = 0.0;
+  if (t.any) {
+    double cross = 0.0;  // sum of A_j ((t_j - top) - (z_j - m)), A_j = p_j * sum
+    for (int j = lane; j < a.topk; j += kLanes) {
+      float tj;
+      const int at = a.entry(row, j, &tj);
+      if (at >= 0) {
+        const float w = exp2_hw((tj - t.top) * a.c_soft);
+        if (w != 0.f) cross += (double)w * (((double)tj - (double)t.top) - ((double)Wide<T>::one(z + at) - (double)s.m));
+      }
+    }
+    cross = wave_add(cross);
+    const double kl = cross * inv_t / (double)t.sum - log((double)t.sum) + s.log_soft;
+    value += (double)a.soft * (double)a.temperature * (double)a.temperature * kl;
+  }
+  if (label >= 0) value += (double)a.hard * (s.log_hard - ((double)Wide<T>::one(z + label) - (double)s.m));
+  if (lane == 0) {
+    loss[row] = (float)value;
+    if (stats) {
+      const bool some = t.any || label >= 0;
+      stats[row * 3] = some ? s.m : 0.f;
+      stats[row * 3 + 1] = t.any ? (float)s.log_soft : 0.f;
+      stats[row * 3 + 2] = label >= 0 ? (float)s.log_hard : 0.f;
+    }
+  }
+}
+
+constexpr int kLossBlock = 512;
+
+template <typename T, bool kTwo>
+__global__ __launch_bounds__(kLossBlock) void row_loss(Task a, float c0, float* loss, float* stats) {
+  constexpr int kWaves = kLossBlock / kLanes;
+  __shared__ float red[kWaves][3];
+  const int64_t row = blockIdx.x;
+  const Teacher t = teacher_of(a, row);
+  const int label = a.label(row);
+  Sums<kTwo> s;
+  if (t.any || label >= 0) {  // the same in all threads
+    add_columns<T, kTwo, kLossBlock>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
+    block_merge<kWaves>(s, red, c0);
+  }
+  if (threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, stats);
+}
+
+constexpr int kPartBlock = 256;
+
+// Columns [split * per_split, ...) of a row: partial sums to parts[row][split][4].
+template <typename T, bool kTwo>
+__global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per_split, float* parts) {
+  constexpr int kWaves = kPartBlock / kLanes;
+  __shared__ float red[kWaves][3];
+  const int64_t row = blockIdx.y;
+  const int from = (int)blockIdx.x * per_split;
+  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
+  bool any = a.label(row) >= 0;  // a row without targets is not read
+  for (int j = threadIdx.x & (kLanes - 1); j < a.topk && !any; j += kLanes) {
+    float t;
+    any = a.entry(row, j, &t) >= 0;
+  }
+  Sums<kTwo> s;
+  if (__any(any)) {
+    add_columns<T, kTwo, kPartBlock>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
+    block_merge<kWaves>(s, red, c0);
+  }
+  if (threadIdx.x == 0) {
+    float* p = parts + (row * gridDim.x + blockIdx.x) * 4;
+    p[0] = s.m;
+    p[1] = s.s0;
+    p[2] = s.s1;
+  }
+}
+
+// The sums of a row from its parts, by a wavefront (the same in all lanes).
+template <bool kTwo>
+__device__ __forceinline__ Sums<kTwo> join_parts(const float* parts, int64_t row, int splits, float c0) {
+  Sums<kTwo> s;
+  const int lane = threadIdx.x & (kLanes - 1);
+  for (int i = lane; i < splits; i += kLanes) {
+    const float* p = parts + (row * splits + i) * 4;
+    s.merge(p[0], p[1], p[2], c0);
+  }
+  s.wave_merge(c0);
+  return s;
+}
+
+template <typename T, bool kTwo>
+__global__ __launch_bounds__(kLanes) void join_loss(Task a, float c0, const float* parts, int splits, float* loss,
+                                                    float* stats) {
+  const int64_t row = blockIdx.x;
+  const Teacher t = teacher_of(a, row);
+  finish_row<T>(a, row, t, a.label(row), row_sums_of(join_parts<kTwo>(parts, row, splits, c0)), loss, stats);
+}
+
+// ------------------------------------------------------------------------------------ gradient
+// g(z) = a0 exp2((z - m) c0 - l0) [+ a1 exp2((z - m) log2(e) - l1)], before the corrections.
+struct Grad {
+  float m, c0, l0, a0, l1, a1;
+  template <bool kTwo>
+  __device__ __forceinline__ float at(float z) const {
+    const float d = z - m;
+    float g = a0 * exp2_hw(fmaf(d, c0, -l0));
+    if constexpr (kTwo) g += a1 * exp2_hw(fmaf(d, kLog2e, -l1));
+    return g;
+  }
+};
+
+// kTwo: both sums are needed.  Otherwise one factor serves whatever is wanted: c0 is log2(e)/T with
+// hard == 0, or T == 1, or soft == 0 and c0 = log2(e).
+template <bool kTwo>
+__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, float m, float log_soft,
+                                        float log_hard) {
+  Grad g;
+  const float as = soft ? dloss * a.soft * a.temperature : 0.f, ah = hard ? dloss * a.hard : 0.f;
+  g.m = m;
+  g.c0 = c0;
+  if constexpr (kTwo) {
+    g.l0 = log_soft * kLog2e;
+    g.a0 = as;
+    g.l1 = log_hard * kLog2e;
+    g.a1 = ah;
+  } else {
+    g.l0 = (soft ? log_soft : log_hard) * kLog2e;
+    g.a0 = as + ah;
+    g.l1 = g.a1 = 0.f;
+  }
+  return g;
+}
+
+// The columns a row's targets correct.  Entries with the same column are taken together by the
+// first of them; whether there are any is found by a hash table, since comparing all pairs would
+// cost more than the row for hundreds of entries.
+// In dynamic LDS: picks_bytes(topk) bytes.
+struct Picks {
+  int n, n_slots;  // topk and the label; a power of two of at least twice that many
+  int* at;
+  float* minus;
+  int* slots;
+  int* twice;
+
+  __device__ __forceinline__ Picks(int topk, int log2_slots, int* lds) {
+    n = topk + 1;
+    n_slots = 1 << log2_slots;
+    twice = lds;
+    at = lds + 1;
+    minus = (float*)(at + n);
+    slots = (int*)(minus + n);
+  }
+};
+inline int picks_log2_slots(int topk) {
+  int log2 = 5;
+  while ((1 << log2) < 2 * (topk + 1)) ++log2;
+  return log2;
+}
+inline size_t picks_bytes(int topk) {
+  return 4 * (1 + 2 * ((size_t)topk + 1) + ((size_t)1 << picks_log2_slots(topk)));
+}
+
+// Fills in the targets of a row that lie in [from, from + count); a barrier must follow.
+template <int kBlock>
+__device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Teacher& t, int label, float dloss, int from,
+                                           int count, const Picks& p) {
+  for (int i = threadIdx.x; i < p.n_slots; i += kBlock) p.slots[i] = -1;
+  if (threadIdx.x == 0) *p.twice = 0;
+  const float scale = dloss * a.soft * a.temperature;
+  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+    int at = -1;
+    float minus = 0.f;
+    if (j == a.topk) {
+      at = label;
+      minus = dloss * a.hard;
+    } else {
+      float tj;
+      at = a.entry(row, j, &tj);
+      minus = scale * (exp2_hw((tj - t.top) * a.c_soft) / t.sum);
+    }
+    p.at[j] = at >= from && at < from + count ? at : -1;
+    p.minus[j] = minus;
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+    const int at = p.at[j];
+    if (at < 0) continue;
+    for (int h = at & (p.n_slots - 1);; h = (h + 1) & (p.n_slots - 1)) {  // half of the slots stay free
+      const int before = atomicCAS(&p.slots[h], -1, at);
+      if (before == -1) break;
+      if (before == at) {
+        *p.twice = 1;
+        break;
+      }
+    }
+  }
+}
+
+// Writes the corrected columns, behind a barrier that follows list_picks and the plain columns.
+template <typename T, bool kTwo, int kBlock>
+__device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T* z, T* out) {
+  const bool twice = *p.twice != 0;
+  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+    const int at = p.at[j];
+    if (at < 0) continue;
+    float minus = p.minus[j];
+    if (twice) {
+      bool first = true;
+      for (int i = 0; i < j && first; ++i) first = p.at[i] != at;
+      if (!first) continue;
+      for (int i = j + 1; i < p.n; ++i)
+        if (p.at[i] == at) minus += p.minus[i];
+    }
+    Wide<T>::put(out + at, g.template at<kTwo>(Wide<T>::one(z + at)) - minus);
+  }
+}
+
+template <typename T, int kBlock>
+__device__ __forceinline__ void put_zeros(T* out, int64_t count) {
+  const float none[kWide] = {};
+  const int64_t words = count / kWide;
+  for (int64_t w = threadIdx.x; w < words; w += kBlock) Wide<T>::store(out + w * kWide, none);
+  for (int64_t i = words * kWide + threadIdx.x; i < count; i += kBlock) Wide<T>::put(out + i, 0.f);
+}
+
+constexpr int kGradBlock = 256;
+
+// Columns [split * per_split, ...) of a row.  With `parts` the row's sums are joined from them and
+// the first split writes the loss; otherwise they come from `stats`.
+template <typename T, bool kTwo>
+__global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per_split, const float* dloss, int dloss_step,
+                                                       const float* stats, const float* parts, float* loss, T* dlogits,
+                                                       int64_t out_width, int log2_slots) {
+  constexpr int kInFlight = 4;
+  extern __shared__ int lds[];
+  const Picks picks(a.topk, log2_slots, lds);
+  const int64_t row = blockIdx.y;
+  const int splits = (int)gridDim.x;
+  const int from = (int)blockIdx.x * per_split;
+  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
+  const Teacher t = teacher_of(a, row);
+  const int label = a.label(row);
+  const float dl = dloss[row * dloss_step];
+  T* out_row = dlogits + row * out_width;
+  const T* z_row = (const T*)a.logits + row * a.row_stride;
+  if ((int)blockIdx.x == splits - 1) put_zeros<T, kGradBlock>(out_row + a.vocab, out_width - a.vocab);
+  Grad g;
+  if (parts) {
+    const RowSums s = row_sums_of(join_parts<kTwo>(parts, row, splits, c0));
+    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, s.m, (float)s.log_soft, (float)s.log_hard);
+    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, s, loss, nullptr);
+  } else {
+    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1], stats[row * 3 + 2]);
+  }
+  if (!t.any && label < 0) {
+    put_zeros<T, kGradBlock>(out_row + from, count);
+    return;
+  }
+  list_picks<kGradBlock>(a, row, t, label, dl, from, count, picks);
+  const T* z = z_row + from;
+  T* out = out_row + from;
+  const Stretch s = stretch_of(out, count);
+  for (int w0 = threadIdx.x; w0 < s.words; w0 += kGradBlock * kInFlight) {
+    typename Wide<T>::Raw raw[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int w = w0 + u * kGradBlock;
+      if (w < s.words) raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int w = w0 + u * kGradBlock;
+      if (w < s.words) {
+        float v[kWide];
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) v[j] = g.template at<kTwo>(Wide<T>::get(raw[u], j));
+        Wide<T>::store(out + s.head + (int64_t)w * kWide, v);
+      }
+    }
+  }
+  const int i = (int)threadIdx.x;
+  if (i < s.head + s.tail) {
+    const int c = i < s.head ? i : s.tail_at + i - s.head;
+    Wide<T>::put(out + c, g.template at<kTwo>(Wide<T>::one(z + c)));
+  }
+  __syncthreads();
+  put_picks<T, kTwo, kGradBlock>(picks, g, z_row, out_row);
+}
+
+constexpr int kStepBlock = 1024;
+constexpr int kStepMaxWords16 = 16, kStepMaxWords32 = 8;  // words per thread that stay in registers
+
+// Loss and gradient of a row that fits kWords words per thread.
+template <typename T, bool kTwo, int kWords>
+__global__ __launch_bounds__(kStepBlock) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
+                                                       T* dlogits, int64_t out_width, int log2_slots) {
+  constexpr int kWaves = kStepBlock / kLanes;
+  __shared__ float red[2][kWaves][3];
+  extern __shared__ int lds[];
+  const Picks picks(a.topk, log2_slots, lds);
+  const int64_t row = blockIdx.x;
+  const T* z = (const T*)a.logits + row * a.row_stride;
+  T* out = dlogits + row * out_width;
+  const Stretch s = stretch_of(out, a.vocab);
+  const int i = (int)threadIdx.x;
+  const bool single = i < s.head + s.tail;
+  const int single_at = i < s.head ? i : s.tail_at + i - s.head;
+  const Teacher t = teacher_of(a, row);
+  const int label = a.label(row);
+  const float dl = dloss[row * dloss_step];
+  put_zeros<T, kStepBlock>(out + a.vocab, out_width - a.vocab);
+  if (!t.any && label < 0) {
+    put_zeros<T, kStepBlock>(out, a.vocab);
+    if (i == 0) loss[row] = 0.f;
+    return;
+  }
+  typename Wide<T>::Raw raw[kWords];
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+    const int w = i + u * kStepBlock;
+    raw[u] = w < s.words ? Wide<T>::load(z + s.head + (int64_t)w * kWide) : Wide<T>::fill(-INFINITY);
+  }
+  const float x1 = single ? Wide<T>::one(z + single_at) : -INFINITY;
+  list_picks<kStepBlock>(a, row, t, label, dl, 0, a.vocab, picks);
+  // The row's maximum first: the sums then need no rescaling.
+  float top = x1;
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) top = fmaxf(top, Wide<T>::get(raw[u], j));
+  }
+  top = wave_max(top);
+  if ((i & (kLanes - 1)) == 0) red[0][i / kLanes][0] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red[0][w][0]);
+  // The words are widened again for the sums and for the gradient: kept in 16 bits between the
+  // phases they leave room for two workgroups per CU.
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
+  Sums<kTwo> sums;
+  sums.m = top;
+  const float b = Sums<kTwo>::base(top);
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+    if (i + u * kStepBlock < s.words) {
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) sums.term(Wide<T>::get(raw[u], j), b, c0);
+    }
+  }
+  if (single) sums.term(x1, b, c0);
+  sums.s0 = wave_add(sums.s0);
+  if constexpr (kTwo) sums.s1 = wave_add(sums.s1);
+  if ((i & (kLanes - 1)) == 0) {
+    red[1][i / kLanes][0] = sums.s0;
+    red[1][i / kLanes][1] = sums.s1;
+  }
+  __syncthreads();
+  sums.s0 = sums.s1 = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    sums.s0 += red[1][w][0];
+    sums.s1 += red[1][w][1];
+  }
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
+  const RowSums rs = row_sums_of(sums);
+  const Grad g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, rs.m, (float)rs.log_soft, (float)rs.log_hard);
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+    const int w = i + u * kStepBlock;
+    if (w < s.words) {
+      float v[kWide];
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) v[j] = g.template at<kTwo>(Wide<T>::get(raw[u], j));
+      Wide<T>::store(out + s.head + (int64_t)w * kWide, v);
+    }
+  }
+  if (single) Wide<T>::put(out + single_at, g.template at<kTwo>(x1));
+  if (i < kLanes) finish_row<T>(a, row, t, label, rs, loss, nullptr);
+  __syncthreads();
+  put_picks<T, kTwo, kStepBlock>(picks, g, z, out);
+}
+
+// ---------------------------------------------------------------------------------------- host
+constexpr int kWantBlocks = 1024;     // four workgroups for each of 256 CUs
+constexpr int kMinPerSplit = 4096;    // columns below which another workgroup does not pay
+constexpr int kGradColumns = 16384;   // columns of a row_grad workgroup where rows are plenty
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Columns per workgroup so that `rows` rows make kWantBlocks workgroups, a multiple of a word.
+int columns_per_split(int64_t rows, int64_t vocab, int64_t most) {
+  const int64_t splits = ceil_div(kWantBlocks, rows < 1 ? 1 : rows);
+  int64_t per = ceil_div(vocab, splits);
+  if (per > most) per = ceil_div(vocab, ceil_div(vocab, most));
+  if (per < kMinPerSplit) per = kMinPerSplit;
+  return (int)((per + kWide - 1) / kWide * kWide);
+}
+
+// One workgroup per row, or several with their partial sums in the workspace.
+bool rows_are_split(int64_t rows, int64_t vocab) { return rows < kWantBlocks / 2 && vocab > kMinPerSplit; }
+int splits_of(int64_t rows, int64_t vocab) { return (int)ceil_div(vocab, columns_per_split(rows, vocab, vocab)); }
+
+int words_per_thread(int64_t vocab) { return (int)ceil_div(vocab / kWide, kStepBlock); }
+bool row_fits(int64_t vocab, int32_t dtype) {
+  return words_per_thread(vocab) <= (dtype == RAFHIP_F32 ? kStepMaxWords32 : kStepMaxWords16);
+}
+
+int check_args(const char* who, const rafhip_topk_distill_args* p) {
+  if (!p) return fail(RAFHIP_ERR_INVALID_ARG, "%s: args is NULL", who);
+  const rafhip_topk_distill_args& a = *p;
+  if (element_bytes(a.logits_dtype) == 0 || element_bytes(a.topk_dtype) == 0)
+    return fail(RAFHIP_ERR_UNSUPPORTED, "%s: dtypes %d and %d", who, a.logits_dtype, a.topk_dtype);
+  if (a.index_bits != 32 && a.index_bits != 64) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %d-bit indices", who, a.index_bits);
+  if (a.rows < 0 || a.vocab < 0 || a.topk < 0 || a.row_stride < a.vocab)
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: rows = %lld, vocab = %lld, row_stride = %lld, topk = %d", who, (long long)a.rows,
+                (long long)a.vocab, (long long)a.row_stride, a.topk);
+  if (a.vocab >= (1LL << 28) || a.row_stride >= (1LL << 28) || a.rows >= (1LL << 31) || a.topk > kMaxTop)
+    return fail(RAFHIP_ERR_UNSUPPORTED, "%s: rows = %lld, vocab = %lld, row_stride = %lld, topk = %d", who, (long long)a.rows,
+                (long long)a.vocab, (long long)a.row_stride, a.topk);
+  if (!(a.temperature > 0.f) || !std::isfinite(a.temperature) || !std::isfinite(1.f / a.temperature))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: temperature = %g", who, (double)a.temperature);
+  if (!std::isfinite(a.soft_weight) || !std::isfinite(a.hard_weight))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: soft_weight = %g, hard_weight = %g", who, (double)a.soft_weight, (double)a.hard_weight);
+  return RAFHIP_OK;
+}
+
+int check_pointers(const char* who, const rafhip_topk_distill_args& a) {
+  if ((a.vocab > 0 && !a.logits) || (a.topk > 0 && (!a.topk_indices || !a.topk_logits)))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
+  if (!is_aligned(a.logits, element_bytes(a.logits_dtype)) || !is_aligned(a.topk_logits, element_bytes(a.topk_dtype)) ||
+      !is_aligned(a.topk_indices, a.index_bits / 8) || !is_aligned(a.labels, a.index_bits / 8))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  return RAFHIP_OK;
+}
+
+int check_workspace(const char* who, int64_t need, const void* workspace, int64_t bytes) {
+  if (need > 0 && (!workspace || bytes < need))
+    return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p of %lld bytes, need %lld", who, workspace, (long long)bytes, (long long)need);
+  if (need > 0 && !is_aligned(workspace, 16)) return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
+  return RAFHIP_OK;
+}
+
+int check_gradient(const char* who, const rafhip_topk_distill_args& a, const float* dloss, int64_t dloss_count,
+                   const void* dlogits, int64_t out_width) {
+  if (dloss_count != a.rows && dloss_count != 1)
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: dloss has %lld values for %lld rows", who, (long long)dloss_count, (long long)a.rows);
+  if (out_width < a.vocab) return fail(RAFHIP_ERR_INVALID_ARG, "%s: out_width = %lld < vocab", who, (long long)out_width);
+  if (out_width >= (1LL << 28)) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: out_width = %lld", who, (long long)out_width);
+  if (a.rows > 0 && (!dloss || (out_width > 0 && !dlogits))) return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
+  if (!is_aligned(dloss, 4) || !is_aligned(dlogits, element_bytes(a.logits_dtype)))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  return RAFHIP_OK;
+}
+
+// A term that cannot matter is dropped here, so that the kernels neither read for it nor sum for it.
+Task task_of(const rafhip_topk_distill_args& a, bool* two, float* c0) {
+  Task t;
+  t.logits = a.logits;
+  t.indices = a.topk_indices;
+  t.teacher = a.topk_logits;
+  t.labels = a.hard_weight != 0.f ? a.labels : nullptr;
+  t.rows = a.rows;
+  t.row_stride = a.row_stride;
+  t.vocab = (int)a.vocab;
+  t.topk = a.soft_weight != 0.f ? a.topk : 0;
+  t.teacher_dtype = a.topk_dtype;
+  t.index_bits = a.index_bits;
+  t.temperature = a.temperature;
+  t.soft = a.soft_weight;
+  t.hard = a.hard_weight;
+  t.c_soft = (float)(1.44269504088896340736 / (double)a.temperature);
+  const bool soft = t.topk > 0, hard = t.labels != nullptr;
+  *two = soft && hard && a.temperature != 1.f;
+  *c0 = soft ? t.c_soft : kLog2e;
+  return t;
+}
+
+template <typename F>
+void with_flag(bool flag, F&& f) {
+  if (flag)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
+
+constexpr int64_t kMaxGridY = 65535;
+
+// Rows beyond what a launch's second dimension holds go into further launches.
+template <typename F>
+void for_row_blocks(const Task& t, size_t element, F&& f) {
+  for (int64_t r0 = 0; r0 < t.rows; r0 += kMaxGridY) {
+    Task part = t;
+    part.rows = t.rows - r0 < kMaxGridY ? t.rows - r0 : kMaxGridY;
+    part.logits = static_cast<const char*>(t.logits) + (size_t)r0 * (size_t)t.row_stride * element;
+    const size_t index = (size_t)t.index_bits / 8, teacher = t.teacher_dtype == RAFHIP_F32 ? 4 : 2;
+    part.indices = static_cast<const char*>(t.indices) + (size_t)r0 * (size_t)t.topk * index;
+    part.teacher = static_cast<const char*>(t.teacher) + (size_t)r0 * (size_t)t.topk * teacher;
+    if (t.labels) part.labels = static_cast<const char*>(t.labels) + (size_t)r0 * index;
+    f(part, r0);
+  }
+}
+
+}  // namespace
+}  // namespace rafhip
+
+extern "C" int64_t rafhip_topk_distill_workspace_bytes(const rafhip_topk_distill_args* args) {
+  using namespace rafhip;
+  clear_error();
+  if (check_args("rafhip_topk_distill_workspace_bytes", args) != RAFHIP_OK) return -1;
+  const rafhip_topk_distill_args& a = *args;
+  if (a.rows == 0 || a.vocab == 0) return 0;
+  // The combined call splits long rows too, whatever their number.
+  if (!rows_are_split(a.rows, a.vocab) && row_fits(a.vocab, a.logits_dtype)) return 0;
+  return a.rows * splits_of(a.rows, a.vocab) * 16;
+}
+
+extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* loss, float* stats, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  using namespace rafhip;
+  clear_error();
+  const char* who = "rafhip_topk_distill";
+  if (int st = check_args(who, args)) return st;
+  const rafhip_topk_distill_args& a = *args;
+  if (a.rows == 0) return RAFHIP_OK;
+  if (int st = check_pointers(who, a)) return st;
+  if (!loss) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss is NULL", who);
+  if (!is_aligned(loss, 4) || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  const bool split = rows_are_split(a.rows, a.vocab);
+  const int64_t need = split ? rafhip_topk_distill_workspace_bytes(args) : 0;
+  if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
+  bool two;
+  float c0;
+  const Task t = task_of(a, &two, &c0);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  with_element(a.logits_dtype, [&](auto e) {
+    with_flag(two, [&](auto flag) {
+      using T = decltype(e);
+      constexpr bool kTwo = decltype(flag)::value;
+      if (!split) {
+        hipLaunchKernelGGL((row_loss<T, kTwo>), dim3((unsigned)a.rows), dim3(kLossBlock), 0, s, t, c0, loss, stats);
+        return;
+      }
+      float* parts = static_cast<float*>(workspace);
+      const int splits = splits_of(a.rows, a.vocab);
+      hipLaunchKernelGGL((row_part<T, kTwo>), dim3((unsigned)splits, (unsigned)a.rows), dim3(kPartBlock), 0, s, t, c0,
+                         columns_per_split(a.rows, a.vocab, a.vocab), parts);
+      hipLaunchKernelGGL((join_loss<T, kTwo>), dim3((unsigned)a.rows), dim3(kLanes), 0, s, t, c0, parts, splits, loss, stats);
+    });
+  });
+  RAFHIP_HIP_TRY(hipGetLastError());
+  return RAFHIP_OK;
+}
+
+extern "C" int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, const float* dloss, int64_t dloss_count,
+                                      const float* stats, void* dlogits, int64_t out_width, void* stream) {
+  using namespace rafhip;
+  clear_error();
+  const char* who = "rafhip_topk_distill_dx";
+  if (int st = check_args(who, args)) return st;
+  const rafhip_topk_distill_args& a = *args;
+  if (int st = check_gradient(who, a, dloss, dloss_count, dlogits, out_width)) return st;
+  if (a.rows == 0 || out_width == 0) return RAFHIP_OK;
+  if (int st = check_pointers(who, a)) return st;
+  if (!stats || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: stats %p", who, (const void*)stats);
+  bool two;
+  float c0;
+  const Task t = task_of(a, &two, &c0);
+  const int per = columns_per_split(a.rows, a.vocab, kGradColumns);
+  const unsigned splits = (unsigned)(a.vocab > 0 ? ceil_div(a.vocab, per) : 1);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  with_element(a.logits_dtype, [&](auto e) {
+    with_flag(two, [&](auto flag) {
+      using T = decltype(e);
+      constexpr bool kTwo = decltype(flag)::value;
+      for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
+        const int step = dloss_count == 1 ? 0 : 1;
+        hipLaunchKernelGGL((row_grad<T, kTwo>), dim3(splits, (unsigned)part.rows), dim3(kGradBlock),
+                           picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, stats + r0 * 3,
+                           (const float*)nullptr, (float*)nullptr, static_cast<T*>(dlogits) + r0 * out_width, out_width,
+                           picks_log2_slots(t.topk));
+      });
+    });
+  });
+  RAFHIP_HIP_TRY(hipGetLastError());
+  return RAFHIP_OK;
+}
+
+extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, const float* dloss, int64_t dloss_count,
+                                        float* loss, void* dlogits, int64_t out_width, void* workspace,
+                                        int64_t workspace_bytes, void* stream) {
+  using namespace rafhip;
+  clear_error();
+  const char* who = "rafhip_topk_distill_step";
+  if (int st = check_args(who, args)) return st;
+  const rafhip_topk_distill_args& a = *args;
+  if (int st = check_gradient(who, a, dloss, dloss_count, dlogits, out_width)) return st;
+  if (a.rows == 0) return RAFHIP_OK;
+  if (int st = check_pointers(who, a)) return st;
+  if (!loss || !is_aligned(loss, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss %p", who, (const void*)loss);
+  const int64_t need = rafhip_topk_distill_workspace_bytes(args);
+  if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
+  bool two;
+  float c0;
+  const Task t = task_of(a, &two, &c0);
+  const int step = dloss_count == 1 ? 0 : 1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  with_element(a.logits_dtype, [&](auto e) {
+    with_flag(two, [&](auto flag) {
+      using T = decltype(e);
+      constexpr bool kTwo = decltype(flag)::value;
+      if (need == 0) {
+        auto go = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(kStepBlock), picks_bytes(t.topk), s, t, c0, dloss, step,
+                             loss, static_cast<T*>(dlogits), out_width, picks_log2_slots(t.topk));
+        };
+        const int words = words_per_thread(a.vocab);
+        if (words <= 1)
+          go(row_step<T, kTwo, 1>);
+        else if (words <= 2)
+          go(row_step<T, kTwo, 2>);
+        else if (words <= 4)
+          go(row_step<T, kTwo, 4>);
+        else if (words <= 8)
+          go(row_step<T, kTwo, 8>);
+        else if constexpr (sizeof(T) == 2)
+          go(row_step<T, kTwo, 16>);
+        return;
+      }
+      const int splits = splits_of(a.rows, a.vocab), per = columns_per_split(a.rows, a.vocab, a.vocab);
+      for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
+        float* parts = static_cast<float*>(workspace) + r0 * splits * 4;
+        hipLaunchKernelGGL((row_part<T, kTwo>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
+                           per, parts);
+        hipLaunchKernelGGL((row_grad<T, kTwo>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kGradBlock),
+                           picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, (const float*)nullptr,
+                           (const float*)parts, loss + r0, static_cast<T*>(dlogits) + r0 * out_width, out_width,
+                           picks_log2_slots(t.topk));
+      });
+    });
+  });
+  RAFHIP_HIP_TRY(hipGetLastError());
+  return RAFHIP_OK;
+}

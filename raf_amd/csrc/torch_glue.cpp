@@ -30,6 +30,14 @@
 //   grads(params) -> (list, missing)
 //       the `.grad` of every parameter (None where there is none) and how many are None
 //
+//   key(tensors) -> bytes
+//       dtype, device and shape of every tensor of a tuple (None allowed) packed into one bytes
+//       object: with the scalar arguments, what calls of one operator must share to be served by
+//       one OpEnv
+//   execute(env, inputs, outputs, workspace, workspace_bytes, stream) -> status
+//       rafhip_raf_execute on tuples of tensors (None for an absent input).  The interpreter's lock
+//       is held meanwhile: the call enqueues kernels and returns
+//
 // torch is used for nothing but this object access; no kernels, no allocator, no dispatcher.
 #include <Python.h>
 
@@ -240,6 +248,79 @@ PyObject* grads_impl(PyObject* args) {
   return Py_BuildValue("(Nn)", out, missing);
 }
 
+// One descriptor; a None becomes one of negative rank.  `shape` points into the tensor, which its
+// owner keeps.
+bool describe_one(PyObject* o, rafhip_tensor_desc* d) {
+  if (o == Py_None) {
+    *d = rafhip_tensor_desc{nullptr, 0, 0, 0, 0, -1, nullptr};
+    return true;
+  }
+  if (!THPVariable_Check(o)) {
+    PyErr_Format(PyExc_TypeError, "expected a tensor, got %s", Py_TYPE(o)->tp_name);
+    return false;
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_contiguous()) {
+    PyErr_SetString(PyExc_ValueError, "tensors must be contiguous");
+    return false;
+  }
+  if (!dtype_of(t.scalar_type(), &d->dtype_code, &d->dtype_bits)) {
+    PyErr_SetString(PyExc_TypeError, "a tensor has a dtype the operators do not take");
+    return false;
+  }
+  d->data = t.data_ptr();
+  d->device_type = t.is_cuda() ? kDevRocm : kDevCpu;
+  d->device_id = t.is_cuda() && t.device().has_index() ? t.device().index() : 0;
+  d->ndim = (int32_t)t.dim();
+  d->shape = t.sizes().data();
+  return true;
+}
+
+constexpr Py_ssize_t kMaxTensors = 8;
+
+bool describe_tuple(PyObject* tuple, rafhip_tensor_desc* descs, Py_ssize_t* n) {
+  if (!PyTuple_CheckExact(tuple) || PyTuple_GET_SIZE(tuple) > kMaxTensors) {
+    PyErr_SetString(PyExc_TypeError, "expected a tuple of up to 8 tensors");
+    return false;
+  }
+  *n = PyTuple_GET_SIZE(tuple);
+  for (Py_ssize_t i = 0; i < *n; ++i)
+    if (!describe_one(PyTuple_GET_ITEM(tuple, i), &descs[i])) return false;
+  return true;
+}
+
+PyObject* key_impl(PyObject* args) {
+  PyObject* tuple;
+  if (!PyArg_ParseTuple(args, "O", &tuple)) return nullptr;
+  rafhip_tensor_desc descs[kMaxTensors];
+  Py_ssize_t n = 0;
+  if (!describe_tuple(tuple, descs, &n)) return nullptr;
+  std::vector<int64_t> words;
+  words.reserve((size_t)n * 6);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const rafhip_tensor_desc& d = descs[i];
+    words.push_back(((int64_t)d.dtype_code << 40) | ((int64_t)d.dtype_bits << 32) | (uint32_t)d.ndim);
+    if (d.ndim < 0) continue;
+    words.push_back(((int64_t)d.device_type << 32) | (uint32_t)d.device_id);
+    for (int32_t k = 0; k < d.ndim; ++k) words.push_back(d.shape[k]);
+  }
+  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(words.data()),
+                                   (Py_ssize_t)(words.size() * sizeof(int64_t)));
+}
+
+PyObject* execute_impl(PyObject* args) {
+  unsigned long long env, workspace, stream;
+  long long workspace_bytes;
+  PyObject *inputs, *outputs;
+  if (!PyArg_ParseTuple(args, "KOOKLK", &env, &inputs, &outputs, &workspace, &workspace_bytes, &stream)) return nullptr;
+  rafhip_tensor_desc in[kMaxTensors], out[kMaxTensors];
+  Py_ssize_t n_in = 0, n_out = 0;
+  if (!describe_tuple(inputs, in, &n_in) || !describe_tuple(outputs, out, &n_out)) return nullptr;
+  return PyLong_FromLong(rafhip_raf_execute(reinterpret_cast<rafhip_raf_env*>(env), (int32_t)n_in, in, (int32_t)n_out, out,
+                                            reinterpret_cast<void*>(workspace), workspace_bytes,
+                                            reinterpret_cast<void*>(stream)));
+}
+
 // No C++ exception may reach the interpreter: torch raises c10::Error for tensors without storage.
 template <PyObject* (*F)(PyObject*)>
 PyObject* guarded(PyObject*, PyObject* args) {
@@ -260,6 +341,8 @@ PyMethodDef kMethods[] = {
     {"rebind", guarded<rebind_impl>, METH_VARARGS, "bring a described list up to date with tensors that replace a range of it"},
     {"unreferenced", guarded<unreferenced_impl>, METH_VARARGS, "whether the list holds the only reference to a range of its objects"},
     {"grads", guarded<grads_impl>, METH_VARARGS, "the .grad of every parameter and the number of missing ones"},
+    {"key", guarded<key_impl>, METH_VARARGS, "dtype, device and shape of the tensors of a tuple as bytes"},
+    {"execute", guarded<execute_impl>, METH_VARARGS, "run an OpEnv on tuples of tensors"},
     {"signature", guarded<signature_impl>, METH_VARARGS, "dtype, device and shape of every descriptor as bytes"},
     {nullptr, nullptr, 0, nullptr}};
 

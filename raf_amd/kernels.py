@@ -146,6 +146,150 @@ def l2norm(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     return out
 
 
+_INDEX_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _vocab_tensor(t: torch.Tensor, name: str, dtypes, device=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor on the GPU")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, expected {device}")
+    return t
+
+
+def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_row: int = 0,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rafhip_embedding``: ``out[t] = scale * x[indices[t] - first_row]`` (a new tensor of x's dtype
+    unless given; any of float32, float16, bfloat16)."""
+    _vocab_tensor(x, "x", _DTYPE_CODE)
+    _vocab_tensor(indices, "indices", _INDEX_BITS, x.device)
+    if x.dim() != 2:
+        raise ValueError(f"x: expected a table of rows, got {tuple(x.shape)}")
+    if out is None:
+        out = torch.empty(*indices.shape, x.shape[1], dtype=x.dtype, device=x.device)
+    elif tuple(_vocab_tensor(out, "out", _DTYPE_CODE, x.device).shape) != (*indices.shape, x.shape[1]):
+        raise ValueError(f"out: shape {tuple(out.shape)}")
+    with torch.cuda.device(x.device):
+        check(_lib.optim().rafhip_embedding(x.data_ptr(), _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], indices.data_ptr(),
+                                            _INDEX_BITS[indices.dtype], indices.numel(), int(first_row), float(scale),
+                                            out.data_ptr(), _DTYPE_CODE[out.dtype], _current_stream(x.device)))
+    return out
+
+
+def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, out: torch.Tensor, scale: float = 1.0,
+                 padding_idx: Optional[int] = None, first_row: int = 0, accumulate: bool = False) -> torch.Tensor:
+    """``rafhip_embedding_dx``: the gradient of ``embedding`` for its table into ``out`` (rows x
+    width), overwritten or, with ``accumulate``, added to."""
+    _vocab_tensor(dy, "dy", _DTYPE_CODE)
+    _vocab_tensor(indices, "indices", _INDEX_BITS, dy.device)
+    _vocab_tensor(out, "out", _DTYPE_CODE, dy.device)
+    if out.dim() != 2 or tuple(dy.shape) != (*indices.shape, out.shape[1]):
+        raise ValueError(f"dy {tuple(dy.shape)}, indices {tuple(indices.shape)}, out {tuple(out.shape)}")
+    lib = _lib.optim()
+    need = lib.rafhip_embedding_dx_workspace_bytes(indices.numel(), *out.shape)
+    ws = _scratch(need, dy.device)
+    with torch.cuda.device(dy.device):
+        check(lib.rafhip_embedding_dx(dy.data_ptr(), _DTYPE_CODE[dy.dtype], indices.data_ptr(), _INDEX_BITS[indices.dtype],
+                                      indices.numel(), out.shape[0], out.shape[1], int(first_row),
+                                      int(padding_idx is not None), int(padding_idx or 0), float(scale), out.data_ptr(),
+                                      _DTYPE_CODE[out.dtype], int(bool(accumulate)), ws.data_ptr() if ws is not None else None,
+                                      max(need, 0), _current_stream(dy.device)))
+    return out
+
+
+class TopkDistill:
+    """The arguments of ``rafhip_topk_distill`` and its gradient calls for one set of tensors:
+    ``logits`` of shape [rows, vocab], whose rows may lie further apart than vocab elements (a view of
+    the first columns of a wider matrix), ``topk_indices`` and ``topk_logits`` [rows, k], ``labels``
+    [rows] or None."""
+
+    def __init__(self, logits, topk_indices, topk_logits, temperature=1.0, soft_weight=1.0, labels=None, hard_weight=0.0):
+        if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
+            raise ValueError("logits: expected a matrix on the GPU")
+        if logits.dtype not in _DTYPE_CODE:
+            raise TypeError(f"logits: unsupported dtype {logits.dtype}")
+        rows, vocab = logits.shape
+        if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+            raise ValueError("logits: the elements of a row must be neighbours")
+        _vocab_tensor(topk_indices, "topk_indices", _INDEX_BITS, logits.device)
+        _vocab_tensor(topk_logits, "topk_logits", _DTYPE_CODE, logits.device)
+        if topk_indices.dim() != 2 or topk_indices.shape[0] != rows or topk_logits.shape != topk_indices.shape:
+            raise ValueError(f"topk_indices {tuple(topk_indices.shape)}, topk_logits {tuple(topk_logits.shape)}: need "
+                             f"[{rows}, k]")
+        if labels is not None:
+            _vocab_tensor(labels, "labels", (topk_indices.dtype,), logits.device)
+            if tuple(labels.shape) != (rows,):
+                raise ValueError(f"labels: shape {tuple(labels.shape)}")
+        self.logits, self.rows, self.vocab = logits, rows, vocab
+        self._keep = (topk_indices, topk_logits, labels)
+        self.args = _lib.TopkDistillArgs(logits.data_ptr(), topk_indices.data_ptr(), topk_logits.data_ptr(),
+                                         labels.data_ptr() if labels is not None else None, rows, vocab,
+                                         logits.stride(0) if rows > 1 else vocab, topk_indices.shape[1],
+                                         _DTYPE_CODE[logits.dtype], _DTYPE_CODE[topk_logits.dtype],
+                                         _INDEX_BITS[topk_indices.dtype], float(temperature), float(soft_weight),
+                                         float(hard_weight))
+
+    def _workspace(self):
+        need = _lib.optim().rafhip_topk_distill_workspace_bytes(ctypes.byref(self.args))
+        ws = _scratch(need, self.logits.device)
+        return ws, ws.data_ptr() if ws is not None else None, max(need, 0)
+
+    def _f32(self, t, name, numel):
+        _vocab_tensor(t, name, (torch.float32,), self.logits.device)
+        if t.numel() not in numel:
+            raise ValueError(f"{name}: {t.numel()} elements")
+        return t
+
+    def _out(self, out):
+        if out is None:
+            return torch.empty(self.rows, self.vocab, dtype=self.logits.dtype, device=self.logits.device)
+        _vocab_tensor(out, "out", (self.logits.dtype,), self.logits.device)
+        if out.dim() != 2 or out.shape[0] != self.rows or out.shape[1] < self.vocab:
+            raise ValueError(f"out: shape {tuple(out.shape)}")
+        return out
+
+    def loss(self):
+        """``rafhip_topk_distill``: ``(loss [rows], stats [rows, 3])``."""
+        dev = self.logits.device
+        loss = torch.empty(self.rows, dtype=torch.float32, device=dev)
+        stats = torch.empty(self.rows, 3, dtype=torch.float32, device=dev)
+        ws, at, nbytes = self._workspace()
+        with torch.cuda.device(dev):
+            check(_lib.optim().rafhip_topk_distill(ctypes.byref(self.args), loss.data_ptr(), stats.data_ptr(), at, nbytes,
+                                                   _current_stream(dev)))
+        return loss, stats
+
+    def dx(self, dloss, stats, out=None):
+        """``rafhip_topk_distill_dx``: the gradient for the logits; ``out`` may be wider than vocab."""
+        self._f32(dloss, "dloss", (1, self.rows))
+        self._f32(stats, "stats", (3 * self.rows,))
+        out = self._out(out)
+        with torch.cuda.device(self.logits.device):
+            check(_lib.optim().rafhip_topk_distill_dx(ctypes.byref(self.args), dloss.data_ptr(), dloss.numel(),
+                                                      stats.data_ptr(), out.data_ptr(), out.shape[1],
+                                                      _current_stream(self.logits.device)))
+        return out
+
+    def step(self, dloss, out=None):
+        """``rafhip_topk_distill_step``: ``(loss, gradient)`` at once."""
+        self._f32(dloss, "dloss", (1, self.rows))
+        out = self._out(out)
+        dev = self.logits.device
+        loss = torch.empty(self.rows, dtype=torch.float32, device=dev)
+        ws, at, nbytes = self._workspace()
+        with torch.cuda.device(dev):
+            check(_lib.optim().rafhip_topk_distill_step(ctypes.byref(self.args), dloss.data_ptr(), dloss.numel(),
+                                                        loss.data_ptr(), out.data_ptr(), out.shape[1], at, nbytes,
+                                                        _current_stream(dev)))
+        return loss, out
+
+
 class FusePlan:
     """Owns a ``rafhip_fuse_plan`` for a list of tensors of fixed byte sizes: ``fuse`` packs them
     back to back into one flat buffer, ``defuse`` unpacks it, one kernel launch each."""

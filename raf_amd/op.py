@@ -130,6 +130,7 @@ _env_cache = _EnvCache()
 
 def clear_op_env_cache() -> None:
     _env_cache.clear()
+    _vocab_envs.clear()
     _recent_lists.clear()
 
 
@@ -678,6 +679,163 @@ def defuse_tensor(data: torch.Tensor, sizes, shapes, shape_indices):
     descs = (TensorDesc * max(len(outs), 1))(*[_desc(t, keep) for t in outs])
     check_raf(lib.rafhip_raf_defuse_tensor_execute(env.handle, dd, len(outs), descs, _stream(data)))
     return outs
+
+
+# ------------------------------------------------------------------- the operators at the vocabulary
+class _VocabEnvCache(_EnvCache):
+    """Theirs are kept apart: batches of ever new lengths should not push the optimizers' OpEnvs out,
+    and these own no device memory."""
+
+    capacity = 256
+
+
+_vocab_envs = _VocabEnvCache()
+
+
+class _VocabEnv(_Env):
+    """An OpEnv with what a call of it allocates, read once: the outputs' shapes and dtypes."""
+
+    def __init__(self, handle, device):
+        super().__init__(handle)
+        self.address = handle.value
+        self.device = device
+        self.index = device.index or 0
+        lib = _lib.dialect()
+        self.outputs = []
+        for i in range(lib.rafhip_raf_env_num_outputs(handle)):
+            code, bits, ndim = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
+            shape = (c_int64 * 64)()
+            check_raf(lib.rafhip_raf_env_output(handle, i, ctypes.byref(code), ctypes.byref(bits), ctypes.byref(ndim),
+                                                shape, 64))
+            self.outputs.append((tuple(shape[:ndim.value]), _TORCH_DTYPES[(code.value, bits.value)]))
+
+
+def _make_vocab_env(key, device, make, tensors, *scalars) -> _VocabEnv:
+    keep: list = []
+    descs = [ctypes.byref(_desc(t, keep)) if t is not None else None for t in tensors]
+    h = c_void_p(None)
+    check_raf(make(*descs, *scalars, ctypes.byref(h)))
+    env = _vocab_envs[key] = _VocabEnv(h, device)
+    return env
+
+
+def _run_vocab(env: _VocabEnv, inputs, outputs=None):
+    """One call: outputs and workspace are torch's to allocate, on the current stream of the tensors'
+    device, so calls on several streams and captured graphs share neither."""
+    if env.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(env.index):
+            return _run_vocab(env, inputs, outputs)
+    if outputs is None:
+        outputs = tuple([torch.empty(shape, dtype=dtype, device=env.device) for shape, dtype in env.outputs])
+    nbytes = env.workspace_bytes
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=env.device) if nbytes else None
+    if _lib.glue().execute(env.address, inputs, outputs, ws.data_ptr() if nbytes else 0, nbytes,
+                           torch._C._cuda_getCurrentRawStream(env.index)):
+        check_raf(1)
+    return outputs
+
+
+def _out_dtype(dtype):
+    try:
+        return _DTYPES[dtype]
+    except KeyError:
+        raise TypeError(f"out_dtype: {dtype} is not a dtype the operators take") from None
+
+
+def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_row: int = 0,
+              out_dtype=None) -> torch.Tensor:
+    """``raf._op.imp.embedding(x, indices)``: the rows of the table ``x`` that ``indices`` (int32 or
+    int64, of any shape) name, one for each, as a new tensor.
+
+    Extensions: every element is multiplied by ``scale`` and rounded once to ``out_dtype`` (x's
+    unless given), so an fp32 master table can feed a 16-bit model directly.  ``first_row`` is the
+    index of the table's first row, for a table that is one shard of a vocabulary.  An index outside
+    the table (another shard's, or a negative one for padding) gives zeros, not an error: the host
+    does not look at the indices."""
+    scale, first_row = float(scale), int(first_row)
+    key = ("embedding", _lib.glue().key((x, indices)), scale, first_row, out_dtype)
+    env = _vocab_envs.get(key)
+    if env is None:
+        code, bits = _out_dtype(x.dtype if out_dtype is None else out_dtype)
+        env = _make_vocab_env(key, x.device, _lib.dialect().rafhip_raf_embedding_make, (x, indices), scale, first_row,
+                              code, bits)
+    return _run_vocab(env, (x, indices))[0]
+
+
+def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, num_weight: int, scale: float = 1.0, padding_idx=None,
+                 first_row: int = 0, out_dtype=None, grad: torch.Tensor = None) -> torch.Tensor:
+    """``raf._op.imp.embedding_dx(dy, indices, num_weight)``: the gradient of ``embedding`` for its
+    table, ``[num_weight, width]`` with zeros in the rows that no index names.
+
+    Extensions: ``scale`` and ``first_row`` as in ``embedding``; the gradient is summed in fp32 and
+    rounded once to ``out_dtype`` (dy's unless given).  Indices outside the table and those equal to
+    ``padding_idx`` take no part.  With ``grad`` the result is added to it in place and ``grad`` is
+    returned (of ``out_dtype``, if both are given): the gradient of a table that an output projection
+    shares, or of a batch in several parts.  Equal inputs give equal bits, however often an index
+    occurs."""
+    if out_dtype is None:
+        out_dtype = dy.dtype if grad is None else grad.dtype
+    num_weight, scale, first_row = int(num_weight), float(scale), int(first_row)
+    padding_idx = None if padding_idx is None else int(padding_idx)
+    key = ("embedding_dx", _lib.glue().key((dy, indices, grad)), num_weight, scale, padding_idx, first_row, out_dtype)
+    env = _vocab_envs.get(key)
+    if env is None:
+        code, bits = _out_dtype(out_dtype)
+        env = _make_vocab_env(key, dy.device, _lib.dialect().rafhip_raf_embedding_dx_make, (dy, indices, grad),
+                              num_weight, scale, first_row, int(padding_idx is not None), padding_idx or 0, code, bits)
+    return _run_vocab(env, (dy, indices, grad), (grad,) if grad is not None else None)[0]
+
+
+def _topk_distill(kind, logits, topk_indices, topk_logits, labels, dloss, stats, temperature, soft_weight, hard_weight,
+                  vocab_size):
+    inputs = (logits, topk_indices, topk_logits, labels, dloss, stats)
+    temperature, soft_weight, hard_weight = float(temperature), float(soft_weight), float(hard_weight)
+    vocab_size = None if vocab_size is None else int(vocab_size)
+    key = (kind, _lib.glue().key(inputs), temperature, soft_weight, hard_weight, vocab_size)
+    env = _vocab_envs.get(key)
+    if env is None:
+        if logits.dim() == 0:
+            raise ValueError("logits must have a vocabulary dimension")
+        make = lambda *a: _lib.dialect().rafhip_raf_topk_distill_make(kind, *a)
+        env = _make_vocab_env(key, logits.device, make, inputs, temperature, soft_weight, hard_weight,
+                              logits.shape[-1] if vocab_size is None else vocab_size)
+    return _run_vocab(env, inputs)
+
+
+def topk_distill(logits: torch.Tensor, topk_indices: torch.Tensor, topk_logits: torch.Tensor, temperature: float = 1.0,
+                 soft_weight: float = 1.0, labels: torch.Tensor = None, hard_weight: float = 0.0, vocab_size: int = None):
+    """Extension op: the loss of a student's ``logits [..., width]`` against the top logits of a
+    teacher, ``topk_logits [..., k]`` at the columns ``topk_indices``, per row
+
+        soft_weight * T^2 * KL(softmax(topk_logits / T) || softmax(logits / T))
+        + hard_weight * (-log softmax(logits)[label])
+
+    with T = ``temperature``.  Returns ``(loss [...], stats [..., 3])`` in float32; ``stats`` is what
+    ``topk_distill_dx`` needs.  A teacher entry whose index is outside the vocabulary (-1, say) or
+    whose logit is -inf is absent, and so is a label outside it (-100, say); a row without any has
+    loss 0 and no gradient, whatever its logits hold.  ``vocab_size`` leaves out the padding columns
+    of a widened output projection.  ``labels`` have the dtype of ``topk_indices``."""
+    return _topk_distill(0, logits, topk_indices, topk_logits, labels, None, None, temperature, soft_weight, hard_weight,
+                         vocab_size)
+
+
+def topk_distill_dx(dloss: torch.Tensor, logits: torch.Tensor, topk_indices: torch.Tensor, topk_logits: torch.Tensor,
+                    stats: torch.Tensor, temperature: float = 1.0, soft_weight: float = 1.0, labels: torch.Tensor = None,
+                    hard_weight: float = 0.0, vocab_size: int = None) -> torch.Tensor:
+    """Extension op: the gradient of ``topk_distill`` for the logits, in their shape and dtype (zeros
+    in padding columns), from the ``stats`` that a call with the same arguments returned.  ``dloss``:
+    the gradient of the row losses, float32, one for each row or a single one for all."""
+    return _topk_distill(1, logits, topk_indices, topk_logits, labels, dloss, stats, temperature, soft_weight, hard_weight,
+                         vocab_size)[0]
+
+
+def topk_distill_step(logits: torch.Tensor, topk_indices: torch.Tensor, topk_logits: torch.Tensor, dloss: torch.Tensor,
+                      temperature: float = 1.0, soft_weight: float = 1.0, labels: torch.Tensor = None,
+                      hard_weight: float = 0.0, vocab_size: int = None):
+    """Extension op: ``topk_distill`` and ``topk_distill_dx`` in one pass over the logits, for a step
+    that knows ``dloss`` beforehand (1 / rows times the loss scale, say): ``(loss, dlogits)``."""
+    return _topk_distill(2, logits, topk_indices, topk_logits, labels, dloss, None, temperature, soft_weight, hard_weight,
+                         vocab_size)
 
 
 _lans_grad_unscale = 1.0
