@@ -81,31 +81,38 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(const TX* x, const Id
 
 // ------------------------------------------------------------------------------------ gradient
 constexpr int kFewTokens = 256;  // one launch up to here
-constexpr int kDirect = 32;      // tokens a wavefront sums by itself
+constexpr int kDirect = 8;       // tokens of a row that one wavefront sums
 constexpr int kChunk = 64;       // tokens of one partial sum of a longer row
-constexpr int kPerWave = kChunk / kWaves;
+constexpr int kChunkBlock = 512;
+constexpr int kChunkWaves = kChunkBlock / kLanes;
+constexpr int kPerWave = kChunk / kChunkWaves;
 constexpr int kMinTileBits = 11, kMaxTileBits = 14;
-constexpr int kTilesPerRound = kLanes;  // a wavefront looks at this many tiles at once
-constexpr int kMaxRounds = 8;
+constexpr int kMaxTiles = 512;
+constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens have a lane each
 constexpr int kSortBlock = 1024;
-constexpr int kInFlight = 8;  // token rows in flight per lane
+constexpr int kInFlight = 8;  // words in flight per lane
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 struct Layout {
   int tile_bits = 0;
   int tiles = 0;
-  int64_t max_long = 0;   // rows of more than kDirect tokens
-  int64_t max_items = 0;  // chunks of them
+  int bucket_bits = 0;  // log2 of the rows that share an entry of a tile's index
+  int buckets = 0;
+  int64_t max_long = 0;   // rows of more than kChunk tokens
+  int64_t max_items = 0;  // chunks of rows of more than kDirect
+  int64_t max_runs = 0;   // runs of them
   int64_t max_parts = 0;  // chunks of rows with more than one
-  int64_t keys_at = 0, counters_at = 0, rows_at = 0, items_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
+  int64_t keys_at = 0, index_at = 0, counters_at = 0, rows_at = 0, items_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
 };
 
-// A row of more than kDirect tokens: where its runs are listed and what it is cut into.
+// A row of more than kChunk tokens, whose chunks are to be joined, and one chunk of a row of more than
+// kDirect with all that its sum needs to know: where the row's runs are listed and where the
+// partial sums go.
 struct LongRow {
-  uint32_t row, tokens, n_runs, first_run, first_part;
+  uint32_t row, tokens, first_part;
 };
 struct Item {
-  uint32_t long_row, chunk;
+  uint32_t row, tokens, n_runs, first_run, first_part, chunk;
 };
 struct Run {
   uint32_t at, before;  // first key of the run; tokens of the row in earlier runs
@@ -121,14 +128,17 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   while ((1LL << row_bits) <= rows) ++row_bits;
   const int most = 32 - row_bits < kMaxTileBits ? 32 - row_bits : kMaxTileBits;
   int bits = kMinTileBits;
-  while (bits < most && (n >> bits) >= kTilesPerRound) ++bits;
+  while (bits < most && (n >> bits) >= kLanes) ++bits;
   const int64_t tiles = (n + (1LL << bits) - 1) >> bits;
-  if (tiles > kTilesPerRound * kMaxRounds) return false;
+  if (tiles > kMaxTiles) return false;
   l->tile_bits = bits;
   l->tiles = (int)tiles;
-  l->max_long = n / (kDirect + 1);
-  l->max_parts = n / kChunk + n / (kChunk + 1);
-  l->max_items = n / kChunk + l->max_long;
+  // r rows of n tokens together have at most n / kChunk + r chunks.
+  const int64_t listed = n / (kDirect + 1);
+  l->max_long = n / (kChunk + 1);
+  l->max_items = n / kChunk + listed;
+  l->max_runs = n < listed * tiles ? n : listed * tiles;
+  l->max_parts = n / kChunk + l->max_long;
   auto take = [&](int64_t bytes) {
     const int64_t at = l->bytes;
     l->bytes += align256(bytes);
@@ -136,9 +146,15 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   };
   l->counters_at = take(kCounters * 4);
   l->keys_at = take((tiles << bits) * 4);
+  // About one key per entry, or 16 rows where the keys are many: a search then takes a step or two.
+  int bucket = row_bits - bits;
+  if (bucket < 4) bucket = 4;
+  l->bucket_bits = bucket;
+  l->buckets = (int)((rows + (1LL << bucket) - 1) >> bucket);
+  l->index_at = take(tiles * (l->buckets + 1) * 2);
   l->rows_at = take(l->max_long * (int64_t)sizeof(LongRow));
   l->items_at = take(l->max_items * (int64_t)sizeof(Item));
-  l->runs_at = take((n < l->max_long * tiles ? n : l->max_long * tiles) * (int64_t)sizeof(Run));
+  l->runs_at = take(l->max_runs * (int64_t)sizeof(Run));
   l->parts_at = take(l->max_parts * width * 4);
   return true;
 }
@@ -153,80 +169,143 @@ struct Which {
   }
 };
 
-// Sorts one tile in LDS by a bitonic network over (row << tile_bits | position).
-template <typename Id>
+// Sorts one tile by a bitonic network over (row << tile_bits | position), kEach = 2^tile_bits /
+// kSortBlock keys in the registers of each thread: key i sits in register i % kEach of thread
+// i / kEach, so of the 66 stages of 2048 keys 11 stay inside a thread, 45 inside a wavefront and 10
+// go through LDS.  Then the index: for every bucket of rows the first key that is not below it.
+template <typename Id, int kEach>
 __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n, Which which, int tile_bits,
-                                                        uint32_t* keys, uint32_t* counters) {
-  extern __shared__ uint32_t tile[];
-  const int size = 1 << tile_bits;
-  const int64_t t0 = (int64_t)blockIdx.x << tile_bits;
-  if (blockIdx.x == 0 && threadIdx.x < kCounters) counters[threadIdx.x] = 0;
-  for (int i = threadIdx.x; i < size; i += kSortBlock) {
+                                                        int bucket_bits, int buckets, uint32_t* keys, uint16_t* index,
+                                                        uint32_t* counters) {
+  constexpr int kSize = kEach * kSortBlock;
+  __shared__ uint32_t lds[kSize];
+  const int tid = threadIdx.x;
+  const int64_t t0 = (int64_t)blockIdx.x * kSize;
+  if (blockIdx.x == 0 && tid < kCounters) counters[tid] = 0;
+  uint32_t v[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = e * kSortBlock + tid;  // any order will do before the sort
     const int64_t row = t0 + i < n ? which.row((int64_t)ids[t0 + i]) : -1;
-    tile[i] = row >= 0 ? (uint32_t)row << tile_bits | (uint32_t)i : kNoToken;
+    v[e] = row >= 0 ? (uint32_t)row << tile_bits | (uint32_t)i : kNoToken;
+  }
+#pragma unroll 1
+  for (int k = 2; k <= kSize; k <<= 1) {
+    for (int j = k >> 1; j >= kEach * kLanes; j >>= 1) {  // across wavefronts
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) lds[e * kSortBlock + tid] = v[e];
+      __syncthreads();
+      const int other = tid ^ (j / kEach);
+      const bool low = (tid & (j / kEach)) == 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const uint32_t y = lds[e * kSortBlock + other];
+        const bool up = ((tid * kEach + e) & k) == 0;
+        v[e] = low == up ? min(v[e], y) : max(v[e], y);
+      }
+    }
+    for (int j = (k >> 1) < kEach * kLanes ? k >> 1 : kEach * kLanes / 2; j >= kEach; j >>= 1) {  // across lanes
+      const bool low = (tid & (j / kEach)) == 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const uint32_t y = __shfl_xor(v[e], j / kEach, kLanes);
+        const bool up = ((tid * kEach + e) & k) == 0;
+        v[e] = low == up ? min(v[e], y) : max(v[e], y);
+      }
+    }
+#pragma unroll
+    for (int j = kEach / 2; j > 0; j >>= 1) {  // across registers
+      if (j >= k) continue;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (e & j) continue;
+        const bool up = ((tid * kEach + e) & k) == 0;
+        const uint32_t x = v[e], y = v[e | j];
+        v[e] = up ? min(x, y) : max(x, y);
+        v[e | j] = up ? max(x, y) : min(x, y);
+      }
+    }
   }
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += kSortBlock) {
-        const int a = (i & (j - 1)) | (i & ~(j - 1)) << 1, b = a | j;
-        const uint32_t x = tile[a], y = tile[b];
-        const bool up = (a & k) == 0;
-        if ((x > y) == up) {
-          tile[a] = y;
-          tile[b] = x;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) lds[tid * kEach + e] = v[e];
+  __syncthreads();
+  for (int i = tid; i < kSize; i += kSortBlock) keys[t0 + i] = lds[i];
+  for (int b = tid; b <= buckets; b += kSortBlock) {
+    // The last entry lies behind every row; its key may exceed 32 bits.
+    const uint64_t key = (uint64_t)b << (bucket_bits + tile_bits);
+    int at = 0;
+    for (int step = kSize >> 1; step > 0; step >>= 1)
+      if (lds[at + step - 1] < key) at += step;
+    at += lds[at] < key ? 1 : 0;
+    index[(int64_t)blockIdx.x * (buckets + 1) + b] = (uint16_t)at;
+  }
+}
+
+// First index in [lo, hi) of a sorted tile whose key is not below `key`, or hi.
+__device__ __forceinline__ int lower_bound(const uint32_t* tile, int lo, int hi, uint32_t key) {
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (tile[mid] < key)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// A wavefront's share of a row: kSweeps words per lane, 64 words apart, or single columns.
+// Adds `count` tokens, of which lane first + e of `token` holds the e-th; `count` is the same in all
+// lanes.  kInFlight words are requested before the first is needed: of several tokens, or of one token
+// where rows are long and tokens few.
+template <typename TD, int kSweeps>
+__device__ __forceinline__ void add_words(const TD* dy, int64_t width, int64_t word, int64_t words, int token, int count,
+                                          float (&acc)[kSweeps][kWide]) {
+  constexpr int kTokens = kInFlight / kSweeps;
+  for (int e0 = 0; e0 < count; e0 += kTokens) {
+    typename Wide<TD>::Raw raw[kTokens][kSweeps];
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      if (e0 + u < count) {
+        const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
+#pragma unroll
+        for (int s = 0; s < kSweeps; ++s)
+          if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      if (e0 + u < count) {
+#pragma unroll
+        for (int s = 0; s < kSweeps; ++s) {
+          if (word + s * kLanes < words) {
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
+          }
         }
       }
-      __syncthreads();
     }
   }
-  for (int i = threadIdx.x; i < size; i += kSortBlock) keys[t0 + i] = tile[i];
 }
 
-// First index in a sorted tile whose key is not below `key`.
-__device__ __forceinline__ int lower_bound(const uint32_t* tile, int size, uint32_t key) {
-  int at = 0;
-  for (int step = size >> 1; step > 0; step >>= 1)
-    if (tile[at + step - 1] < key) at += step;
-  return at + (tile[at] < key ? 1 : 0);
-}
-
-// Columns [col, col + kCols) of the sum over `count` tokens, of which lane e of `token` holds the
-// e-th; lanes that are not active have no column.  `count` is the same in all lanes.
-template <typename TD, int kCols>
-__device__ __forceinline__ void add_tokens(const TD* dy, int64_t width, int64_t col, bool active, int token, int first,
-                                           int count, float (&acc)[kCols]) {
+template <typename TD>
+__device__ __forceinline__ float add_singles(const TD* dy, int64_t width, int64_t col, int token, int count) {
+  float acc = 0.f;
   for (int e0 = 0; e0 < count; e0 += kInFlight) {
-    if constexpr (kCols == kWide) {
-      typename Wide<TD>::Raw raw[kInFlight];
+    float one[kInFlight];
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u) {
-        if (e0 + u < count) {
-          const int64_t t = __builtin_amdgcn_readlane(token, first + e0 + u);
-          if (active) raw[u] = Wide<TD>::load(dy + t * width + col);
-        }
+    for (int u = 0; u < kInFlight; ++u) {
+      if (e0 + u < count) {
+        const int64_t t = __builtin_amdgcn_readlane(token, e0 + u);
+        if (col < width) one[u] = Wide<TD>::one(dy + t * width + col);
       }
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) {
-        if (e0 + u < count && active) {
-#pragma unroll
-          for (int j = 0; j < kWide; ++j) acc[j] += Wide<TD>::get(raw[u], j);
-        }
-      }
-    } else {
-      float one[kInFlight];
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) {
-        if (e0 + u < count) {
-          const int64_t t = __builtin_amdgcn_readlane(token, first + e0 + u);
-          if (active) one[u] = Wide<TD>::one(dy + t * width + col);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (e0 + u < count && active) acc[0] += one[u];
     }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (e0 + u < count && col < width) acc += one[u];
   }
+  return acc;
 }
 
 // dx = [dx +] scale * acc.
@@ -248,33 +327,26 @@ __device__ __forceinline__ void put_row(TO* at, const float (&acc)[kCols], float
   }
 }
 
-// Calls f(col, active, whole word or single column) so that the wavefront covers `width` columns.
-template <typename F>
-__device__ __forceinline__ void for_columns(int64_t width, F&& f) {
-  const int lane = threadIdx.x & (kLanes - 1);
-  const int64_t words = width / kWide;
-  for (int64_t w = 0; w < words; w += kLanes) f(std::integral_constant<int, kWide>{}, (w + lane) * kWide, w + lane < words);
-  const int64_t rest = words * kWide;
-  if (rest < width) f(std::integral_constant<int, 1>{}, rest + lane, rest + lane < width);
-}
-
+// Sixteen bytes per lane and store, side by side.
 template <typename TO>
 __device__ __forceinline__ void zero_row(TO* at, int64_t width) {
-  for_columns(width, [&](auto cols, int64_t col, bool active) {
-    const float none[decltype(cols)::value] = {};
-    if (active) put_row<TO, decltype(cols)::value>(at + col, none, 0.f, false);
-  });
+  typedef typename Wide<TO>::Sixteen Sixteen;
+  constexpr int kEach = 16 / (int)sizeof(TO);
+  const int lane = threadIdx.x & (kLanes - 1);
+  const int64_t pieces = width / kEach;
+  RAFHIP_GLOBAL Sixteen* out = (RAFHIP_GLOBAL Sixteen*)at;
+  for (int64_t w = lane; w < pieces; w += kLanes) out[w] = Sixteen{};
+  const int64_t col = pieces * kEach + lane;
+  if (col < width) Wide<TO>::put(at + col, 0.f);
 }
 
-// One row whose tokens (at most kLanes) the lanes hold.
-template <typename TD, typename TO>
-__device__ __forceinline__ void sum_row(const TD* dy, int64_t width, int token, int count, float scale, bool accumulate,
-                                        TO* at) {
-  for_columns(width, [&](auto cols, int64_t col, bool active) {
-    float acc[decltype(cols)::value] = {};
-    add_tokens<TD, decltype(cols)::value>(dy, width, col, active, token, 0, count, acc);
-    if (active) put_row<TO, decltype(cols)::value>(at + col, acc, scale, accumulate);
-  });
+// Calls f(sweeps, first word) until the wavefront has covered `words` words, two words per lane at a
+// time where the row has them.
+template <typename F>
+__device__ __forceinline__ void for_words(int64_t words, F&& f) {
+  int64_t w = 0;
+  for (; words - w > kLanes; w += 2 * kLanes) f(std::integral_constant<int, 2>{}, w);
+  if (words > w) f(std::integral_constant<int, 1>{}, w);
 }
 
 // All of the gradient for up to kFewTokens tokens: every wavefront looks through the ids for its rows.
@@ -308,93 +380,103 @@ __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids
       if (!accumulate) zero_row(at, width);
       continue;
     }
-    for_columns(width, [&](auto cols, int64_t col, bool active) {
-      constexpr int kCols = decltype(cols)::value;
-      float acc[kCols] = {};
+    // The set bits in ascending order: lane e learns the position of the e-th.
+    int token[kRounds], count[kRounds];
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k) {
-        // The set bits in ascending order: lane e learns the position of the e-th.
-        const uint64_t m = hits[k];
-        const int count = __popcll(m);
-        if (count == 0) continue;
-        const bool set = m >> lane & 1;
-        const int place = __popcll(m & ((1ull << lane) - 1));
-        // A lane that holds a token sends it to the lane of its rank, the others behind the last.
-        const int token = __builtin_amdgcn_ds_permute((set ? place : count + (lane - place)) * 4, k * kLanes + lane);
-        add_tokens<TD, kCols>(dy, width, col, active, token, 0, count, acc);
+    for (int k = 0; k < kRounds; ++k) {
+      const uint64_t m = hits[k];
+      const bool set = m >> lane & 1;
+      const int place = __popcll(m & ((1ull << lane) - 1));
+      count[k] = __popcll(m);
+      // A lane that holds a token sends it to the lane of its rank, the others behind the last.
+      token[k] = __builtin_amdgcn_ds_permute((set ? place : count[k] + (lane - place)) * 4, k * kLanes + lane);
+    }
+    const int64_t words = width / kWide;
+    for_words(words, [&](auto sweeps, int64_t w) {
+      constexpr int kSweeps = decltype(sweeps)::value;
+      float acc[kSweeps][kWide] = {};
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
+#pragma unroll
+      for (int s = 0; s < kSweeps; ++s) {
+        const int64_t word = w + lane + s * kLanes;
+        if (word < words) put_row<TO, kWide>(at + word * kWide, acc[s], scale, accumulate != 0);
       }
-      if (active) put_row<TO, kCols>(at + col, acc, scale, accumulate != 0);
     });
+    const int64_t col = words * kWide + lane;
+    if (words * kWide < width) {
+      float acc[1] = {};
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) acc[0] += add_singles(dy, width, col, token[k], count[k]);
+      if (col < width) put_row<TO, 1>(at + col, acc, scale, accumulate != 0);
+    }
   }
 }
 
-// Rows of a wavefront: kGroup rows side by side, `spread` lanes (one per tile) each; with more
-// than 64 tiles one row at a time in kRounds rounds.
-template <typename TD, typename TO, int kRounds>
-__global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t* keys, int tiles, int tile_bits,
-                                                   int spread_bits, int group, int64_t rows, int64_t width, float scale,
-                                                   int accumulate, TO* dx, uint32_t* counters, LongRow* long_rows,
-                                                   Item* items, Run* runs) {
+// A wavefront takes kSlots rows.  First it looks them up: kLanes / kSlots lanes for each row share the
+// tiles, kRounds tiles a lane.  Rows without tokens become zeros, long ones are listed, and the
+// tokens of the others -- a lane for each -- are summed in one go, so that the loads of the next row
+// are under way while this one is finished.
+// Its rows lie `stride` apart: neighbours in a vocabulary are often alike in frequency, and a
+// wavefront with eight rows of many tokens would finish long after the rest.
+template <typename TD, typename TO, int kSlots, int kRounds>
+__global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t* keys, const uint16_t* index,
+                                                   int tiles, int tile_bits, int bucket_bits, int buckets, int64_t stride,
+                                                   int64_t rows, int64_t width, float scale, int accumulate, TO* dx,
+                                                   uint32_t* counters, LongRow* long_rows, Item* items, Run* runs) {
+  constexpr int kSpread = kLanes / kSlots;
+  constexpr int kSlotShift = 28;  // a key's place needs 23 bits (kMaxTiles tiles of 2^14), a slot three
+  __shared__ uint32_t places[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
-  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+  const int in_block = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + in_block;
   const int64_t n_waves = (int64_t)gridDim.x * kWaves;
-  const int size = 1 << tile_bits;
-  const int spread = 1 << spread_bits;
-  const int slot = lane >> spread_bits, tile0 = lane & (spread - 1);
-  for (int64_t r0 = wave * group; r0 < rows; r0 += n_waves * group) {
-    const int64_t my_row = r0 + slot;
+  const uint32_t size = 1u << tile_bits;
+  const int slot = lane / kSpread, tile0 = lane % kSpread;
+  const int64_t words = width / kWide;
+  for (int64_t r0 = wave; r0 < stride; r0 += n_waves) {
+    const int64_t my_row = r0 + slot * stride;
     uint32_t at[kRounds];
     int len[kRounds], before[kRounds];
     int total = 0;  // tokens of this lane's row, the same in all its lanes
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
-      const int t = q * kTilesPerRound + tile0;
+      const int t = q * kSpread + tile0;
       at[q] = 0;
       len[q] = 0;
-      if (slot < group && my_row < rows && t < tiles) {
+      if (my_row < rows && t < tiles) {
         const uint32_t* tile = keys + ((int64_t)t << tile_bits);
-        const int lo = lower_bound(tile, size, (uint32_t)my_row << tile_bits);
-        const int hi = lower_bound(tile, size, (uint32_t)(my_row + 1) << tile_bits);
+        const uint16_t* bucket = index + (int64_t)t * (buckets + 1) + (my_row >> bucket_bits);
+        const int end = bucket[1];
+        const int lo = lower_bound(tile, bucket[0], end, (uint32_t)my_row << tile_bits);
+        const int hi = lower_bound(tile, lo, end, (uint32_t)(my_row + 1) << tile_bits);
         at[q] = ((uint32_t)t << tile_bits) + (uint32_t)lo;
         len[q] = hi - lo;
       }
+    }
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
       int sum = len[q];  // inclusive over the row's lanes
-      for (int d = 1; d < spread; d <<= 1) {
-        const int up = __shfl_up(sum, d, spread);
+#pragma unroll
+      for (int d = 1; d < kSpread; d <<= 1) {
+        const int up = __shfl_up(sum, d, kSpread);
         if (tile0 >= d) sum += up;
       }
       before[q] = total + sum - len[q];
-      total += __shfl(sum, spread - 1, spread);
+      total += __shfl(sum, kSpread - 1, kSpread);
     }
-    const int here = (int)(rows - r0 < group ? rows - r0 : group);
-    for (int i = 0; i < here; ++i) {
-      TO* out = dx + (r0 + i) * width;
-      const int count = __builtin_amdgcn_readlane(total, i << spread_bits);
-      if (count == 0) {
-        if (!accumulate) zero_row(out, width);
-        continue;
-      }
-      if (count <= kDirect) {
-        int key_at = 0;  // lane e: where the e-th token's key is
+    int entries = 0, base = 0;  // tokens of the short rows; of those in front of this lane's row
 #pragma unroll
-        for (int q = 0; q < kRounds; ++q) {
-          uint64_t some = __ballot(slot == i && len[q] > 0);
-          while (some) {
-            const int src = __ffsll((unsigned long long)some) - 1;
-            some &= some - 1;
-            const int a = __builtin_amdgcn_readlane((int)at[q], src), b = __builtin_amdgcn_readlane(before[q], src);
-            if (lane >= b) key_at = a + (lane - b);
-          }
-        }
-        int token = 0;
-        if (lane < count) {
-          const uint32_t tile = (uint32_t)key_at >> tile_bits;
-          token = (int)((tile << tile_bits) + (keys[key_at] & (uint32_t)(size - 1)));
-        }
-        sum_row(dy, width, token, count, scale, accumulate != 0, out);
+    for (int i = 0; i < kSlots; ++i) {
+      const int64_t row = r0 + i * stride;
+      if (row >= rows) break;
+      const int count = __builtin_amdgcn_readlane(total, i * kSpread);
+      if (count <= kDirect) {
+        if (count == 0 && !accumulate) zero_row(dx + row * width, width);
+        if (slot == i) base = entries;
+        entries += count;
         continue;
       }
-      // Listed for the next launch.
       int n_runs = 0;
       int place[kRounds];
 #pragma unroll
@@ -404,75 +486,164 @@ __global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t*
         n_runs += __popcll(some);
       }
       const int chunks = (count + kChunk - 1) / kChunk;
-      uint32_t base = 0;
+      uint32_t first = 0;
       if (lane < kCounters)
-        base = atomicAdd(&counters[lane], (uint32_t)(lane == kLongRows ? 1 : lane == kItems ? chunks : lane == kRuns ? n_runs : chunks > 1 ? chunks : 0));
-      const uint32_t id = __builtin_amdgcn_readlane((int)base, kLongRows);
-      const uint32_t first_item = __builtin_amdgcn_readlane((int)base, kItems);
-      const uint32_t first_run = __builtin_amdgcn_readlane((int)base, kRuns);
-      if (lane == 0) {
-        const uint32_t first_part = __builtin_amdgcn_readlane((int)base, kParts);
-        long_rows[id] = LongRow{(uint32_t)(r0 + i), (uint32_t)count, (uint32_t)n_runs, first_run, first_part};
-      }
-      for (int c = lane; c < chunks; c += kLanes) items[first_item + c] = Item{id, (uint32_t)c};
+        first = atomicAdd(&counters[lane],
+                          (uint32_t)(lane == kItems ? chunks : lane == kRuns ? n_runs : chunks == 1 ? 0 : lane == kParts ? chunks : 1));
+      const uint32_t id = __builtin_amdgcn_readlane((int)first, kLongRows);
+      const uint32_t first_item = __builtin_amdgcn_readlane((int)first, kItems);
+      const uint32_t first_run = __builtin_amdgcn_readlane((int)first, kRuns);
+      const uint32_t first_part = __builtin_amdgcn_readlane((int)first, kParts);
+      if (lane == 0 && chunks > 1) long_rows[id] = LongRow{(uint32_t)row, (uint32_t)count, first_part};
+      for (int c = lane; c < chunks; c += kLanes)
+        items[first_item + c] = Item{(uint32_t)row, (uint32_t)count, (uint32_t)n_runs, first_run, first_part, (uint32_t)c};
 #pragma unroll
       for (int q = 0; q < kRounds; ++q)
         if (slot == i && len[q] > 0) runs[first_run + place[q]] = Run{at[q], (uint32_t)before[q]};
     }
+    if (entries == 0) continue;
+    // Lane e gets the e-th token of the short rows, row by row.
+    if (total <= kDirect) {
+#pragma unroll
+      for (int q = 0; q < kRounds; ++q)
+        for (int x = 0; x < len[q]; ++x) places[in_block][base + before[q] + x] = (at[q] + x) | (uint32_t)slot << kSlotShift;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t place = lane < entries ? places[in_block][lane] : 0;
+    const uint32_t key_at = place & ((1u << kSlotShift) - 1);
+    const int of = (int)(place >> kSlotShift);
+    int token = 0;
+    if (lane < entries) token = (int)((key_at >> tile_bits << tile_bits) + (keys[key_at] & (size - 1)));
+    const int next = __shfl_down(of, 1, kLanes);
+    const uint64_t last = __ballot(lane < entries && (lane + 1 == entries || next != of));  // of its row
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for_words(words, [&](auto sweeps, int64_t w) {
+      constexpr int kSweeps = decltype(sweeps)::value;
+      constexpr int kTokens = kInFlight / kSweeps;
+      const int64_t word = w + lane;
+      float acc[kSweeps][kWide] = {};
+      for (int e0 = 0; e0 < entries; e0 += kTokens) {
+        typename Wide<TD>::Raw raw[kTokens][kSweeps];
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u) {
+          if (e0 + u < entries) {
+            const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
+#pragma unroll
+            for (int s = 0; s < kSweeps; ++s)
+              if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u) {
+          if (e0 + u < entries) {
+            const bool done = last >> (e0 + u) & 1;
+            TO* out = dx + (r0 + __builtin_amdgcn_readlane(of, e0 + u) * stride) * width;
+#pragma unroll
+            for (int s = 0; s < kSweeps; ++s) {
+              if (word + s * kLanes < words) {
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
+                if (done) {
+                  put_row<TO, kWide>(out + (word + s * kLanes) * kWide, acc[s], scale, accumulate != 0);
+#pragma unroll
+                  for (int j = 0; j < kWide; ++j) acc[s][j] = 0.f;
+                }
+              }
+            }
+          }
+        }
+      }
+    });
+    const int64_t col = words * kWide + lane;  // columns behind the last whole word
+    if (words * kWide < width) {
+      float acc[1] = {0.f};
+      for (int e = 0; e < entries; ++e) {
+        const int64_t t = __builtin_amdgcn_readlane(token, e);
+        if (col < width) {
+          acc[0] += Wide<TD>::one(dy + t * width + col);
+          if (last >> e & 1) {
+            put_row<TO, 1>(dx + (r0 + __builtin_amdgcn_readlane(of, e) * stride) * width + col, acc, scale, accumulate != 0);
+            acc[0] = 0.f;
+          }
+        }
+      }
+    }
   }
 }
 
-// One chunk of a long row per workgroup: each wavefront sums kPerWave tokens, the four sums are
+// One chunk of a long row per workgroup: each of eight wavefronts sums kPerWave tokens, the sums are
 // added in order, and the result is the row (a row of one chunk) or a partial sum.
 template <typename TD, typename TO>
-__global__ __launch_bounds__(kBlock) void chunk_sums(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
-                                                     float scale, int accumulate, TO* dx, const uint32_t* counters,
-                                                     const LongRow* long_rows, const Item* items, const Run* runs,
-                                                     float* parts) {
-  __shared__ float sums[kWaves][kLanes * kWide];
+__global__ __launch_bounds__(kChunkBlock) void chunk_sums(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
+                                                          float scale, int accumulate, TO* dx, const uint32_t* counters,
+                                                          const Item* items, const Run* runs, float* parts) {
+  constexpr int kSweeps = 1;
+  __shared__ float sums[kChunkWaves][kLanes * kWide];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   const uint32_t n_items = counters[kItems];
+  const int64_t words = width / kWide;
   for (uint32_t it = blockIdx.x; it < n_items; it += gridDim.x) {
     const Item item = items[it];
-    const LongRow row = long_rows[item.long_row];
     const int first = (int)item.chunk * kChunk + wave * kPerWave;
-    int count = (int)row.tokens - first;
+    int count = (int)item.tokens - first;
     count = count < 0 ? 0 : count > kPerWave ? kPerWave : count;
-    int token = 0;
-    if (lane < count) {  // the run that holds this lane's token
-      const Run* r = runs + row.first_run;
-      const uint32_t want = (uint32_t)(first + lane);
-      uint32_t lo = 0, hi = row.n_runs;  // the last run that starts at or before it
-      while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (r[mid].before <= want)
-          lo = mid;
-        else
-          hi = mid;
+    // Where this lane's token is: in the last run that starts at or before it.
+    const uint32_t want = (uint32_t)(first + lane);
+    uint32_t at = 0, before = 0;
+    for (uint32_t r0 = 0; r0 < item.n_runs && count > 0; r0 += kLanes) {
+      Run mine{0, 0xffffffffu};
+      if (r0 + lane < item.n_runs) mine = runs[item.first_run + r0 + lane];
+#pragma unroll
+      for (int e = 0; e < kPerWave; ++e) {
+        const uint64_t started = __ballot(mine.before <= (uint32_t)(first + e));
+        if (started != 0) {
+          const int last = 63 - __clzll((long long)started);
+          const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)mine.at, last);
+          const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)mine.before, last);
+          if (lane == e) {
+            at = a;
+            before = b;
+          }
+        }
       }
-      const uint32_t key_at = r[lo].at + (want - r[lo].before);
+    }
+    int token = 0;
+    if (lane < count) {
+      const uint32_t key_at = at + (want - before);
       token = (int)((key_at >> tile_bits << tile_bits) + (keys[key_at] & ((1u << tile_bits) - 1)));
     }
-    const bool whole = row.tokens <= (uint32_t)kChunk;
-    for_columns(width, [&](auto cols, int64_t col, bool active) {
-      constexpr int kCols = decltype(cols)::value;
-      float acc[kCols] = {};
-      add_tokens<TD, kCols>(dy, width, col, active, token, 0, count, acc);
-      __syncthreads();  // the sums of the previous columns have been read
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) sums[wave][lane * kCols + j] = acc[j];
+    const bool whole = item.tokens <= (uint32_t)kChunk;
+    float* part = parts + ((int64_t)item.first_part + item.chunk) * width;
+    TO* out = dx + (int64_t)item.row * width;
+    // `n` columns from `col` on, each the sum of the wavefronts' in order.
+    auto join = [&](int64_t col, int n) {
       __syncthreads();
-      const int64_t c0 = col - (int64_t)lane * kCols;  // the first column of lane 0
-      const int64_t end = kCols == kWide ? width / kWide * kWide : width;
-      for (int c = threadIdx.x; c < kLanes * kCols && c0 + c < end; c += kBlock) {
-        float total[1] = {((sums[0][c] + sums[1][c]) + sums[2][c]) + sums[3][c]};
+      for (int c = threadIdx.x; c < n; c += kChunkBlock) {
+        float total[1] = {sums[0][c]};
+#pragma unroll
+        for (int k = 1; k < kChunkWaves; ++k) total[0] += sums[k][c];
         if (whole)
-          put_row<TO, 1>(dx + (int64_t)row.row * width + c0 + c, total, scale, accumulate != 0);
+          put_row<TO, 1>(out + col + c, total, scale, accumulate != 0);
         else
-          parts[((int64_t)row.first_part + item.chunk) * width + c0 + c] = total[0];
+          part[col + c] = total[0];
       }
-    });
+      __syncthreads();
+    };
+    for (int64_t w = 0; w < words; w += kLanes) {
+      float acc[kSweeps][kWide] = {};
+      add_words<TD, kSweeps>(dy, width, w + lane, words, token, count, acc);
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) sums[wave][lane * kWide + j] = acc[0][j];
+      const int64_t left = (words - w) * kWide;
+      join(w * kWide, (int)(left < kLanes * kWide ? left : kLanes * kWide));
+    }
+    if (words * kWide < width) {
+      sums[wave][lane] = add_singles(dy, width, words * kWide + lane, token, count);
+      join(words * kWide, (int)(width - words * kWide));
+    }
   }
 }
 
@@ -488,7 +659,6 @@ __global__ __launch_bounds__(kBlock) void chunk_join(int64_t width, float scale,
   const uint32_t n_long = counters[kLongRows];
   for (uint32_t h = blockIdx.y; h < n_long; h += gridDim.y) {
     const LongRow row = long_rows[h];
-    if (row.tokens <= (uint32_t)kChunk) continue;
     const int chunks = (int)((row.tokens + kChunk - 1) / kChunk);
     const int per = (chunks + kWaves - 1) / kWaves;
     const int from = wave * per, to = from + per < chunks ? from + per : chunks;
@@ -531,29 +701,40 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   }
   auto* counters = reinterpret_cast<uint32_t*>(ws + l.counters_at);
   auto* keys = reinterpret_cast<uint32_t*>(ws + l.keys_at);
+  auto* index = reinterpret_cast<uint16_t*>(ws + l.index_at);
   auto* long_rows = reinterpret_cast<LongRow*>(ws + l.rows_at);
   auto* items = reinterpret_cast<Item*>(ws + l.items_at);
   auto* runs = reinterpret_cast<Run*>(ws + l.runs_at);
   auto* parts = reinterpret_cast<float*>(ws + l.parts_at);
-  hipLaunchKernelGGL(tile_sort<Id>, dim3((unsigned)l.tiles), dim3(kSortBlock), (size_t)4 << l.tile_bits, s, ids, n, which,
-                     l.tile_bits, keys, counters);
-  int spread_bits = 0;
-  while (spread_bits < 6 && (1 << spread_bits) < l.tiles) ++spread_bits;
-  int group = kLanes >> spread_bits;
-  if (group > kFewRowsPerWave) group = kFewRowsPerWave;
-  const int64_t waves = (rows + group - 1) / group;
-  int64_t blocks = (waves + kWaves - 1) / kWaves;
-  if (blocks > kMaxRowBlocks) blocks = kMaxRowBlocks;
-  auto rows_go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, s, dy, keys, l.tiles, l.tile_bits, spread_bits,
-                       group, rows, width, scale, accumulate, dx, counters, long_rows, items, runs);
+  auto sort = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)l.tiles), dim3(kSortBlock), 0, s, ids, n, which, l.tile_bits, l.bucket_bits,
+                       l.buckets, keys, index, counters);
   };
-  l.tiles <= kTilesPerRound ? rows_go(row_sums<TD, TO, 1>) : rows_go(row_sums<TD, TO, kMaxRounds>);
+  switch (l.tile_bits) {
+    case 11: sort(tile_sort<Id, 2>); break;
+    case 12: sort(tile_sort<Id, 4>); break;
+    case 13: sort(tile_sort<Id, 8>); break;
+    default: sort(tile_sort<Id, 16>); break;
+  }
+  auto rows_go = [&](auto kernel, int group) {
+    const int64_t waves = (rows + group - 1) / group;
+    int64_t blocks = (waves + kWaves - 1) / kWaves;
+    if (blocks > kMaxRowBlocks) blocks = kMaxRowBlocks;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, s, dy, keys, index, l.tiles, l.tile_bits,
+                       l.bucket_bits, l.buckets, waves, rows, width, scale, accumulate, dx, counters, long_rows, items, runs);
+  };
+  if (l.tiles <= 8)
+    rows_go(row_sums<TD, TO, kGroup, 1>, kGroup);
+  else if (l.tiles <= 32)
+    rows_go(row_sums<TD, TO, kGroup, 4>, kGroup);
+  else if (l.tiles <= 64)
+    rows_go(row_sums<TD, TO, kGroup, 8>, kGroup);
+  else
+    rows_go(row_sums<TD, TO, 1, kMaxTiles / kLanes>, 1);
   const int64_t chunk_blocks = l.max_items < kMaxChunkBlocks ? l.max_items : kMaxChunkBlocks;
-  hipLaunchKernelGGL((chunk_sums<TD, TO>), dim3((unsigned)chunk_blocks), dim3(kBlock), 0, s, dy, keys, l.tile_bits, width,
-                     scale, accumulate, dx, counters, long_rows, items, runs, parts);
-  const int64_t most = n / (kChunk + 1);
-  hipLaunchKernelGGL(chunk_join<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(most < 64 ? most : 64)),
+  hipLaunchKernelGGL((chunk_sums<TD, TO>), dim3((unsigned)chunk_blocks), dim3(kChunkBlock), 0, s, dy, keys, l.tile_bits,
+                     width, scale, accumulate, dx, counters, items, runs, parts);
+  hipLaunchKernelGGL(chunk_join<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_long < 64 ? l.max_long : 64)),
                      dim3(kBlock), 0, s, width, scale, accumulate, dx, counters, long_rows, parts);
 }
 

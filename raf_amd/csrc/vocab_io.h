@@ -28,6 +28,7 @@ struct Wide;
 
 template <>
 struct Wide<float> {
+  typedef f32x4_any Sixteen;  // what sixteen bytes hold
   struct Raw {
     f32x4 a, b;
   };
@@ -50,6 +51,7 @@ struct Wide<float> {
 
 template <>
 struct Wide<_Float16> {
+  typedef f16x8_any Sixteen;
   typedef f16x8 Raw;
   static __device__ __forceinline__ Raw load(const _Float16* p) { return *(const RAFHIP_GLOBAL f16x8_any*)p; }
   static __device__ __forceinline__ Raw fill(float x) {
@@ -70,6 +72,7 @@ struct Wide<_Float16> {
 
 template <>
 struct Wide<Bf16> {
+  typedef u16x8_any Sixteen;
   typedef u16x8 Raw;
   static __device__ __forceinline__ Raw load(const Bf16* p) { return *(const RAFHIP_GLOBAL u16x8_any*)p; }
   static __device__ __forceinline__ Raw fill(float x) {
