@@ -5,13 +5,13 @@
 //
 // Gradient: dx[r] = scale * sum over the tokens of row r of dy[t].  A sum by floating-point atomics
 // would depend on the order in which they arrive, so tokens are sorted by row first:
-//   1. tile_sort   sorts each tile of tokens by (row, position) in LDS;
-//   2. row_sums    one wavefront per few rows looks its rows up in all sorted tiles at once (a
-//                  binary search per lane and tile), writes zeros for rows without tokens, sums rows
-//                  of up to kDirect tokens, and lists the others;
-//   3. chunk_sums  sums the listed rows in chunks of kChunk tokens, a workgroup each, so that a
-//                  token that fills half the batch is spread over the GPU;
-//   4. chunk_join  adds the chunks of a row in order.
+//   1. tile_sort   sorts each tile of tokens by (row, position);
+//   2. find_rows   looks every row up in all sorted tiles at once (a binary search per lane and
+//                  tile), writes zeros for rows without tokens, and lists the others: the tokens of
+//                  rows of up to kDirect, and chunks of kChunk tokens of longer rows;
+//   3. sum_rows    sums what is listed, a chunk per workgroup and the short rows by wavefronts, so
+//                  that a token that fills half the batch is spread over the GPU;
+//   4. join_chunks adds the chunks of a row in order.
 // Runs of a row are visited in tile order and sorted inside a tile, so every sum runs over
 // ascending positions cut at multiples of kChunk: the result depends on the data alone although
 // the list of long rows is filled in the order in which wavefronts arrive.  Up to kFewTokens
@@ -92,32 +92,38 @@ constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens h
 constexpr int kSortBlock = 1024;
 constexpr int kInFlight = 8;  // words in flight per lane
 constexpr uint32_t kNoToken = 0xffffffffu;
+constexpr int kSlotShift = 28;  // an entry: a token (23 bits: kMaxTiles tiles of 2^14) and its row's slot
 
 struct Layout {
   int tile_bits = 0;
   int tiles = 0;
   int bucket_bits = 0;  // log2 of the rows that share an entry of a tile's index
   int buckets = 0;
-  int64_t max_long = 0;   // rows of more than kChunk tokens
-  int64_t max_items = 0;  // chunks of rows of more than kDirect
+  int64_t max_singles = 0;  // rows of more than kDirect tokens and no more than a chunk
   int64_t max_runs = 0;   // runs of them
   int64_t max_parts = 0;  // chunks of rows with more than one
-  int64_t keys_at = 0, index_at = 0, counters_at = 0, rows_at = 0, items_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
+  int64_t keys_at = 0, index_at = 0, taken_at = 0, entries_at = 0, counts_at = 0, singles_at = 0, items_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
 };
 
-// A row of more than kChunk tokens, whose chunks are to be joined, and one chunk of a row of more than
-// kDirect with all that its sum needs to know: where the row's runs are listed and where the
-// partial sums go.
-struct LongRow {
-  uint32_t row, tokens, first_part;
-};
+// One chunk of a row of more than kDirect tokens, with all that its sum needs to know.  There are two
+// lists: rows of one chunk, and the chunks of the others, whose place there is that of their
+// partial sum.
 struct Item {
-  uint32_t row, tokens, n_runs, first_run, first_part, chunk;
+  uint32_t row, tokens, n_runs, first_run, chunk;
 };
 struct Run {
   uint32_t at, before;  // first key of the run; tokens of the row in earlier runs
 };
-enum { kLongRows = 0, kItems, kRuns, kParts, kCounters };
+// How much of each list is taken, in one word: a wavefront reserves all it needs with one atomic
+// (with four, 800 wavefronts queued for some 60 us).
+typedef unsigned long long Taken;
+constexpr int kRunBits = 24, kSingleBits = 21;  // up to 2^23 runs, 2^20 rows of one chunk, 2^18 chunks
+__device__ __forceinline__ Taken take(uint32_t runs, uint32_t chunks) {
+  return (Taken)runs | (chunks == 1 ? (Taken)1 << kRunBits : (Taken)chunks << (kRunBits + kSingleBits));
+}
+__device__ __forceinline__ uint32_t runs_of(Taken t) { return (uint32_t)t & ((1u << kRunBits) - 1); }
+__device__ __forceinline__ uint32_t singles_of(Taken t) { return (uint32_t)(t >> kRunBits) & ((1u << kSingleBits) - 1); }
+__device__ __forceinline__ uint32_t parts_of(Taken t) { return (uint32_t)(t >> (kRunBits + kSingleBits)); }
 
 inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
@@ -135,27 +141,28 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   l->tiles = (int)tiles;
   // r rows of n tokens together have at most n / kChunk + r chunks.
   const int64_t listed = n / (kDirect + 1);
-  l->max_long = n / (kChunk + 1);
-  l->max_items = n / kChunk + listed;
+  l->max_singles = listed;
   l->max_runs = n < listed * tiles ? n : listed * tiles;
-  l->max_parts = n / kChunk + l->max_long;
-  auto take = [&](int64_t bytes) {
+  l->max_parts = n / kChunk + n / (kChunk + 1);
+  auto place = [&](int64_t bytes) {
     const int64_t at = l->bytes;
     l->bytes += align256(bytes);
     return at;
   };
-  l->counters_at = take(kCounters * 4);
-  l->keys_at = take((tiles << bits) * 4);
+  l->taken_at = place(sizeof(Taken));
+  l->keys_at = place((tiles << bits) * 4);
   // About one key per entry, or 16 rows where the keys are many: a search then takes a step or two.
   int bucket = row_bits - bits;
   if (bucket < 4) bucket = 4;
   l->bucket_bits = bucket;
   l->buckets = (int)((rows + (1LL << bucket) - 1) >> bucket);
-  l->index_at = take(tiles * (l->buckets + 1) * 2);
-  l->rows_at = take(l->max_long * (int64_t)sizeof(LongRow));
-  l->items_at = take(l->max_items * (int64_t)sizeof(Item));
-  l->runs_at = take(l->max_runs * (int64_t)sizeof(Run));
-  l->parts_at = take(l->max_parts * width * 4);
+  l->index_at = place(tiles * (l->buckets + 1) * 2);
+  l->entries_at = place((rows + kGroup) * kDirect * 4);
+  l->counts_at = place(rows * 4);
+  l->singles_at = place(l->max_singles * (int64_t)sizeof(Item));
+  l->items_at = place(l->max_parts * (int64_t)sizeof(Item));
+  l->runs_at = place(l->max_runs * (int64_t)sizeof(Run));
+  l->parts_at = place(l->max_parts * width * 4);
   return true;
 }
 
@@ -176,12 +183,12 @@ struct Which {
 template <typename Id, int kEach>
 __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n, Which which, int tile_bits,
                                                         int bucket_bits, int buckets, uint32_t* keys, uint16_t* index,
-                                                        uint32_t* counters) {
+                                                        Taken* taken) {
   constexpr int kSize = kEach * kSortBlock;
   __shared__ uint32_t lds[kSize];
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * kSize;
-  if (blockIdx.x == 0 && tid < kCounters) counters[tid] = 0;
+  if (blockIdx.x == 0 && tid == 0) *taken = 0;
   uint32_t v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
@@ -241,18 +248,6 @@ __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n
     at += lds[at] < key ? 1 : 0;
     index[(int64_t)blockIdx.x * (buckets + 1) + b] = (uint16_t)at;
   }
-}
-
-// First index in [lo, hi) of a sorted tile whose key is not below `key`, or hi.
-__device__ __forceinline__ int lower_bound(const uint32_t* tile, int lo, int hi, uint32_t key) {
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (tile[mid] < key)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
 }
 
 // A wavefront's share of a row: kSweeps words per lane, 64 words apart, or single columns.
@@ -413,19 +408,17 @@ __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids
   }
 }
 
-// A wavefront takes kSlots rows.  First it looks them up: kLanes / kSlots lanes for each row share the
-// tiles, kRounds tiles a lane.  Rows without tokens become zeros, long ones are listed, and the
-// tokens of the others -- a lane for each -- are summed in one go, so that the loads of the next row
-// are under way while this one is finished.
+// A wavefront takes kSlots rows.  kLanes / kSlots lanes for each row share the tiles, kRounds tiles a
+// lane.  Rows without tokens become zeros, long ones are listed, and the tokens of the others go
+// to the wavefront's own stretch of `entries`, row by row, kDirect of them for each row at most.
 // Its rows lie `stride` apart: neighbours in a vocabulary are often alike in frequency, and a
 // wavefront with eight rows of many tokens would finish long after the rest.
-template <typename TD, typename TO, int kSlots, int kRounds>
-__global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t* keys, const uint16_t* index,
-                                                   int tiles, int tile_bits, int bucket_bits, int buckets, int64_t stride,
-                                                   int64_t rows, int64_t width, float scale, int accumulate, TO* dx,
-                                                   uint32_t* counters, LongRow* long_rows, Item* items, Run* runs) {
+template <typename TO, int kSlots, int kRounds>
+__global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const uint16_t* index, int tiles, int tile_bits,
+                                                    int bucket_bits, int buckets, int64_t stride, int64_t rows,
+                                                    int64_t width, int accumulate, TO* dx, Taken* taken, uint32_t* entries_out,
+                                                    uint32_t* counts, Item* singles, Item* items, Run* runs) {
   constexpr int kSpread = kLanes / kSlots;
-  constexpr int kSlotShift = 28;  // a key's place needs 23 bits (kMaxTiles tiles of 2^14), a slot three
   __shared__ uint32_t places[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
   const int in_block = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
@@ -433,26 +426,53 @@ __global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t*
   const int64_t n_waves = (int64_t)gridDim.x * kWaves;
   const uint32_t size = 1u << tile_bits;
   const int slot = lane / kSpread, tile0 = lane % kSpread;
-  const int64_t words = width / kWide;
   for (int64_t r0 = wave; r0 < stride; r0 += n_waves) {
     const int64_t my_row = r0 + slot * stride;
     uint32_t at[kRounds];
     int len[kRounds], before[kRounds];
     int total = 0;  // tokens of this lane's row, the same in all its lanes
+    // Both ends of the row's run in each tile, by binary search in its bucket; the searches of a lane
+    // go on side by side.
+    uint32_t lo[kRounds], lo_end[kRounds], hi[kRounds], hi_end[kRounds];
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
       const int t = q * kSpread + tile0;
-      at[q] = 0;
-      len[q] = 0;
+      lo[q] = lo_end[q] = 0;
       if (my_row < rows && t < tiles) {
-        const uint32_t* tile = keys + ((int64_t)t << tile_bits);
         const uint16_t* bucket = index + (int64_t)t * (buckets + 1) + (my_row >> bucket_bits);
-        const int end = bucket[1];
-        const int lo = lower_bound(tile, bucket[0], end, (uint32_t)my_row << tile_bits);
-        const int hi = lower_bound(tile, lo, end, (uint32_t)(my_row + 1) << tile_bits);
-        at[q] = ((uint32_t)t << tile_bits) + (uint32_t)lo;
-        len[q] = hi - lo;
+        lo[q] = bucket[0];
+        lo_end[q] = bucket[1];
       }
+      hi[q] = lo[q];
+      hi_end[q] = lo_end[q];
+    }
+    const uint32_t lo_key = (uint32_t)my_row << tile_bits, hi_key = (uint32_t)(my_row + 1) << tile_bits;
+    for (bool more = true; more;) {
+      more = false;
+#pragma unroll
+      for (int q = 0; q < kRounds; ++q) {
+        const uint32_t* tile = keys + ((int64_t)(q * kSpread + tile0) << tile_bits);
+        const uint32_t a = (lo[q] + lo_end[q]) >> 1, b = (hi[q] + hi_end[q]) >> 1;
+        const uint32_t x = lo[q] < lo_end[q] ? tile[a] : 0, y = hi[q] < hi_end[q] ? tile[b] : 0;
+        if (lo[q] < lo_end[q]) {
+          if (x < lo_key)
+            lo[q] = a + 1;
+          else
+            lo_end[q] = a;
+        }
+        if (hi[q] < hi_end[q]) {
+          if (y < hi_key)
+            hi[q] = b + 1;
+          else
+            hi_end[q] = b;
+        }
+        more |= lo[q] < lo_end[q] || hi[q] < hi_end[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
+      at[q] = ((uint32_t)(q * kSpread + tile0) << tile_bits) + lo[q];
+      len[q] = (int)(hi[q] - lo[q]);
     }
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
@@ -466,6 +486,7 @@ __global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t*
       total += __shfl(sum, kSpread - 1, kSpread);
     }
     int entries = 0, base = 0;  // tokens of the short rows; of those in front of this lane's row
+    Taken want = 0;             // by the long ones
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
       const int64_t row = r0 + i * stride;
@@ -478,31 +499,41 @@ __global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t*
         continue;
       }
       int n_runs = 0;
-      int place[kRounds];
 #pragma unroll
-      for (int q = 0; q < kRounds; ++q) {
-        const uint64_t some = __ballot(slot == i && len[q] > 0);
-        place[q] = n_runs + __popcll(some & ((1ull << lane) - 1));
-        n_runs += __popcll(some);
-      }
+      for (int q = 0; q < kRounds; ++q) n_runs += __popcll(__ballot(slot == i && len[q] > 0));
       const int chunks = (count + kChunk - 1) / kChunk;
-      uint32_t first = 0;
-      if (lane < kCounters)
-        first = atomicAdd(&counters[lane],
-                          (uint32_t)(lane == kItems ? chunks : lane == kRuns ? n_runs : chunks == 1 ? 0 : lane == kParts ? chunks : 1));
-      const uint32_t id = __builtin_amdgcn_readlane((int)first, kLongRows);
-      const uint32_t first_item = __builtin_amdgcn_readlane((int)first, kItems);
-      const uint32_t first_run = __builtin_amdgcn_readlane((int)first, kRuns);
-      const uint32_t first_part = __builtin_amdgcn_readlane((int)first, kParts);
-      if (lane == 0 && chunks > 1) long_rows[id] = LongRow{(uint32_t)row, (uint32_t)count, first_part};
-      for (int c = lane; c < chunks; c += kLanes)
-        items[first_item + c] = Item{(uint32_t)row, (uint32_t)count, (uint32_t)n_runs, first_run, first_part, (uint32_t)c};
-#pragma unroll
-      for (int q = 0; q < kRounds; ++q)
-        if (slot == i && len[q] > 0) runs[first_run + place[q]] = Run{at[q], (uint32_t)before[q]};
+      want += take(n_runs, chunks);
     }
+    if (want != 0) {
+      Taken first = 0;
+      if (lane == 0) first = atomicAdd(taken, want);
+      first = (Taken)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)first) |
+              (Taken)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(first >> 32)) << 32;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        const int64_t row = r0 + i * stride;
+        if (row >= rows) break;
+        const int count = __builtin_amdgcn_readlane(total, i * kSpread);
+        if (count <= kDirect) continue;
+        const uint32_t first_run = runs_of(first);
+        int n_runs = 0;
+#pragma unroll
+        for (int q = 0; q < kRounds; ++q) {
+          const uint64_t some = __ballot(slot == i && len[q] > 0);
+          if (slot == i && len[q] > 0)
+            runs[first_run + n_runs + __popcll(some & ((1ull << lane) - 1))] = Run{at[q], (uint32_t)before[q]};
+          n_runs += __popcll(some);
+        }
+        const int chunks = (count + kChunk - 1) / kChunk;
+        Item* list = chunks == 1 ? singles + singles_of(first) : items + parts_of(first);
+        for (int c = lane; c < chunks; c += kLanes)
+          list[c] = Item{(uint32_t)row, (uint32_t)count, (uint32_t)n_runs, first_run, (uint32_t)c};
+        first += take(n_runs, chunks);
+      }
+    }
+    if (lane == 0) counts[r0] = (uint32_t)entries;
     if (entries == 0) continue;
-    // Lane e gets the e-th token of the short rows, row by row.
+    // Lane e gets the e-th token of the short rows.
     if (total <= kDirect) {
 #pragma unroll
       for (int q = 0; q < kRounds; ++q)
@@ -510,83 +541,107 @@ __global__ __launch_bounds__(kBlock) void row_sums(const TD* dy, const uint32_t*
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const uint32_t place = lane < entries ? places[in_block][lane] : 0;
-    const uint32_t key_at = place & ((1u << kSlotShift) - 1);
-    const int of = (int)(place >> kSlotShift);
-    int token = 0;
-    if (lane < entries) token = (int)((key_at >> tile_bits << tile_bits) + (keys[key_at] & (size - 1)));
-    const int next = __shfl_down(of, 1, kLanes);
-    const uint64_t last = __ballot(lane < entries && (lane + 1 == entries || next != of));  // of its row
+    if (lane < entries) {
+      const uint32_t place = places[in_block][lane], key_at = place & ((1u << kSlotShift) - 1);
+      const uint32_t token = (key_at >> tile_bits << tile_bits) + (keys[key_at] & (size - 1));
+      entries_out[r0 * (kSlots * kDirect) + lane] = token | (place >> kSlotShift << kSlotShift);
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    for_words(words, [&](auto sweeps, int64_t w) {
-      constexpr int kSweeps = decltype(sweeps)::value;
-      constexpr int kTokens = kInFlight / kSweeps;
-      const int64_t word = w + lane;
-      float acc[kSweeps][kWide] = {};
-      for (int e0 = 0; e0 < entries; e0 += kTokens) {
-        typename Wide<TD>::Raw raw[kTokens][kSweeps];
+  }
+}
+
+// The short rows of one wavefront of find_rows: `entries` tokens, one per lane, in one go, so that the
+// loads of the next row are under way while this one is finished.
+template <typename TD, typename TO>
+__device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, uint32_t entry, int entries, int64_t r0,
+                                               int64_t stride, float scale, bool accumulate, TO* dx) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  const int64_t words = width / kWide;
+  const int token = (int)(entry & ((1u << kSlotShift) - 1)), of = (int)(entry >> kSlotShift);
+  const int next = __shfl_down(of, 1, kLanes);
+  const uint64_t last = __ballot(lane < entries && (lane + 1 == entries || next != of));  // of its row
+  for_words(words, [&](auto sweeps, int64_t w) {
+    constexpr int kSweeps = decltype(sweeps)::value;
+    constexpr int kTokens = kInFlight / kSweeps;
+    const int64_t word = w + lane;
+    float acc[kSweeps][kWide] = {};
+    for (int e0 = 0; e0 < entries; e0 += kTokens) {
+      typename Wide<TD>::Raw raw[kTokens][kSweeps];
 #pragma unroll
-        for (int u = 0; u < kTokens; ++u) {
-          if (e0 + u < entries) {
-            const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
+      for (int u = 0; u < kTokens; ++u) {
+        if (e0 + u < entries) {
+          const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
 #pragma unroll
-            for (int s = 0; s < kSweeps; ++s)
-              if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
-          }
+          for (int s = 0; s < kSweeps; ++s)
+            if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
         }
+      }
 #pragma unroll
-        for (int u = 0; u < kTokens; ++u) {
-          if (e0 + u < entries) {
-            const bool done = last >> (e0 + u) & 1;
-            TO* out = dx + (r0 + __builtin_amdgcn_readlane(of, e0 + u) * stride) * width;
+      for (int u = 0; u < kTokens; ++u) {
+        if (e0 + u < entries) {
+          const bool done = last >> (e0 + u) & 1;
+          TO* out = dx + (r0 + __builtin_amdgcn_readlane(of, e0 + u) * stride) * width;
 #pragma unroll
-            for (int s = 0; s < kSweeps; ++s) {
-              if (word + s * kLanes < words) {
+          for (int s = 0; s < kSweeps; ++s) {
+            if (word + s * kLanes < words) {
 #pragma unroll
-                for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
-                if (done) {
-                  put_row<TO, kWide>(out + (word + s * kLanes) * kWide, acc[s], scale, accumulate != 0);
+              for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
+              if (done) {
+                put_row<TO, kWide>(out + (word + s * kLanes) * kWide, acc[s], scale, accumulate);
 #pragma unroll
-                  for (int j = 0; j < kWide; ++j) acc[s][j] = 0.f;
-                }
+                for (int j = 0; j < kWide; ++j) acc[s][j] = 0.f;
               }
             }
           }
         }
       }
-    });
-    const int64_t col = words * kWide + lane;  // columns behind the last whole word
-    if (words * kWide < width) {
-      float acc[1] = {0.f};
-      for (int e = 0; e < entries; ++e) {
-        const int64_t t = __builtin_amdgcn_readlane(token, e);
-        if (col < width) {
-          acc[0] += Wide<TD>::one(dy + t * width + col);
-          if (last >> e & 1) {
-            put_row<TO, 1>(dx + (r0 + __builtin_amdgcn_readlane(of, e) * stride) * width + col, acc, scale, accumulate != 0);
-            acc[0] = 0.f;
-          }
+    }
+  });
+  const int64_t col = words * kWide + lane;  // columns behind the last whole word
+  if (words * kWide < width) {
+    float acc[1] = {0.f};
+    for (int e = 0; e < entries; ++e) {
+      const int64_t t = __builtin_amdgcn_readlane(token, e);
+      const int64_t row = r0 + __builtin_amdgcn_readlane(of, e) * stride;
+      if (col < width) {
+        acc[0] += Wide<TD>::one(dy + t * width + col);
+        if (last >> e & 1) {
+          put_row<TO, 1>(dx + row * width + col, acc, scale, accumulate);
+          acc[0] = 0.f;
         }
       }
     }
   }
 }
 
-// One chunk of a long row per workgroup: each of eight wavefronts sums kPerWave tokens, the sums are
-// added in order, and the result is the row (a row of one chunk) or a partial sum.
+// The first chunk_blocks workgroups take the chunks, one after the other: each of eight wavefronts sums
+// kPerWave tokens, the sums are added in order, and the result is the row (a row of one chunk) or a
+// partial sum.  The others take the short rows.
 template <typename TD, typename TO>
-__global__ __launch_bounds__(kChunkBlock) void chunk_sums(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
-                                                          float scale, int accumulate, TO* dx, const uint32_t* counters,
-                                                          const Item* items, const Run* runs, float* parts) {
+__global__ __launch_bounds__(kChunkBlock) void sum_rows(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
+                                                        float scale, int accumulate, TO* dx, const Taken* taken,
+                                                        const uint32_t* entries, const uint32_t* counts, int64_t stride,
+                                                        int per_wave, const Item* singles, const Item* items,
+                                                        const Run* runs, float* parts, unsigned chunk_blocks) {
   constexpr int kSweeps = 1;
   __shared__ float sums[kChunkWaves][kLanes * kWide];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-  const uint32_t n_items = counters[kItems];
+  if (blockIdx.x >= chunk_blocks) {
+    const int64_t n_waves = (int64_t)(gridDim.x - chunk_blocks) * kChunkWaves;
+    for (int64_t r0 = (int64_t)(blockIdx.x - chunk_blocks) * kChunkWaves + wave; r0 < stride; r0 += n_waves) {
+      const int count = __builtin_amdgcn_readfirstlane((int)counts[r0]);
+      const uint32_t entry = lane < per_wave ? entries[r0 * per_wave + lane] : 0;  // what lies behind the last is not used
+      if (count > 0) sum_short_rows(dy, width, entry, count, r0, stride, scale, accumulate != 0, dx);
+    }
+    return;
+  }
+  const Taken listed = *taken;
+  const uint32_t n_parts = parts_of(listed), n_items = n_parts + singles_of(listed);
   const int64_t words = width / kWide;
-  for (uint32_t it = blockIdx.x; it < n_items; it += gridDim.x) {
-    const Item item = items[it];
+  for (uint32_t it = blockIdx.x; it < n_items; it += chunk_blocks) {
+    const Item item = it < n_parts ? items[it] : singles[it - n_parts];
     const int first = (int)item.chunk * kChunk + wave * kPerWave;
     int count = (int)item.tokens - first;
     count = count < 0 ? 0 : count > kPerWave ? kPerWave : count;
@@ -615,8 +670,8 @@ __global__ __launch_bounds__(kChunkBlock) void chunk_sums(const TD* dy, const ui
       const uint32_t key_at = at + (want - before);
       token = (int)((key_at >> tile_bits << tile_bits) + (keys[key_at] & ((1u << tile_bits) - 1)));
     }
-    const bool whole = item.tokens <= (uint32_t)kChunk;
-    float* part = parts + ((int64_t)item.first_part + item.chunk) * width;
+    const bool whole = it >= n_parts;
+    float* part = parts + (int64_t)it * width;
     TO* out = dx + (int64_t)item.row * width;
     // `n` columns from `col` on, each the sum of the wavefronts' in order.
     auto join = [&](int64_t col, int n) {
@@ -649,22 +704,22 @@ __global__ __launch_bounds__(kChunkBlock) void chunk_sums(const TD* dy, const ui
 
 // The chunks of a long row added in order: 64 columns per workgroup, four stretches of chunks.
 template <typename TO>
-__global__ __launch_bounds__(kBlock) void chunk_join(int64_t width, float scale, int accumulate, TO* dx,
-                                                     const uint32_t* counters, const LongRow* long_rows,
-                                                     const float* parts) {
+__global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale, int accumulate, TO* dx,
+                                                     const Taken* taken, const Item* items, const float* parts) {
   __shared__ float sums[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   const int64_t col = (int64_t)blockIdx.x * kLanes + lane;
-  const uint32_t n_long = counters[kLongRows];
-  for (uint32_t h = blockIdx.y; h < n_long; h += gridDim.y) {
-    const LongRow row = long_rows[h];
+  const uint32_t n_parts = parts_of(*taken);
+  for (uint32_t it = blockIdx.y; it < n_parts; it += gridDim.y) {
+    const Item row = items[it];
+    if (row.chunk != 0) continue;  // the first chunk stands for its row
     const int chunks = (int)((row.tokens + kChunk - 1) / kChunk);
     const int per = (chunks + kWaves - 1) / kWaves;
     const int from = wave * per, to = from + per < chunks ? from + per : chunks;
     float acc = 0.f;
     if (col < width) {
-      const float* p = parts + (int64_t)row.first_part * width + col;
+      const float* p = parts + (int64_t)it * width + col;
       for (int c0 = from; c0 < to; c0 += kInFlight) {
         float v[kInFlight];
 #pragma unroll
@@ -686,8 +741,8 @@ __global__ __launch_bounds__(kBlock) void chunk_join(int64_t width, float scale,
 }
 
 constexpr int kFewRowsPerWave = 8;
-constexpr int64_t kMaxRowBlocks = 2048;   // workgroups of row_sums: eight per CU, each strides over rows
-constexpr int64_t kMaxChunkBlocks = 2048;
+constexpr int64_t kMaxFindBlocks = 2048;  // eight per CU; a launch of more would only take longer to start
+constexpr int64_t kMaxSumBlocks = 1024;   // four of twice the size
 
 template <typename TD, typename TO, typename Id>
 void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64_t width, float scale, int accumulate,
@@ -699,16 +754,18 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
                        (int)n, which, width, scale, accumulate, kFewRowsPerWave, dx);
     return;
   }
-  auto* counters = reinterpret_cast<uint32_t*>(ws + l.counters_at);
+  auto* taken = reinterpret_cast<Taken*>(ws + l.taken_at);
   auto* keys = reinterpret_cast<uint32_t*>(ws + l.keys_at);
   auto* index = reinterpret_cast<uint16_t*>(ws + l.index_at);
-  auto* long_rows = reinterpret_cast<LongRow*>(ws + l.rows_at);
+  auto* entries = reinterpret_cast<uint32_t*>(ws + l.entries_at);
+  auto* counts = reinterpret_cast<uint32_t*>(ws + l.counts_at);
+  auto* singles = reinterpret_cast<Item*>(ws + l.singles_at);
   auto* items = reinterpret_cast<Item*>(ws + l.items_at);
   auto* runs = reinterpret_cast<Run*>(ws + l.runs_at);
   auto* parts = reinterpret_cast<float*>(ws + l.parts_at);
   auto sort = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)l.tiles), dim3(kSortBlock), 0, s, ids, n, which, l.tile_bits, l.bucket_bits,
-                       l.buckets, keys, index, counters);
+                       l.buckets, keys, index, taken);
   };
   switch (l.tile_bits) {
     case 11: sort(tile_sort<Id, 2>); break;
@@ -716,26 +773,30 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
     case 13: sort(tile_sort<Id, 8>); break;
     default: sort(tile_sort<Id, 16>); break;
   }
-  auto rows_go = [&](auto kernel, int group) {
-    const int64_t waves = (rows + group - 1) / group;
-    int64_t blocks = (waves + kWaves - 1) / kWaves;
-    if (blocks > kMaxRowBlocks) blocks = kMaxRowBlocks;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kBlock), 0, s, dy, keys, index, l.tiles, l.tile_bits,
-                       l.bucket_bits, l.buckets, waves, rows, width, scale, accumulate, dx, counters, long_rows, items, runs);
+  const int group = l.tiles <= kLanes ? kGroup : 1;
+  const int64_t waves = (rows + group - 1) / group;  // of find_rows, and the distance of a wavefront's rows
+  const int64_t max_blocks = (waves + kWaves - 1) / kWaves;
+  const unsigned find_blocks = (unsigned)(max_blocks < kMaxFindBlocks ? max_blocks : kMaxFindBlocks);
+  auto find = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(find_blocks), dim3(kBlock), 0, s, keys, index, l.tiles, l.tile_bits, l.bucket_bits,
+                       l.buckets, waves, rows, width, accumulate, dx, taken, entries, counts, singles, items, runs);
   };
   if (l.tiles <= 8)
-    rows_go(row_sums<TD, TO, kGroup, 1>, kGroup);
+    find(find_rows<TO, kGroup, 1>);
   else if (l.tiles <= 32)
-    rows_go(row_sums<TD, TO, kGroup, 4>, kGroup);
-  else if (l.tiles <= 64)
-    rows_go(row_sums<TD, TO, kGroup, 8>, kGroup);
+    find(find_rows<TO, kGroup, 4>);
+  else if (l.tiles <= kLanes)
+    find(find_rows<TO, kGroup, 8>);
   else
-    rows_go(row_sums<TD, TO, 1, kMaxTiles / kLanes>, 1);
-  const int64_t chunk_blocks = l.max_items < kMaxChunkBlocks ? l.max_items : kMaxChunkBlocks;
-  hipLaunchKernelGGL((chunk_sums<TD, TO>), dim3((unsigned)chunk_blocks), dim3(kChunkBlock), 0, s, dy, keys, l.tile_bits,
-                     width, scale, accumulate, dx, counters, items, runs, parts);
-  hipLaunchKernelGGL(chunk_join<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_long < 64 ? l.max_long : 64)),
-                     dim3(kBlock), 0, s, width, scale, accumulate, dx, counters, long_rows, parts);
+    find(find_rows<TO, 1, kMaxTiles / kLanes>);
+  const int64_t max_items = l.max_singles + l.max_parts, max_short = (waves + kChunkWaves - 1) / kChunkWaves;
+  const unsigned chunk_blocks = (unsigned)(max_items < kMaxSumBlocks ? max_items : kMaxSumBlocks);
+  const unsigned short_blocks = (unsigned)(max_short < kMaxSumBlocks ? max_short : kMaxSumBlocks);
+  hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kChunkBlock), 0, s, dy, keys, l.tile_bits,
+                     width, scale, accumulate, dx, taken, entries, counts, waves, group * kDirect, singles, items, runs,
+                     parts, chunk_blocks);
+  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_parts < 256 ? l.max_parts : 256)),
+                     dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, parts);
 }
 
 int check_common(const char* who, int32_t a_dtype, int32_t b_dtype, int64_t rows, int64_t width, int32_t index_bits, int64_t n,
