@@ -33,7 +33,7 @@ extern "C" {
  *     y[t, :] = scale * x[indices[t] - first_row, :]
  * for n indices and a table x of rows x width (contiguous).  An index outside
  * [first_row, first_row + rows) -- another shard's, or a negative one that marks nothing -- gives a
- * row of zeros; the table is not read for it.  first_row >= 0 places a vocabulary shard.
+ * row of zeros.  first_row >= 0 places a vocabulary shard.
  * y: n x width of y_dtype, contiguous; it must not overlap x.  n, rows and width may be 0.
  */
 int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, int64_t width, const void* indices,

@@ -32,6 +32,14 @@ constexpr int kLanes = 64;
 constexpr int kWaves = kBlock / kLanes;
 
 // ------------------------------------------------------------------------------------- forward
+// The product as an fp32 number.  For fp16 the compiler would else pick an instruction that rounds the
+// product to 16 bits at once, and only there: the other types' values are rounded to fp32 first.
+__device__ __forceinline__ float scaled(float scale, float x) {
+  float y = scale * x;
+  asm volatile("" : "+v"(y));
+  return y;
+}
+
 template <typename TX, typename TY, typename Id>
 __global__ __launch_bounds__(kBlock) void embedding_kernel(const TX* x, const Id* ids, int64_t n, int64_t rows,
                                                            int64_t first_row, int64_t width, int words,
@@ -43,28 +51,26 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(const TX* x, const Id
   for (unsigned i0 = threadIdx.x; i0 < items; i0 += kBlock * kInFlight) {
     typename Wide<TX>::Raw raw[kInFlight];
     int64_t to[kInFlight];
+    bool inside[kInFlight];
+    // Loads without a condition: a place behind the last repeats it, and for an index outside the
+    // table the word comes from row 0, which exists here, and is not used.  (The compiler puts a
+    // wait for all earlier loads in front of every load in a branch.)
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const unsigned i = i0 + u * kBlock;
-      if (i < items) {
-        const unsigned t = i / (unsigned)words, c = i - t * (unsigned)words;
-        const uint64_t row = (uint64_t)(int64_t)ids[t0 + t] - (uint64_t)first_row;
-        to[u] = (t0 + t) * width + (int64_t)c * kWide;
-        if (row < (uint64_t)rows)
-          raw[u] = Wide<TX>::load(x + (int64_t)row * width + (int64_t)c * kWide);
-        else
-          to[u] = ~to[u];  // no such row: zeros, whatever the scale
-      }
+      const unsigned i = i0 + u * kBlock < items ? i0 + u * kBlock : items - 1;
+      const unsigned t = i / (unsigned)words, c = i - t * (unsigned)words;
+      const uint64_t row = (uint64_t)(int64_t)ids[t0 + t] - (uint64_t)first_row;
+      inside[u] = row < (uint64_t)rows;
+      to[u] = (t0 + t) * width + (int64_t)c * kWide;
+      raw[u] = Wide<TX>::load(x + (inside[u] ? (int64_t)row : 0) * width + (int64_t)c * kWide);
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (i0 + u * kBlock < items) {
-        float v[kWide] = {};
-        if (to[u] >= 0) {
+        float v[kWide];
 #pragma unroll
-          for (int j = 0; j < kWide; ++j) v[j] = scale * Wide<TX>::get(raw[u], j);
-        }
-        Wide<TY>::store(y + (to[u] >= 0 ? to[u] : ~to[u]), v);
+        for (int j = 0; j < kWide; ++j) v[j] = inside[u] ? scaled(scale, Wide<TX>::get(raw[u], j)) : 0.f;
+        Wide<TY>::store(y + to[u], v);
       }
     }
   }
@@ -74,9 +80,16 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(const TX* x, const Id
     const unsigned t = i / (unsigned)rest, c = i - t * (unsigned)rest;
     const uint64_t row = (uint64_t)(int64_t)ids[t0 + t] - (uint64_t)first_row;
     const int64_t col = (int64_t)words * kWide + c;
-    const float v = row < (uint64_t)rows ? scale * Wide<TX>::one(x + (int64_t)row * width + col) : 0.f;
+    const float v = row < (uint64_t)rows ? scaled(scale, Wide<TX>::one(x + (int64_t)row * width + col)) : 0.f;
     Wide<TY>::put(y + (t0 + t) * width + col, v);
   }
+}
+
+// The rows of an empty table: zeros.
+template <typename TY>
+__global__ __launch_bounds__(kBlock) void no_rows(TY* y, int64_t elements) {
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < elements; i += (int64_t)gridDim.x * kBlock)
+    Wide<TY>::put(y + i, 0.f);
 }
 
 // ------------------------------------------------------------------------------------ gradient
@@ -86,10 +99,10 @@ constexpr int kChunk = 64;       // tokens of one partial sum of a longer row
 constexpr int kChunkBlock = 512;
 constexpr int kChunkWaves = kChunkBlock / kLanes;
 constexpr int kPerWave = kChunk / kChunkWaves;
-constexpr int kMinTileBits = 11, kMaxTileBits = 14;
+constexpr int kMinTileBits = 10, kMaxTileBits = 14;
 constexpr int kMaxTiles = 512;
 constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens have a lane each
-constexpr int kSortBlock = 1024;
+constexpr int kSmallSort = 512, kSort = 1024;  // threads of a tile of 2^10 tokens, of more
 constexpr int kInFlight = 8;  // words in flight per lane
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr int kSlotShift = 28;  // an entry: a token (23 bits: kMaxTiles tiles of 2^14) and its row's slot
@@ -157,7 +170,7 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   l->bucket_bits = bucket;
   l->buckets = (int)((rows + (1LL << bucket) - 1) >> bucket);
   l->index_at = place(tiles * (l->buckets + 1) * 2);
-  l->entries_at = place((rows + kGroup) * kDirect * 4);
+  l->entries_at = place(rows * kDirect * 4);
   l->counts_at = place(rows * 4);
   l->singles_at = place(l->max_singles * (int64_t)sizeof(Item));
   l->items_at = place(l->max_parts * (int64_t)sizeof(Item));
@@ -176,15 +189,41 @@ struct Which {
   }
 };
 
-// Sorts one tile by a bitonic network over (row << tile_bits | position), kEach = 2^tile_bits /
-// kSortBlock keys in the registers of each thread: key i sits in register i % kEach of thread
-// i / kEach, so of the 66 stages of 2048 keys 11 stay inside a thread, 45 inside a wavefront and 10
-// go through LDS.  Then the index: for every bucket of rows the first key that is not below it.
-template <typename Id, int kEach>
-__global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n, Which which, int tile_bits,
-                                                        int bucket_bits, int buckets, uint32_t* keys, uint16_t* index,
-                                                        Taken* taken) {
-  constexpr int kSize = kEach * kSortBlock;
+// The value of the lane whose number differs in the bit kMask: without LDS where the lanes are within
+// 16 of each other.
+template <int kMask>
+__device__ __forceinline__ uint32_t from_lane_xor(uint32_t x) {
+  if constexpr (kMask == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);   // quad_perm 1 0 3 2
+  if constexpr (kMask == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  if constexpr (kMask == 4) {  // 7 - i of each eight, then 3 - i of each four
+    const int y = __builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true);
+    return (uint32_t)__builtin_amdgcn_mov_dpp(y, 0x1b, 0xf, 0xf, true);
+  }
+  if constexpr (kMask == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true);  // row_ror 8 of 16
+  return (uint32_t)__shfl_xor((int)x, kMask, kLanes);
+}
+
+template <int kEach, int kMask>
+__device__ __forceinline__ void exchange_lanes(uint32_t (&v)[kEach], int tid, int k) {
+  if (kMask * kEach >= k) return;
+  const bool low = (tid & kMask) == 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const uint32_t y = from_lane_xor<kMask>(v[e]);
+    const bool up = ((tid * kEach + e) & k) == 0;
+    v[e] = low == up ? min(v[e], y) : max(v[e], y);
+  }
+}
+
+// Sorts one tile by a bitonic network over (row << tile_bits | position), kEach keys in the registers
+// of each thread: key i sits in register i % kEach of thread i / kEach, so of the 55 stages of 1024
+// keys 10 stay inside a thread, 39 inside a wavefront and 6 go through LDS.  Then the index: for every
+// bucket of rows the first key that is not below it.
+template <typename Id, int kThreads, int kEach>
+__global__ __launch_bounds__(kThreads) void tile_sort(const Id* ids, int64_t n, Which which, int tile_bits,
+                                                      int bucket_bits, int buckets, uint32_t* keys, uint16_t* index,
+                                                      Taken* taken) {
+  constexpr int kSize = kEach * kThreads;
   __shared__ uint32_t lds[kSize];
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * kSize;
@@ -192,7 +231,7 @@ __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n
   uint32_t v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int i = e * kSortBlock + tid;  // any order will do before the sort
+    const int i = e * kThreads + tid;  // any order will do before the sort
     const int64_t row = t0 + i < n ? which.row((int64_t)ids[t0 + i]) : -1;
     v[e] = row >= 0 ? (uint32_t)row << tile_bits | (uint32_t)i : kNoToken;
   }
@@ -201,26 +240,23 @@ __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n
     for (int j = k >> 1; j >= kEach * kLanes; j >>= 1) {  // across wavefronts
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) lds[e * kSortBlock + tid] = v[e];
+      for (int e = 0; e < kEach; ++e) lds[e * kThreads + tid] = v[e];
       __syncthreads();
       const int other = tid ^ (j / kEach);
       const bool low = (tid & (j / kEach)) == 0;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        const uint32_t y = lds[e * kSortBlock + other];
+        const uint32_t y = lds[e * kThreads + other];
         const bool up = ((tid * kEach + e) & k) == 0;
         v[e] = low == up ? min(v[e], y) : max(v[e], y);
       }
     }
-    for (int j = (k >> 1) < kEach * kLanes ? k >> 1 : kEach * kLanes / 2; j >= kEach; j >>= 1) {  // across lanes
-      const bool low = (tid & (j / kEach)) == 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const uint32_t y = __shfl_xor(v[e], j / kEach, kLanes);
-        const bool up = ((tid * kEach + e) & k) == 0;
-        v[e] = low == up ? min(v[e], y) : max(v[e], y);
-      }
-    }
+    exchange_lanes<kEach, 32>(v, tid, k);
+    exchange_lanes<kEach, 16>(v, tid, k);
+    exchange_lanes<kEach, 8>(v, tid, k);
+    exchange_lanes<kEach, 4>(v, tid, k);
+    exchange_lanes<kEach, 2>(v, tid, k);
+    exchange_lanes<kEach, 1>(v, tid, k);
 #pragma unroll
     for (int j = kEach / 2; j > 0; j >>= 1) {  // across registers
       if (j >= k) continue;
@@ -238,8 +274,8 @@ __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n
 #pragma unroll
   for (int e = 0; e < kEach; ++e) lds[tid * kEach + e] = v[e];
   __syncthreads();
-  for (int i = tid; i < kSize; i += kSortBlock) keys[t0 + i] = lds[i];
-  for (int b = tid; b <= buckets; b += kSortBlock) {
+  for (int i = tid; i < kSize; i += kThreads) keys[t0 + i] = lds[i];
+  for (int b = tid; b <= buckets; b += kThreads) {
     // The last entry lies behind every row; its key may exceed 32 bits.
     const uint64_t key = (uint64_t)b << (bucket_bits + tile_bits);
     int at = 0;
@@ -250,23 +286,23 @@ __global__ __launch_bounds__(kSortBlock) void tile_sort(const Id* ids, int64_t n
   }
 }
 
-// A wavefront's share of a row: kSweeps words per lane, 64 words apart, or single columns.
-// Adds `count` tokens, of which lane first + e of `token` holds the e-th; `count` is the same in all
-// lanes.  kInFlight words are requested before the first is needed: of several tokens, or of one token
-// where rows are long and tokens few.
-template <typename TD, int kSweeps>
+// Words kSweeps times 64 apart of `count` > 0 tokens, of which lane e of `token` holds the e-th, added to
+// acc; `count` is the same in all lanes.  The loads are issued without a condition -- lanes behind
+// the row's last word and places behind the last token repeat that one -- because the compiler puts
+// a wait for all earlier loads in front of every load in a branch.
+template <typename TD, int kSweeps, int kTokens>
 __device__ __forceinline__ void add_words(const TD* dy, int64_t width, int64_t word, int64_t words, int token, int count,
                                           float (&acc)[kSweeps][kWide]) {
-  constexpr int kTokens = kInFlight / kSweeps;
   for (int e0 = 0; e0 < count; e0 += kTokens) {
     typename Wide<TD>::Raw raw[kTokens][kSweeps];
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      if (e0 + u < count) {
-        const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
+      const int e = e0 + u < count ? e0 + u : count - 1;
+      const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e) * width;
 #pragma unroll
-        for (int s = 0; s < kSweeps; ++s)
-          if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
+      for (int s = 0; s < kSweeps; ++s) {
+        const int64_t w = word + s * kLanes;
+        raw[u][s] = Wide<TD>::load(row + (w < words ? w : words - 1) * kWide);
       }
     }
 #pragma unroll
@@ -274,10 +310,8 @@ __device__ __forceinline__ void add_words(const TD* dy, int64_t width, int64_t w
       if (e0 + u < count) {
 #pragma unroll
         for (int s = 0; s < kSweeps; ++s) {
-          if (word + s * kLanes < words) {
 #pragma unroll
-            for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
-          }
+          for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
         }
       }
     }
@@ -287,18 +321,17 @@ __device__ __forceinline__ void add_words(const TD* dy, int64_t width, int64_t w
 template <typename TD>
 __device__ __forceinline__ float add_singles(const TD* dy, int64_t width, int64_t col, int token, int count) {
   float acc = 0.f;
+  if (col >= width) col = width - 1;
   for (int e0 = 0; e0 < count; e0 += kInFlight) {
     float one[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      if (e0 + u < count) {
-        const int64_t t = __builtin_amdgcn_readlane(token, e0 + u);
-        if (col < width) one[u] = Wide<TD>::one(dy + t * width + col);
-      }
+      const int64_t t = __builtin_amdgcn_readlane(token, e0 + u < count ? e0 + u : count - 1);
+      one[u] = Wide<TD>::one(dy + t * width + col);
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u)
-      if (e0 + u < count && col < width) acc += one[u];
+      if (e0 + u < count) acc += one[u];
   }
   return acc;
 }
@@ -391,7 +424,7 @@ __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids
       constexpr int kSweeps = decltype(sweeps)::value;
       float acc[kSweeps][kWide] = {};
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
+      for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps, kInFlight / kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
 #pragma unroll
       for (int s = 0; s < kSweeps; ++s) {
         const int64_t word = w + lane + s * kLanes;
@@ -408,26 +441,28 @@ __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids
   }
 }
 
-// A wavefront takes kSlots rows.  kLanes / kSlots lanes for each row share the tiles, kRounds tiles a
-// lane.  Rows without tokens become zeros, long ones are listed, and the tokens of the others go
-// to the wavefront's own stretch of `entries`, row by row, kDirect of them for each row at most.
-// Its rows lie `stride` apart: neighbours in a vocabulary are often alike in frequency, and a
-// wavefront with eight rows of many tokens would finish long after the rest.
+// Element i of a list whose bytes 32 bits can count: the address is one register behind a base.
+template <typename T>
+__device__ __forceinline__ T element(const T* base, uint32_t i) {
+  return *(const RAFHIP_GLOBAL T*)((const char*)base + (size_t)(i * (uint32_t)sizeof(T)));
+}
+
+// A wavefront takes kSlots neighbouring rows, whose places in a tile are neighbours too.  kLanes /
+// kSlots lanes for each row share the tiles, kRounds tiles a lane.  Rows without tokens become
+// zeros, long ones are listed, and the tokens of the others go to entries[row][kDirect].
 template <typename TO, int kSlots, int kRounds>
 __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const uint16_t* index, int tiles, int tile_bits,
-                                                    int bucket_bits, int buckets, int64_t stride, int64_t rows,
-                                                    int64_t width, int accumulate, TO* dx, Taken* taken, uint32_t* entries_out,
+                                                    int bucket_bits, int buckets, int64_t rows, int64_t width,
+                                                    int accumulate, TO* dx, Taken* taken, uint32_t* entries,
                                                     uint32_t* counts, Item* singles, Item* items, Run* runs) {
   constexpr int kSpread = kLanes / kSlots;
-  __shared__ uint32_t places[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
-  const int in_block = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-  const int64_t wave = (int64_t)blockIdx.x * kWaves + in_block;
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   const int64_t n_waves = (int64_t)gridDim.x * kWaves;
   const uint32_t size = 1u << tile_bits;
   const int slot = lane / kSpread, tile0 = lane % kSpread;
-  for (int64_t r0 = wave; r0 < stride; r0 += n_waves) {
-    const int64_t my_row = r0 + slot * stride;
+  for (int64_t r0 = wave * kSlots; r0 < rows; r0 += n_waves * kSlots) {
+    const int64_t my_row = r0 + slot;
     uint32_t at[kRounds];
     int len[kRounds], before[kRounds];
     int total = 0;  // tokens of this lane's row, the same in all its lanes
@@ -436,32 +471,41 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
     uint32_t lo[kRounds], lo_end[kRounds], hi[kRounds], hi_end[kRounds];
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
-      const int t = q * kSpread + tile0;
-      lo[q] = lo_end[q] = 0;
-      if (my_row < rows && t < tiles) {
-        const uint16_t* bucket = index + (int64_t)t * (buckets + 1) + (my_row >> bucket_bits);
-        lo[q] = bucket[0];
-        lo_end[q] = bucket[1];
-      }
+      // Loads without a condition here and below: lanes without a tile or a row look at the first
+      // tile or the last row.
+      const int t = q * kSpread + tile0 < tiles ? q * kSpread + tile0 : 0;
+      const uint16_t* bucket = index + (int64_t)t * (buckets + 1) + ((my_row < rows ? my_row : rows - 1) >> bucket_bits);
+      lo[q] = bucket[0];
+      lo_end[q] = bucket[1];
+    }
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
+      if (my_row >= rows || q * kSpread + tile0 >= tiles) lo[q] = lo_end[q] = 0;
       hi[q] = lo[q];
       hi_end[q] = lo_end[q];
     }
     const uint32_t lo_key = (uint32_t)my_row << tile_bits, hi_key = (uint32_t)(my_row + 1) << tile_bits;
     for (bool more = true; more;) {
       more = false;
+      uint32_t x[kRounds], y[kRounds];
 #pragma unroll
       for (int q = 0; q < kRounds; ++q) {
-        const uint32_t* tile = keys + ((int64_t)(q * kSpread + tile0) << tile_bits);
+        const uint32_t tile = (uint32_t)(q * kSpread + tile0 < tiles ? q * kSpread + tile0 : 0) << tile_bits;
+        const uint32_t a = (lo[q] + lo_end[q]) >> 1, b = (hi[q] + hi_end[q]) >> 1;  // size where the run ends the tile
+        x[q] = element(keys, tile + (a < size ? a : 0));
+        y[q] = element(keys, tile + (b < size ? b : 0));
+      }
+#pragma unroll
+      for (int q = 0; q < kRounds; ++q) {
         const uint32_t a = (lo[q] + lo_end[q]) >> 1, b = (hi[q] + hi_end[q]) >> 1;
-        const uint32_t x = lo[q] < lo_end[q] ? tile[a] : 0, y = hi[q] < hi_end[q] ? tile[b] : 0;
         if (lo[q] < lo_end[q]) {
-          if (x < lo_key)
+          if (x[q] < lo_key)
             lo[q] = a + 1;
           else
             lo_end[q] = a;
         }
         if (hi[q] < hi_end[q]) {
-          if (y < hi_key)
+          if (y[q] < hi_key)
             hi[q] = b + 1;
           else
             hi_end[q] = b;
@@ -485,17 +529,29 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
       before[q] = total + sum - len[q];
       total += __shfl(sum, kSpread - 1, kSpread);
     }
-    int entries = 0, base = 0;  // tokens of the short rows; of those in front of this lane's row
-    Taken want = 0;             // by the long ones
+    if (my_row < rows && total <= kDirect) {
+      if (tile0 == 0) counts[my_row] = (uint32_t)total;
+      uint32_t key[kRounds];  // of the first token of each run; most runs have no other
+#pragma unroll
+      for (int q = 0; q < kRounds; ++q) key[q] = element(keys, len[q] > 0 ? at[q] : 0);
+#pragma unroll
+      for (int q = 0; q < kRounds; ++q) {
+        const uint32_t first_of_tile = (uint32_t)(q * kSpread + tile0) << tile_bits;
+        uint32_t* out = entries + my_row * kDirect + before[q];
+        if (len[q] > 0) out[0] = first_of_tile + (key[q] & (size - 1));
+        for (int x = 1; x < len[q]; ++x) out[x] = first_of_tile + (element(keys, at[q] + x) & (size - 1));
+      }
+    } else if (my_row < rows && tile0 == 0) {
+      counts[my_row] = 0;
+    }
+    Taken want = 0;  // by the long rows
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      const int64_t row = r0 + i * stride;
+      const int64_t row = r0 + i;
       if (row >= rows) break;
       const int count = __builtin_amdgcn_readlane(total, i * kSpread);
       if (count <= kDirect) {
         if (count == 0 && !accumulate) zero_row(dx + row * width, width);
-        if (slot == i) base = entries;
-        entries += count;
         continue;
       }
       int n_runs = 0;
@@ -511,7 +567,7 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
               (Taken)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(first >> 32)) << 32;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
-        const int64_t row = r0 + i * stride;
+        const int64_t row = r0 + i;
         if (row >= rows) break;
         const int count = __builtin_amdgcn_readlane(total, i * kSpread);
         if (count <= kDirect) continue;
@@ -531,84 +587,73 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
         first += take(n_runs, chunks);
       }
     }
-    if (lane == 0) counts[r0] = (uint32_t)entries;
-    if (entries == 0) continue;
-    // Lane e gets the e-th token of the short rows.
-    if (total <= kDirect) {
-#pragma unroll
-      for (int q = 0; q < kRounds; ++q)
-        for (int x = 0; x < len[q]; ++x) places[in_block][base + before[q] + x] = (at[q] + x) | (uint32_t)slot << kSlotShift;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (lane < entries) {
-      const uint32_t place = places[in_block][lane], key_at = place & ((1u << kSlotShift) - 1);
-      const uint32_t token = (key_at >> tile_bits << tile_bits) + (keys[key_at] & (size - 1));
-      entries_out[r0 * (kSlots * kDirect) + lane] = token | (place >> kSlotShift << kSlotShift);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// The short rows of one wavefront of find_rows: `entries` tokens, one per lane, in one go, so that the
-// loads of the next row are under way while this one is finished.
+// A slice of 64 words of kGroup rows, `stride` apart, by a wavefront: the tokens of the short ones, a lane for each, in one go,
+// so that the loads of the next row are under way while this one is finished.  Neighbours in a
+// vocabulary are often alike in frequency; a wavefront with eight neighbouring rows of many tokens
+// would finish long after the rest.
 template <typename TD, typename TO>
-__device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, uint32_t entry, int entries, int64_t r0,
-                                               int64_t stride, float scale, bool accumulate, TO* dx) {
+__device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, const uint32_t* entry, const uint32_t* counts,
+                                               int64_t r0, int64_t stride, int64_t rows, int slice, float scale,
+                                               bool accumulate, TO* dx) {
   const int lane = threadIdx.x & (kLanes - 1);
+  const int slot = lane / kDirect, x = lane % kDirect;
+  const int64_t my_row = r0 + slot * stride;
+  const bool set = my_row < rows && x < (int)counts[my_row < rows ? my_row : 0];
+  const uint32_t mine = set ? entry[my_row * kDirect + x] | (uint32_t)slot << kSlotShift : 0;
+  const uint64_t m = __ballot(set);
+  const int entries = __popcll(m);
+  if (entries == 0) return;
+  // A lane that holds a token sends it to the lane of its rank, the others behind the last.
+  const int rank = __popcll(m & ((1ull << lane) - 1));
+  const uint32_t got = (uint32_t)__builtin_amdgcn_ds_permute((set ? rank : entries + (lane - rank)) * 4, (int)mine);
+  const int token = (int)(got & ((1u << kSlotShift) - 1)), of = (int)(got >> kSlotShift);
   const int64_t words = width / kWide;
-  const int token = (int)(entry & ((1u << kSlotShift) - 1)), of = (int)(entry >> kSlotShift);
   const int next = __shfl_down(of, 1, kLanes);
   const uint64_t last = __ballot(lane < entries && (lane + 1 == entries || next != of));  // of its row
-  for_words(words, [&](auto sweeps, int64_t w) {
-    constexpr int kSweeps = decltype(sweeps)::value;
-    constexpr int kTokens = kInFlight / kSweeps;
-    const int64_t word = w + lane;
-    float acc[kSweeps][kWide] = {};
-    for (int e0 = 0; e0 < entries; e0 += kTokens) {
-      typename Wide<TD>::Raw raw[kTokens][kSweeps];
+  const int64_t word = (int64_t)slice * kLanes + lane;
+  float acc[kWide] = {};
+  // A batch of kTokens, loads first and without a condition, as in add_words.
+  auto batch = [&](auto tokens, int e0) {
+    constexpr int kTokens = decltype(tokens)::value;
+    typename Wide<TD>::Raw raw[kTokens];
 #pragma unroll
-      for (int u = 0; u < kTokens; ++u) {
-        if (e0 + u < entries) {
-          const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e0 + u) * width;
+    for (int u = 0; u < kTokens; ++u) {
+      const int e = e0 + u < entries ? e0 + u : entries - 1;
+      raw[u] = Wide<TD>::load(dy + (int64_t)__builtin_amdgcn_readlane(token, e) * width + (word < words ? word : words - 1) * kWide);
+    }
 #pragma unroll
-          for (int s = 0; s < kSweeps; ++s)
-            if (word + s * kLanes < words) raw[u][s] = Wide<TD>::load(row + (word + s * kLanes) * kWide);
-        }
-      }
+    for (int u = 0; u < kTokens; ++u) {
+      if (e0 + u < entries) {
 #pragma unroll
-      for (int u = 0; u < kTokens; ++u) {
-        if (e0 + u < entries) {
-          const bool done = last >> (e0 + u) & 1;
+        for (int j = 0; j < kWide; ++j) acc[j] += Wide<TD>::get(raw[u], j);
+        if (last >> (e0 + u) & 1) {
           TO* out = dx + (r0 + __builtin_amdgcn_readlane(of, e0 + u) * stride) * width;
+          if (word < words) put_row<TO, kWide>(out + word * kWide, acc, scale, accumulate);
 #pragma unroll
-          for (int s = 0; s < kSweeps; ++s) {
-            if (word + s * kLanes < words) {
-#pragma unroll
-              for (int j = 0; j < kWide; ++j) acc[s][j] += Wide<TD>::get(raw[u][s], j);
-              if (done) {
-                put_row<TO, kWide>(out + (word + s * kLanes) * kWide, acc[s], scale, accumulate);
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) acc[s][j] = 0.f;
-              }
-            }
-          }
+          for (int j = 0; j < kWide; ++j) acc[j] = 0.f;
         }
       }
     }
-  });
+  };
+  if ((int64_t)slice * kLanes < words) {
+    int e0 = 0;
+    for (; entries - e0 > kInFlight / 2; e0 += kInFlight) batch(std::integral_constant<int, kInFlight>{}, e0);
+    if (e0 < entries) batch(std::integral_constant<int, kInFlight / 2>{}, e0);
+  }
   const int64_t col = words * kWide + lane;  // columns behind the last whole word
-  if (words * kWide < width) {
-    float acc[1] = {0.f};
+  if (slice == 0 && words * kWide < width) {
+    float one[1] = {0.f};
     for (int e = 0; e < entries; ++e) {
       const int64_t t = __builtin_amdgcn_readlane(token, e);
       const int64_t row = r0 + __builtin_amdgcn_readlane(of, e) * stride;
       if (col < width) {
-        acc[0] += Wide<TD>::one(dy + t * width + col);
+        one[0] += Wide<TD>::one(dy + t * width + col);
         if (last >> e & 1) {
-          put_row<TO, 1>(dx + row * width + col, acc, scale, accumulate);
-          acc[0] = 0.f;
+          put_row<TO, 1>(dx + row * width + col, one, scale, accumulate);
+          one[0] = 0.f;
         }
       }
     }
@@ -618,29 +663,30 @@ __device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, uint
 // The first chunk_blocks workgroups take the chunks, one after the other: each of eight wavefronts sums
 // kPerWave tokens, the sums are added in order, and the result is the row (a row of one chunk) or a
 // partial sum.  The others take the short rows.
+// A unit of work is a slice of 64 words, so that a wide row's loads are all under way at once rather
+// than one slice after the other behind the same look-ups (65536 tokens of width 1600: 106 to SLICED us).
 template <typename TD, typename TO>
 __global__ __launch_bounds__(kChunkBlock) void sum_rows(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
                                                         float scale, int accumulate, TO* dx, const Taken* taken,
                                                         const uint32_t* entries, const uint32_t* counts, int64_t stride,
-                                                        int per_wave, const Item* singles, const Item* items,
-                                                        const Run* runs, float* parts, unsigned chunk_blocks) {
-  constexpr int kSweeps = 1;
+                                                        int64_t rows, const Item* singles, const Item* items, const Run* runs,
+                                                        float* parts, unsigned chunk_blocks, unsigned slices) {
   __shared__ float sums[kChunkWaves][kLanes * kWide];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   if (blockIdx.x >= chunk_blocks) {
     const int64_t n_waves = (int64_t)(gridDim.x - chunk_blocks) * kChunkWaves;
-    for (int64_t r0 = (int64_t)(blockIdx.x - chunk_blocks) * kChunkWaves + wave; r0 < stride; r0 += n_waves) {
-      const int count = __builtin_amdgcn_readfirstlane((int)counts[r0]);
-      const uint32_t entry = lane < per_wave ? entries[r0 * per_wave + lane] : 0;  // what lies behind the last is not used
-      if (count > 0) sum_short_rows(dy, width, entry, count, r0, stride, scale, accumulate != 0, dx);
+    for (int64_t u = (int64_t)(blockIdx.x - chunk_blocks) * kChunkWaves + wave; u < stride * slices; u += n_waves) {
+      const int64_t r0 = u / slices;
+      sum_short_rows(dy, width, entries, counts, r0, stride, rows, (int)(u - r0 * slices), scale, accumulate != 0, dx);
     }
     return;
   }
   const Taken listed = *taken;
   const uint32_t n_parts = parts_of(listed), n_items = n_parts + singles_of(listed);
   const int64_t words = width / kWide;
-  for (uint32_t it = blockIdx.x; it < n_items; it += chunk_blocks) {
+  for (uint32_t u = blockIdx.x; u < n_items * slices; u += chunk_blocks) {
+    const uint32_t it = u / slices, slice = u - it * slices;
     const Item item = it < n_parts ? items[it] : singles[it - n_parts];
     const int first = (int)item.chunk * kChunk + wave * kPerWave;
     int count = (int)item.tokens - first;
@@ -687,15 +733,16 @@ __global__ __launch_bounds__(kChunkBlock) void sum_rows(const TD* dy, const uint
       }
       __syncthreads();
     };
-    for (int64_t w = 0; w < words; w += kLanes) {
-      float acc[kSweeps][kWide] = {};
-      add_words<TD, kSweeps>(dy, width, w + lane, words, token, count, acc);
+    const int64_t w = (int64_t)slice * kLanes;
+    if (w < words) {
+      float acc[1][kWide] = {};
+      add_words<TD, 1, kPerWave>(dy, width, w + lane, words, token, count, acc);
 #pragma unroll
       for (int j = 0; j < kWide; ++j) sums[wave][lane * kWide + j] = acc[0][j];
       const int64_t left = (words - w) * kWide;
       join(w * kWide, (int)(left < kLanes * kWide ? left : kLanes * kWide));
     }
-    if (words * kWide < width) {
+    if (slice == 0 && words * kWide < width) {
       sums[wave][lane] = add_singles(dy, width, words * kWide + lane, token, count);
       join(words * kWide, (int)(width - words * kWide));
     }
@@ -764,37 +811,42 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   auto* runs = reinterpret_cast<Run*>(ws + l.runs_at);
   auto* parts = reinterpret_cast<float*>(ws + l.parts_at);
   auto sort = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)l.tiles), dim3(kSortBlock), 0, s, ids, n, which, l.tile_bits, l.bucket_bits,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)l.tiles), dim3(l.tile_bits == kMinTileBits ? kSmallSort : kSort), 0, s, ids, n, which, l.tile_bits, l.bucket_bits,
                        l.buckets, keys, index, taken);
   };
   switch (l.tile_bits) {
-    case 11: sort(tile_sort<Id, 2>); break;
-    case 12: sort(tile_sort<Id, 4>); break;
-    case 13: sort(tile_sort<Id, 8>); break;
-    default: sort(tile_sort<Id, 16>); break;
+    case kMinTileBits: sort(tile_sort<Id, kSmallSort, 2>); break;
+    case 11: sort(tile_sort<Id, kSort, 2>); break;
+    case 12: sort(tile_sort<Id, kSort, 4>); break;
+    case 13: sort(tile_sort<Id, kSort, 8>); break;
+    default: sort(tile_sort<Id, kSort, 16>); break;
   }
   const int group = l.tiles <= kLanes ? kGroup : 1;
-  const int64_t waves = (rows + group - 1) / group;  // of find_rows, and the distance of a wavefront's rows
-  const int64_t max_blocks = (waves + kWaves - 1) / kWaves;
+  const int64_t max_blocks = ((rows + group - 1) / group + kWaves - 1) / kWaves;
   const unsigned find_blocks = (unsigned)(max_blocks < kMaxFindBlocks ? max_blocks : kMaxFindBlocks);
   auto find = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(find_blocks), dim3(kBlock), 0, s, keys, index, l.tiles, l.tile_bits, l.bucket_bits,
-                       l.buckets, waves, rows, width, accumulate, dx, taken, entries, counts, singles, items, runs);
+                       l.buckets, rows, width, accumulate, dx, taken, entries, counts, singles, items, runs);
   };
   if (l.tiles <= 8)
     find(find_rows<TO, kGroup, 1>);
+  else if (l.tiles <= 16)
+    find(find_rows<TO, kGroup, 2>);
   else if (l.tiles <= 32)
     find(find_rows<TO, kGroup, 4>);
   else if (l.tiles <= kLanes)
     find(find_rows<TO, kGroup, 8>);
   else
     find(find_rows<TO, 1, kMaxTiles / kLanes>);
-  const int64_t max_items = l.max_singles + l.max_parts, max_short = (waves + kChunkWaves - 1) / kChunkWaves;
+  const unsigned slices = (unsigned)((width / kWide + kLanes - 1) / kLanes > 0 ? (width / kWide + kLanes - 1) / kLanes : 1);
+  const int64_t max_items = (l.max_singles + l.max_parts) * slices;
+  const int64_t stride = (rows + kGroup - 1) / kGroup;  // wavefronts with short rows
+  const int64_t max_short = (stride * slices + kChunkWaves - 1) / kChunkWaves;
   const unsigned chunk_blocks = (unsigned)(max_items < kMaxSumBlocks ? max_items : kMaxSumBlocks);
   const unsigned short_blocks = (unsigned)(max_short < kMaxSumBlocks ? max_short : kMaxSumBlocks);
   hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kChunkBlock), 0, s, dy, keys, l.tile_bits,
-                     width, scale, accumulate, dx, taken, entries, counts, waves, group * kDirect, singles, items, runs,
-                     parts, chunk_blocks);
+                     width, scale, accumulate, dx, taken, entries, counts, stride, rows, singles, items, runs,
+                     parts, chunk_blocks, slices);
   hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_parts < 256 ? l.max_parts : 256)),
                      dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, parts);
 }
@@ -828,6 +880,15 @@ extern "C" int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, in
   if ((rows > 0 && !x) || !indices || !y) return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
   if (!is_aligned(x, element_bytes(x_dtype)) || !is_aligned(y, element_bytes(y_dtype)) || !is_aligned(indices, index_bits / 8))
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) {
+    with_element(y_dtype, [&](auto ty) {
+      using TY = decltype(ty);
+      hipLaunchKernelGGL(no_rows<TY>, dim3(1024), dim3(kBlock), 0, s, static_cast<TY*>(y), n * width);
+    });
+    RAFHIP_HIP_TRY(hipGetLastError());
+    return RAFHIP_OK;
+  }
   const int words = (int)(width / kWide);
   // Four words in flight per lane where that still leaves every CU several workgroups, one where it does not.
   const int64_t all = n * (words > 0 ? words : 1);
@@ -836,7 +897,6 @@ extern "C" int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, in
   tokens = tokens < 1 ? 1 : tokens;
   const int64_t blocks = (n + tokens - 1) / tokens;
   if (blocks > INT32_MAX) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)n);
-  hipStream_t s = static_cast<hipStream_t>(stream);
   with_element(x_dtype, [&](auto tx) {
     with_element(y_dtype, [&](auto ty) {
       with_index(index_bits, [&](auto id) {

@@ -191,8 +191,10 @@ __device__ __forceinline__ void add_columns(Sums<kTwo>& a, const T* z, int count
     typename Wide<T>::Raw raw[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int w = w0 + u * kBlock;
-      raw[u] = w < s.words ? Wide<T>::load(z + s.head + (int64_t)w * kWide) : Wide<T>::fill(-INFINITY);
+      // Without a condition, the last word again behind the last: the compiler puts a wait for all
+      // earlier loads in front of every load in a branch.
+      const int w = w0 + u * kBlock < s.words ? w0 + u * kBlock : s.words - 1;
+      raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
     }
     float top = a.m;
 #pragma unroll
@@ -501,8 +503,8 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
     typename Wide<T>::Raw raw[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int w = w0 + u * kGradBlock;
-      if (w < s.words) raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
+      const int w = w0 + u * kGradBlock < s.words ? w0 + u * kGradBlock : s.words - 1;
+      raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
@@ -552,10 +554,15 @@ __global__ __launch_bounds__(kStepBlock) void row_step(Task a, float c0, const f
     return;
   }
   typename Wide<T>::Raw raw[kWords];
+  if (s.words > 0) {
 #pragma unroll
-  for (int u = 0; u < kWords; ++u) {
-    const int w = i + u * kStepBlock;
-    raw[u] = w < s.words ? Wide<T>::load(z + s.head + (int64_t)w * kWide) : Wide<T>::fill(-INFINITY);
+    for (int u = 0; u < kWords; ++u) {
+      const int w = i + u * kStepBlock < s.words ? i + u * kStepBlock : s.words - 1;
+      raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) raw[u] = Wide<T>::fill(-INFINITY);
   }
   const float x1 = single ? Wide<T>::one(z + single_at) : -INFINITY;
   list_picks<kStepBlock>(a, row, t, label, dl, 0, a.vocab, picks);
