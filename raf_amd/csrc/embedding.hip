@@ -95,10 +95,7 @@ __global__ __launch_bounds__(kBlock) void no_rows(TY* y, int64_t elements) {
 // ------------------------------------------------------------------------------------ gradient
 constexpr int kFewTokens = 256;  // one launch up to here
 constexpr int kDirect = 8;       // tokens of a row that one wavefront sums
-constexpr int kChunk = 64;       // tokens of one partial sum of a longer row
-constexpr int kChunkBlock = 512;
-constexpr int kChunkWaves = kChunkBlock / kLanes;
-constexpr int kPerWave = kChunk / kChunkWaves;
+constexpr int kChunk = 32;       // tokens of one partial sum of a longer row
 constexpr int kMinTileBits = 10, kMaxTileBits = 14;
 constexpr int kMaxTiles = 512;
 constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens have a lane each
@@ -130,7 +127,7 @@ struct Run {
 // How much of each list is taken, in one word: a wavefront reserves all it needs with one atomic
 // (with four, 800 wavefronts queued for some 60 us).
 typedef unsigned long long Taken;
-constexpr int kRunBits = 24, kSingleBits = 21;  // up to 2^23 runs, 2^20 rows of one chunk, 2^18 chunks
+constexpr int kRunBits = 24, kSingleBits = 21;  // up to 2^23 runs, 2^23 / 9 rows of one chunk, 2^23 / 16 chunks
 __device__ __forceinline__ Taken take(uint32_t runs, uint32_t chunks) {
   return (Taken)runs | (chunks == 1 ? (Taken)1 << kRunBits : (Taken)chunks << (kRunBits + kSingleBits));
 }
@@ -660,23 +657,69 @@ __device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, cons
   }
 }
 
-// The first chunk_blocks workgroups take the chunks, one after the other: each of eight wavefronts sums
-// kPerWave tokens, the sums are added in order, and the result is the row (a row of one chunk) or a
-// partial sum.  The others take the short rows.
-// A unit of work is a slice of 64 words, so that a wide row's loads are all under way at once rather
-// than one slice after the other behind the same look-ups (65536 tokens of width 1600: 106 to SLICED us).
+// A slice of 64 words of one chunk, by a wavefront: the row itself (a row of one chunk) or a partial sum.
 template <typename TD, typename TO>
-__global__ __launch_bounds__(kChunkBlock) void sum_rows(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
-                                                        float scale, int accumulate, TO* dx, const Taken* taken,
-                                                        const uint32_t* entries, const uint32_t* counts, int64_t stride,
-                                                        int64_t rows, const Item* singles, const Item* items, const Run* runs,
-                                                        float* parts, unsigned chunk_blocks, unsigned slices) {
-  __shared__ float sums[kChunkWaves][kLanes * kWide];
+__device__ __forceinline__ void sum_chunk(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width, const Item& item,
+                                          const Run* runs, int slice, float scale, bool accumulate, TO* row, float* part) {
   const int lane = threadIdx.x & (kLanes - 1);
+  const int first = (int)item.chunk * kChunk;
+  const int count = (int)item.tokens - first < kChunk ? (int)item.tokens - first : kChunk;
+  // Where this lane's token is: in the last run that starts at or before it.
+  const uint32_t want = (uint32_t)(first + (lane < count ? lane : 0));
+  uint32_t at = 0, before = 0;
+  for (uint32_t r0 = 0; r0 < item.n_runs; r0 += kLanes) {
+    const uint32_t r = r0 + lane < item.n_runs ? r0 + lane : item.n_runs - 1;  // the last run again behind the last
+    const Run mine = runs[item.first_run + r];
+    int found = 0;  // all lanes take part in every exchange, whether or not their run is among these
+#pragma unroll
+    for (int step = kLanes / 2; step > 0; step >>= 1) {
+      const uint32_t start = (uint32_t)__shfl((int)mine.before, found + step, kLanes);
+      found += start <= want ? step : 0;
+    }
+    const uint32_t a = (uint32_t)__shfl((int)mine.at, found, kLanes), b = (uint32_t)__shfl((int)mine.before, found, kLanes);
+    at = b <= want ? a : at;
+    before = b <= want ? b : before;
+  }
+  const uint32_t key_at = at + (want - before);
+  const int token = (int)((key_at >> tile_bits << tile_bits) + (element(keys, key_at) & ((1u << tile_bits) - 1)));
+  const int64_t words = width / kWide;
+  const int64_t word = (int64_t)slice * kLanes + lane;
+  if ((int64_t)slice * kLanes < words) {
+    float acc[1][kWide] = {};
+    add_words<TD, 1, kInFlight>(dy, width, word, words, token, count, acc);
+    if (word < words) {
+      if (part)
+        Wide<float>::store(part + word * kWide, acc[0]);
+      else
+        put_row<TO, kWide>(row + word * kWide, acc[0], scale, accumulate);
+    }
+  }
+  const int64_t col = words * kWide + lane;  // columns behind the last whole word
+  if (slice == 0 && words * kWide < width) {
+    const float one[1] = {add_singles(dy, width, col, token, count)};
+    if (col < width) {
+      if (part)
+        part[col] = one[0];
+      else
+        put_row<TO, 1>(row + col, one, scale, accumulate);
+    }
+  }
+}
+
+// The first chunk_blocks workgroups take the chunks, the others the short rows.  A unit of work is a
+// wavefront's: a slice of 64 words, so that a wide row's loads are all under way at once rather than
+// one slice after the other behind the same look-ups.  (Eight wavefronts to a chunk, joined in LDS,
+// spent most of their time on looking up their eight tokens each.)
+template <typename TD, typename TO>
+__global__ __launch_bounds__(kBlock) void sum_rows(const TD* dy, const uint32_t* keys, int tile_bits, int64_t width,
+                                                   float scale, int accumulate, TO* dx, const Taken* taken,
+                                                   const uint32_t* entries, const uint32_t* counts, int64_t stride,
+                                                   int64_t rows, const Item* singles, const Item* items, const Run* runs,
+                                                   float* parts, unsigned chunk_blocks, unsigned slices) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   if (blockIdx.x >= chunk_blocks) {
-    const int64_t n_waves = (int64_t)(gridDim.x - chunk_blocks) * kChunkWaves;
-    for (int64_t u = (int64_t)(blockIdx.x - chunk_blocks) * kChunkWaves + wave; u < stride * slices; u += n_waves) {
+    const int64_t n_waves = (int64_t)(gridDim.x - chunk_blocks) * kWaves;
+    for (int64_t u = (int64_t)(blockIdx.x - chunk_blocks) * kWaves + wave; u < stride * slices; u += n_waves) {
       const int64_t r0 = u / slices;
       sum_short_rows(dy, width, entries, counts, r0, stride, rows, (int)(u - r0 * slices), scale, accumulate != 0, dx);
     }
@@ -684,68 +727,11 @@ __global__ __launch_bounds__(kChunkBlock) void sum_rows(const TD* dy, const uint
   }
   const Taken listed = *taken;
   const uint32_t n_parts = parts_of(listed), n_items = n_parts + singles_of(listed);
-  const int64_t words = width / kWide;
-  for (uint32_t u = blockIdx.x; u < n_items * slices; u += chunk_blocks) {
-    const uint32_t it = u / slices, slice = u - it * slices;
+  for (uint64_t u = (uint64_t)blockIdx.x * kWaves + wave; u < (uint64_t)n_items * slices; u += (uint64_t)chunk_blocks * kWaves) {
+    const uint32_t it = (uint32_t)(u / slices), slice = (uint32_t)(u - (uint64_t)it * slices);
     const Item item = it < n_parts ? items[it] : singles[it - n_parts];
-    const int first = (int)item.chunk * kChunk + wave * kPerWave;
-    int count = (int)item.tokens - first;
-    count = count < 0 ? 0 : count > kPerWave ? kPerWave : count;
-    // Where this lane's token is: in the last run that starts at or before it.
-    const uint32_t want = (uint32_t)(first + lane);
-    uint32_t at = 0, before = 0;
-    for (uint32_t r0 = 0; r0 < item.n_runs && count > 0; r0 += kLanes) {
-      Run mine{0, 0xffffffffu};
-      if (r0 + lane < item.n_runs) mine = runs[item.first_run + r0 + lane];
-#pragma unroll
-      for (int e = 0; e < kPerWave; ++e) {
-        const uint64_t started = __ballot(mine.before <= (uint32_t)(first + e));
-        if (started != 0) {
-          const int last = 63 - __clzll((long long)started);
-          const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)mine.at, last);
-          const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)mine.before, last);
-          if (lane == e) {
-            at = a;
-            before = b;
-          }
-        }
-      }
-    }
-    int token = 0;
-    if (lane < count) {
-      const uint32_t key_at = at + (want - before);
-      token = (int)((key_at >> tile_bits << tile_bits) + (keys[key_at] & ((1u << tile_bits) - 1)));
-    }
-    const bool whole = it >= n_parts;
-    float* part = parts + (int64_t)it * width;
-    TO* out = dx + (int64_t)item.row * width;
-    // `n` columns from `col` on, each the sum of the wavefronts' in order.
-    auto join = [&](int64_t col, int n) {
-      __syncthreads();
-      for (int c = threadIdx.x; c < n; c += kChunkBlock) {
-        float total[1] = {sums[0][c]};
-#pragma unroll
-        for (int k = 1; k < kChunkWaves; ++k) total[0] += sums[k][c];
-        if (whole)
-          put_row<TO, 1>(out + col + c, total, scale, accumulate != 0);
-        else
-          part[col + c] = total[0];
-      }
-      __syncthreads();
-    };
-    const int64_t w = (int64_t)slice * kLanes;
-    if (w < words) {
-      float acc[1][kWide] = {};
-      add_words<TD, 1, kPerWave>(dy, width, w + lane, words, token, count, acc);
-#pragma unroll
-      for (int j = 0; j < kWide; ++j) sums[wave][lane * kWide + j] = acc[0][j];
-      const int64_t left = (words - w) * kWide;
-      join(w * kWide, (int)(left < kLanes * kWide ? left : kLanes * kWide));
-    }
-    if (slice == 0 && words * kWide < width) {
-      sums[wave][lane] = add_singles(dy, width, words * kWide + lane, token, count);
-      join(words * kWide, (int)(width - words * kWide));
-    }
+    sum_chunk(dy, keys, tile_bits, width, item, runs, (int)slice, scale, accumulate != 0, dx + (int64_t)item.row * width,
+              it < n_parts ? parts + (int64_t)it * width : nullptr);
   }
 }
 
@@ -788,8 +774,8 @@ __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale
 }
 
 constexpr int kFewRowsPerWave = 8;
-constexpr int64_t kMaxFindBlocks = 2048;  // eight per CU; a launch of more would only take longer to start
-constexpr int64_t kMaxSumBlocks = 1024;   // four of twice the size
+// Eight workgroups per CU; a launch of more would only take longer to start.
+constexpr int64_t kMaxFindBlocks = 2048, kMaxSumBlocks = 2048;
 
 template <typename TD, typename TO, typename Id>
 void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64_t width, float scale, int accumulate,
@@ -841,13 +827,13 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   const unsigned slices = (unsigned)((width / kWide + kLanes - 1) / kLanes > 0 ? (width / kWide + kLanes - 1) / kLanes : 1);
   const int64_t max_items = (l.max_singles + l.max_parts) * slices;
   const int64_t stride = (rows + kGroup - 1) / kGroup;  // wavefronts with short rows
-  const int64_t max_short = (stride * slices + kChunkWaves - 1) / kChunkWaves;
-  const unsigned chunk_blocks = (unsigned)(max_items < kMaxSumBlocks ? max_items : kMaxSumBlocks);
+  const int64_t max_short = (stride * slices + kWaves - 1) / kWaves, max_chunks = (max_items + kWaves - 1) / kWaves;
+  const unsigned chunk_blocks = (unsigned)(max_chunks < kMaxSumBlocks ? max_chunks : kMaxSumBlocks);
   const unsigned short_blocks = (unsigned)(max_short < kMaxSumBlocks ? max_short : kMaxSumBlocks);
-  hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kChunkBlock), 0, s, dy, keys, l.tile_bits,
+  hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kBlock), 0, s, dy, keys, l.tile_bits,
                      width, scale, accumulate, dx, taken, entries, counts, stride, rows, singles, items, runs,
                      parts, chunk_blocks, slices);
-  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_parts < 256 ? l.max_parts : 256)),
+  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_parts < 1024 ? l.max_parts : 1024)),
                      dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, parts);
 }
 

@@ -351,23 +351,29 @@ struct Grad {
 // kTwo: both sums are needed.  Otherwise one factor serves whatever is wanted: c0 is log2(e)/T with
 // hard == 0, or T == 1, or soft == 0 and c0 = log2(e).
 template <bool kTwo>
-__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, float m, float log_soft,
-                                        float log_hard) {
+__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, float m, float log2_soft,
+                                        float log2_hard) {
   Grad g;
   const float as = soft ? dloss * a.soft * a.temperature : 0.f, ah = hard ? dloss * a.hard : 0.f;
   g.m = m;
   g.c0 = c0;
   if constexpr (kTwo) {
-    g.l0 = log_soft * kLog2e;
+    g.l0 = log2_soft;
     g.a0 = as;
-    g.l1 = log_hard * kLog2e;
+    g.l1 = log2_hard;
     g.a1 = ah;
   } else {
-    g.l0 = (soft ? log_soft : log_hard) * kLog2e;
+    g.l0 = soft ? log2_soft : log2_hard;
     g.a0 = as + ah;
     g.l1 = g.a1 = 0.f;
   }
   return g;
+}
+
+template <bool kTwo>
+__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, const Sums<kTwo>& s) {
+  const float log2_soft = s.m == -INFINITY ? NAN : __builtin_amdgcn_logf(s.s0);  // base 2
+  return grad_of<kTwo>(a, c0, dloss, soft, hard, s.m, log2_soft, kTwo ? __builtin_amdgcn_logf(s.s1) : log2_soft);
 }
 
 // The columns a row's targets correct.  Entries with the same column are taken together by the
@@ -485,11 +491,11 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   if ((int)blockIdx.x == splits - 1) put_zeros<T, kGradBlock>(out_row + a.vocab, out_width - a.vocab);
   Grad g;
   if (parts) {
-    const RowSums s = row_sums_of(join_parts<kTwo>(parts, row, splits, c0));
-    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, s.m, (float)s.log_soft, (float)s.log_hard);
-    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, s, loss, nullptr);
+    const Sums<kTwo> s = join_parts<kTwo>(parts, row, splits, c0);
+    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, s);
+    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, nullptr);
   } else {
-    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1], stats[row * 3 + 2]);
+    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
   }
   if (!t.any && label < 0) {
     put_zeros<T, kGradBlock>(out_row + from, count);
@@ -531,7 +537,7 @@ constexpr int kStepMaxWords16 = 16, kStepMaxWords32 = 8;  // words per thread th
 
 // Loss and gradient of a row that fits kWords words per thread.
 template <typename T, bool kTwo, int kWords>
-__global__ __launch_bounds__(kStepBlock) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
+__global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 : 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
                                                        T* dlogits, int64_t out_width, int log2_slots) {
   constexpr int kWaves = kStepBlock / kLanes;
   __shared__ float red[2][kWaves][3];
@@ -608,8 +614,7 @@ __global__ __launch_bounds__(kStepBlock) void row_step(Task a, float c0, const f
   }
 #pragma unroll
   for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
-  const RowSums rs = row_sums_of(sums);
-  const Grad g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, rs.m, (float)rs.log_soft, (float)rs.log_hard);
+  const Grad g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, sums);
 #pragma unroll
   for (int u = 0; u < kWords; ++u) {
     const int w = i + u * kStepBlock;
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(kStepBlock) void row_step(Task a, float c0, const f
     }
   }
   if (single) Wide<T>::put(out + single_at, g.template at<kTwo>(x1));
-  if (i < kLanes) finish_row<T>(a, row, t, label, rs, loss, nullptr);
+  if (i < kLanes) finish_row<T>(a, row, t, label, row_sums_of(sums), loss, nullptr);
   __syncthreads();
   put_picks<T, kTwo, kStepBlock>(picks, g, z, out);
 }
@@ -860,16 +865,24 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
                              loss, static_cast<T*>(dlogits), out_width, picks_log2_slots(t.topk));
         };
         const int words = words_per_thread(a.vocab);
-        if (words <= 1)
-          go(row_step<T, kTwo, 1>);
-        else if (words <= 2)
-          go(row_step<T, kTwo, 2>);
-        else if (words <= 4)
-          go(row_step<T, kTwo, 4>);
-        else if (words <= 8)
-          go(row_step<T, kTwo, 8>);
-        else if constexpr (sizeof(T) == 2)
-          go(row_step<T, kTwo, 16>);
+        switch (words) {
+          case 0:
+          case 1: go(row_step<T, kTwo, 1>); break;
+          case 2: go(row_step<T, kTwo, 2>); break;
+          case 3: go(row_step<T, kTwo, 3>); break;
+          case 4: go(row_step<T, kTwo, 4>); break;
+          case 5: go(row_step<T, kTwo, 5>); break;
+          case 6: go(row_step<T, kTwo, 6>); break;
+          case 7: go(row_step<T, kTwo, 7>); break;
+          case 8: go(row_step<T, kTwo, 8>); break;
+          default:
+            if constexpr (sizeof(T) == 2) {
+              if (words <= 12)
+                go(row_step<T, kTwo, 12>);
+              else
+                go(row_step<T, kTwo, 16>);
+            }
+        }
         return;
       }
       const int splits = splits_of(a.rows, a.vocab), per = columns_per_split(a.rows, a.vocab, a.vocab);

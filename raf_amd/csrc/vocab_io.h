@@ -20,6 +20,7 @@ namespace rafhip {
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef f16x8 f16x8_any __attribute__((aligned(2)));
 typedef u16x8 u16x8_any __attribute__((aligned(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kWide = 8;  // elements per lane and access
 
@@ -81,11 +82,12 @@ struct Wide<Bf16> {
   }
   static __device__ __forceinline__ void keep_narrow(Raw& r) { asm volatile("" : "+v"(r)); }
   static __device__ __forceinline__ float get(const Raw& r, int j) { return bf16_widen(r[j]); }
+  // gfx950 narrows two at once, to nearest even as bf16_narrow does.
   static __device__ __forceinline__ void store(Bf16* p, const float (&v)[kWide]) {
-    u16x8 r;
+    bf16x8 r;
 #pragma unroll
-    for (int j = 0; j < kWide; ++j) r[j] = bf16_narrow(v[j]);
-    *(RAFHIP_GLOBAL u16x8_any*)p = r;
+    for (int j = 0; j < kWide; ++j) r[j] = (__bf16)v[j];
+    *(RAFHIP_GLOBAL u16x8_any*)p = __builtin_bit_cast(u16x8, r);
   }
   static __device__ __forceinline__ float one(const Bf16* p) {
     return bf16_widen(*(const RAFHIP_GLOBAL unsigned short*)p);
