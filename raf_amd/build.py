@@ -14,6 +14,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -58,8 +60,17 @@ def dialect_lib() -> Path:
 def build_optim() -> Path:
     LIB.mkdir(parents=True, exist_ok=True)
     out = optim_lib()
-    srcs = [CSRC / s for s in OPTIM_SOURCES]
-    _run([hipcc(), *HIP_FLAGS, "-shared", f"-I{INCLUDE}", f"-I{CSRC}", "-o", out, *srcs])
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [Path(tmp) / (Path(s).stem + ".o") for s in OPTIM_SOURCES]
+
+        def compile_one(job):
+            src, obj = job
+            _run([hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", "-o", obj, CSRC / src])
+
+        # the files with many kernel variants take most of a minute each
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(compile_one, zip(OPTIM_SOURCES, objs)))
+        _run([hipcc(), *HIP_FLAGS, "-shared", "-o", out, *objs])
     return out
 
 

@@ -111,8 +111,9 @@ struct Layout {
   int buckets = 0;
   int64_t max_singles = 0;  // rows of more than kDirect tokens and no more than a chunk
   int64_t max_runs = 0;   // runs of them
-  int64_t max_parts = 0;  // chunks of rows with more than one
-  int64_t keys_at = 0, index_at = 0, taken_at = 0, entries_at = 0, counts_at = 0, singles_at = 0, items_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
+  int64_t max_long = 0;   // rows of more than one chunk
+  int64_t max_parts = 0;  // their chunks
+  int64_t keys_at = 0, index_at = 0, taken_at = 0, entries_at = 0, counts_at = 0, singles_at = 0, items_at = 0, long_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
 };
 
 // One chunk of a row of more than kDirect tokens, with all that its sum needs to know.  There are two
@@ -153,13 +154,14 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   const int64_t listed = n / (kDirect + 1);
   l->max_singles = listed;
   l->max_runs = n < listed * tiles ? n : listed * tiles;
-  l->max_parts = n / kChunk + n / (kChunk + 1);
+  l->max_long = n / (kChunk + 1);
+  l->max_parts = n / kChunk + l->max_long;
   auto place = [&](int64_t bytes) {
     const int64_t at = l->bytes;
     l->bytes += align256(bytes);
     return at;
   };
-  l->taken_at = place(sizeof(Taken));
+  l->taken_at = place(2 * sizeof(Taken));  // and how many rows of more than one chunk there are
   l->keys_at = place((tiles << bits) * 4);
   // About one key per entry, or 16 rows where the keys are many: a search then takes a step or two.
   int bucket = row_bits - bits;
@@ -171,6 +173,7 @@ bool layout_of(int64_t n, int64_t rows, int64_t width, Layout* l) {
   l->counts_at = place(rows * 4);
   l->singles_at = place(l->max_singles * (int64_t)sizeof(Item));
   l->items_at = place(l->max_parts * (int64_t)sizeof(Item));
+  l->long_at = place(l->max_long * 4);
   l->runs_at = place(l->max_runs * (int64_t)sizeof(Run));
   l->parts_at = place(l->max_parts * width * 4);
   return true;
@@ -224,7 +227,7 @@ __global__ __launch_bounds__(kThreads) void tile_sort(const Id* ids, int64_t n, 
   __shared__ uint32_t lds[kSize];
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * kSize;
-  if (blockIdx.x == 0 && tid == 0) *taken = 0;
+  if (blockIdx.x == 0 && tid < 2) taken[tid] = 0;
   uint32_t v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
@@ -451,7 +454,7 @@ template <typename TO, int kSlots, int kRounds>
 __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const uint16_t* index, int tiles, int tile_bits,
                                                     int bucket_bits, int buckets, int64_t rows, int64_t width,
                                                     int accumulate, TO* dx, Taken* taken, uint32_t* entries,
-                                                    uint32_t* counts, Item* singles, Item* items, Run* runs) {
+                                                    uint32_t* counts, Item* singles, Item* items, uint32_t* long_rows, Run* runs) {
   constexpr int kSpread = kLanes / kSlots;
   const int lane = threadIdx.x & (kLanes - 1);
   const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
@@ -581,6 +584,7 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
         Item* list = chunks == 1 ? singles + singles_of(first) : items + parts_of(first);
         for (int c = lane; c < chunks; c += kLanes)
           list[c] = Item{(uint32_t)row, (uint32_t)count, (uint32_t)n_runs, first_run, (uint32_t)c};
+        if (chunks > 1 && lane == 0) long_rows[atomicAdd((uint32_t*)(taken + 1), 1u)] = parts_of(first);
         first += take(n_runs, chunks);
       }
     }
@@ -738,15 +742,16 @@ __global__ __launch_bounds__(kBlock) void sum_rows(const TD* dy, const uint32_t*
 // The chunks of a long row added in order: 64 columns per workgroup, four stretches of chunks.
 template <typename TO>
 __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale, int accumulate, TO* dx,
-                                                     const Taken* taken, const Item* items, const float* parts) {
+                                                     const Taken* taken, const Item* items, const uint32_t* long_rows,
+                                                      const float* parts) {
   __shared__ float sums[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   const int64_t col = (int64_t)blockIdx.x * kLanes + lane;
-  const uint32_t n_parts = parts_of(*taken);
-  for (uint32_t it = blockIdx.y; it < n_parts; it += gridDim.y) {
+  const uint32_t n_long = (uint32_t)taken[1];
+  for (uint32_t h = blockIdx.y; h < n_long; h += gridDim.y) {
+    const uint32_t it = long_rows[h];  // its first chunk and partial sum
     const Item row = items[it];
-    if (row.chunk != 0) continue;  // the first chunk stands for its row
     const int chunks = (int)((row.tokens + kChunk - 1) / kChunk);
     const int per = (chunks + kWaves - 1) / kWaves;
     const int from = wave * per, to = from + per < chunks ? from + per : chunks;
@@ -794,6 +799,7 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   auto* counts = reinterpret_cast<uint32_t*>(ws + l.counts_at);
   auto* singles = reinterpret_cast<Item*>(ws + l.singles_at);
   auto* items = reinterpret_cast<Item*>(ws + l.items_at);
+  auto* long_rows = reinterpret_cast<uint32_t*>(ws + l.long_at);
   auto* runs = reinterpret_cast<Run*>(ws + l.runs_at);
   auto* parts = reinterpret_cast<float*>(ws + l.parts_at);
   auto sort = [&](auto kernel) {
@@ -812,7 +818,7 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   const unsigned find_blocks = (unsigned)(max_blocks < kMaxFindBlocks ? max_blocks : kMaxFindBlocks);
   auto find = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(find_blocks), dim3(kBlock), 0, s, keys, index, l.tiles, l.tile_bits, l.bucket_bits,
-                       l.buckets, rows, width, accumulate, dx, taken, entries, counts, singles, items, runs);
+                       l.buckets, rows, width, accumulate, dx, taken, entries, counts, singles, items, long_rows, runs);
   };
   if (l.tiles <= 8)
     find(find_rows<TO, kGroup, 1>);
@@ -833,8 +839,8 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kBlock), 0, s, dy, keys, l.tile_bits,
                      width, scale, accumulate, dx, taken, entries, counts, stride, rows, singles, items, runs,
                      parts, chunk_blocks, slices);
-  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_parts < 1024 ? l.max_parts : 1024)),
-                     dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, parts);
+  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_long < 128 ? l.max_long : 128)),
+                     dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, long_rows, parts);
 }
 
 int check_common(const char* who, int32_t a_dtype, int32_t b_dtype, int64_t rows, int64_t width, int32_t index_bits, int64_t n,

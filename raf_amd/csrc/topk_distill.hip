@@ -114,10 +114,17 @@ __device__ __forceinline__ Teacher teacher_of(const Task& a, int64_t row) {
   return r;
 }
 
-// Running maximum and sums of exp((z - m)/T) and, kTwo, exp(z - m) over the columns a lane has seen.
-// With one sum the factor is c_soft, or log2(e) if only the hard term is wanted.
-template <bool kTwo>
-struct Sums {
+// Which sums a row needs.  kOne: a single factor serves whatever is wanted -- T == 1, or only one of the
+// two terms.  Else both exp((z - m)/T) and exp(z - m); for the temperatures 2 and 4 the second is a
+// power of the first, which saves an exponential (a quarter-rate instruction) per element and pass:
+// 8192 rows of 50257 in 16 bits, loss and gradient at once, take SQUARE_US with the square and
+// 460 us with two exponentials, which is then what bounds them.
+enum { kOne = 0, kBoth, kSquare, kFourth };
+
+// Running maximum and sums over the columns a lane has seen.  c0 is log2(e)/T, or log2(e) if only the
+// hard term is wanted.
+template <int kSums>
+struct Exps {
   float m = -INFINITY;
   float s0 = 0.f, s1 = 0.f;
 
@@ -125,33 +132,40 @@ struct Sums {
   // -inf - -inf does not arise.
   static __device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.f : m; }
 
+  // exp(d) where e = exp(d / T).
+  static __device__ __forceinline__ float hard(float d, float e) {
+    if constexpr (kSums == kSquare) return e * e;
+    if constexpr (kSums == kFourth) return (e * e) * (e * e);
+    return exp2_hw(d * kLog2e);
+  }
+
   __device__ __forceinline__ void rescale(float m2, float c0) {
-    const float d = m - base(m2);
-    s0 *= exp2_hw(d * c0);
-    if constexpr (kTwo) s1 *= exp2_hw(d * kLog2e);
+    const float d = m - base(m2), e = exp2_hw(d * c0);
+    s0 *= e;
+    if constexpr (kSums != kOne) s1 *= hard(d, e);
     m = m2;
   }
   __device__ __forceinline__ void term(float z, float b, float c0) {
-    const float d = z - b;
-    s0 += exp2_hw(d * c0);
-    if constexpr (kTwo) s1 += exp2_hw(d * kLog2e);
+    const float d = z - b, e = exp2_hw(d * c0);
+    s0 += e;
+    if constexpr (kSums != kOne) s1 += hard(d, e);
   }
   __device__ __forceinline__ void merge(float om, float o0, float o1, float c0) {
     rescale(fmaxf(m, om), c0);
-    const float d = om - base(m);
-    s0 += o0 * exp2_hw(d * c0);
-    if constexpr (kTwo) s1 += o1 * exp2_hw(d * kLog2e);
+    const float d = om - base(m), e = exp2_hw(d * c0);
+    s0 += o0 * e;
+    if constexpr (kSums != kOne) s1 += o1 * hard(d, e);
   }
   __device__ __forceinline__ void wave_merge(float c0) {
     rescale(wave_max(m), c0);
     s0 = wave_add(s0);
-    if constexpr (kTwo) s1 = wave_add(s1);
+    if constexpr (kSums != kOne) s1 = wave_add(s1);
   }
 };
 
 // Joined over the workgroup, the same in every thread; `red` holds three floats per wavefront.
-template <int kWaves, bool kTwo>
-__device__ __forceinline__ void block_merge(Sums<kTwo>& a, float (*red)[3], float c0) {
+template <int kWaves, int kSums>
+__device__ __forceinline__ void block_merge(Exps<kSums>& a, float (*red)[3], float c0) {
   a.wave_merge(c0);
   if ((threadIdx.x & (kLanes - 1)) == 0) {
     float* r = red[threadIdx.x / kLanes];
@@ -160,7 +174,7 @@ __device__ __forceinline__ void block_merge(Sums<kTwo>& a, float (*red)[3], floa
     r[2] = a.s1;
   }
   __syncthreads();
-  Sums<kTwo> all;
+  Exps<kSums> all;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) all.merge(red[w][0], red[w][1], red[w][2], c0);
   a = all;
@@ -183,8 +197,8 @@ __device__ __forceinline__ Stretch stretch_of(const T* at, int count) {
 }
 
 // The sums over `count` columns at z, by kBlock threads.
-template <typename T, bool kTwo, int kBlock>
-__device__ __forceinline__ void add_columns(Sums<kTwo>& a, const T* z, int count, float c0) {
+template <typename T, int kSums, int kBlock>
+__device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int count, float c0) {
   constexpr int kInFlight = 4;
   const Stretch s = stretch_of(z, count);
   for (int w0 = threadIdx.x; w0 < s.words; w0 += kBlock * kInFlight) {
@@ -203,7 +217,7 @@ __device__ __forceinline__ void add_columns(Sums<kTwo>& a, const T* z, int count
       for (int j = 0; j < kWide; ++j) top = fmaxf(top, Wide<T>::get(raw[u], j));
     }
     a.rescale(top, c0);
-    const float b = Sums<kTwo>::base(top);
+    const float b = Exps<kSums>::base(top);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (w0 + u * kBlock < s.words) {
@@ -217,7 +231,7 @@ __device__ __forceinline__ void add_columns(Sums<kTwo>& a, const T* z, int count
   if (i < s.head + s.tail) {
     const float x = Wide<T>::one(z + (i < s.head ? i : s.tail_at + i - s.head));
     a.rescale(fmaxf(a.m, x), c0);
-    a.term(x, Sums<kTwo>::base(a.m), c0);
+    a.term(x, Exps<kSums>::base(a.m), c0);
   }
 }
 
@@ -226,12 +240,12 @@ struct RowSums {
   float m;
   double log_soft, log_hard;  // log S_T, log S_1
 };
-template <bool kTwo>
-__device__ __forceinline__ RowSums row_sums_of(const Sums<kTwo>& s) {
+template <int kSums>
+__device__ __forceinline__ RowSums row_sums_of(const Exps<kSums>& s) {
   RowSums r;
   r.m = s.s0 != s.s0 && s.m != INFINITY ? NAN : s.m;  // the running maximum passes over a NaN
   r.log_soft = s.m == -INFINITY ? (double)NAN : log((double)s.s0);  // nothing but -inf has no softmax
-  r.log_hard = kTwo && s.m != -INFINITY ? log((double)s.s1) : r.log_soft;
+  r.log_hard = kSums != kOne && s.m != -INFINITY ? log((double)s.s1) : r.log_soft;
   return r;
 }
 
@@ -269,18 +283,18 @@ __device__ __forceinline__ void finish_row(const Task& a, int64_t row, const Tea
   }
 }
 
-constexpr int kLossBlock = 512;
+constexpr int kLossBlock = 256;
 
-template <typename T, bool kTwo>
+template <typename T, int kSums>
 __global__ __launch_bounds__(kLossBlock) void row_loss(Task a, float c0, float* loss, float* stats) {
   constexpr int kWaves = kLossBlock / kLanes;
   __shared__ float red[kWaves][3];
   const int64_t row = blockIdx.x;
   const Teacher t = teacher_of(a, row);
   const int label = a.label(row);
-  Sums<kTwo> s;
+  Exps<kSums> s;
   if (t.any || label >= 0) {  // the same in all threads
-    add_columns<T, kTwo, kLossBlock>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
+    add_columns<T, kSums, kLossBlock>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
     block_merge<kWaves>(s, red, c0);
   }
   if (threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, stats);
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(kLossBlock) void row_loss(Task a, float c0, float* 
 constexpr int kPartBlock = 256;
 
 // Columns [split * per_split, ...) of a row: partial sums to parts[row][split][4].
-template <typename T, bool kTwo>
+template <typename T, int kSums>
 __global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per_split, float* parts) {
   constexpr int kWaves = kPartBlock / kLanes;
   __shared__ float red[kWaves][3];
@@ -301,9 +315,9 @@ __global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per
     float t;
     any = a.entry(row, j, &t) >= 0;
   }
-  Sums<kTwo> s;
+  Exps<kSums> s;
   if (__any(any)) {
-    add_columns<T, kTwo, kPartBlock>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
+    add_columns<T, kSums, kPartBlock>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
     block_merge<kWaves>(s, red, c0);
   }
   if (threadIdx.x == 0) {
@@ -315,9 +329,9 @@ __global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per
 }
 
 // The sums of a row from its parts, by a wavefront (the same in all lanes).
-template <bool kTwo>
-__device__ __forceinline__ Sums<kTwo> join_parts(const float* parts, int64_t row, int splits, float c0) {
-  Sums<kTwo> s;
+template <int kSums>
+__device__ __forceinline__ Exps<kSums> join_parts(const float* parts, int64_t row, int splits, float c0) {
+  Exps<kSums> s;
   const int lane = threadIdx.x & (kLanes - 1);
   for (int i = lane; i < splits; i += kLanes) {
     const float* p = parts + (row * splits + i) * 4;
@@ -327,41 +341,43 @@ __device__ __forceinline__ Sums<kTwo> join_parts(const float* parts, int64_t row
   return s;
 }
 
-template <typename T, bool kTwo>
+template <typename T, int kSums>
 __global__ __launch_bounds__(kLanes) void join_loss(Task a, float c0, const float* parts, int splits, float* loss,
                                                     float* stats) {
   const int64_t row = blockIdx.x;
   const Teacher t = teacher_of(a, row);
-  finish_row<T>(a, row, t, a.label(row), row_sums_of(join_parts<kTwo>(parts, row, splits, c0)), loss, stats);
+  finish_row<T>(a, row, t, a.label(row), row_sums_of(join_parts<kSums>(parts, row, splits, c0)), loss, stats);
 }
 
 // ------------------------------------------------------------------------------------ gradient
-// g(z) = a0 exp2((z - m) c0 - l0) [+ a1 exp2((z - m) log2(e) - l1)], before the corrections.
+// g(z) = a0 exp2((z - m) c0 - l0) [+ a1 exp2((z - m) log2(e) - l1)], before the corrections.  Where the
+// second exponential is a power of the first, a1 holds the factor of that power.
 struct Grad {
   float m, c0, l0, a0, l1, a1;
-  template <bool kTwo>
+  template <int kSums>
   __device__ __forceinline__ float at(float z) const {
-    const float d = z - m;
-    float g = a0 * exp2_hw(fmaf(d, c0, -l0));
-    if constexpr (kTwo) g += a1 * exp2_hw(fmaf(d, kLog2e, -l1));
-    return g;
+    const float d = z - m, e = exp2_hw(fmaf(d, c0, -l0));
+    if constexpr (kSums == kSquare) return e * fmaf(a1, e, a0);
+    if constexpr (kSums == kFourth) return e * fmaf(a1 * e, e * e, a0);
+    if constexpr (kSums == kBoth) return fmaf(a1, exp2_hw(fmaf(d, kLog2e, -l1)), a0 * e);
+    return a0 * e;
   }
 };
 
-// kTwo: both sums are needed.  Otherwise one factor serves whatever is wanted: c0 is log2(e)/T with
-// hard == 0, or T == 1, or soft == 0 and c0 = log2(e).
-template <bool kTwo>
+template <int kSums>
 __device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, float m, float log2_soft,
                                         float log2_hard) {
   Grad g;
   const float as = soft ? dloss * a.soft * a.temperature : 0.f, ah = hard ? dloss * a.hard : 0.f;
   g.m = m;
   g.c0 = c0;
-  if constexpr (kTwo) {
+  if constexpr (kSums != kOne) {
     g.l0 = log2_soft;
     g.a0 = as;
     g.l1 = log2_hard;
     g.a1 = ah;
+    if constexpr (kSums == kSquare || kSums == kFourth)
+      g.a1 = hard ? ah * exp2_hw((kSums == kSquare ? 2.f : 4.f) * log2_soft - log2_hard) : 0.f;
   } else {
     g.l0 = soft ? log2_soft : log2_hard;
     g.a0 = as + ah;
@@ -370,10 +386,10 @@ __device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bo
   return g;
 }
 
-template <bool kTwo>
-__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, const Sums<kTwo>& s) {
+template <int kSums>
+__device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bool soft, bool hard, const Exps<kSums>& s) {
   const float log2_soft = s.m == -INFINITY ? NAN : __builtin_amdgcn_logf(s.s0);  // base 2
-  return grad_of<kTwo>(a, c0, dloss, soft, hard, s.m, log2_soft, kTwo ? __builtin_amdgcn_logf(s.s1) : log2_soft);
+  return grad_of<kSums>(a, c0, dloss, soft, hard, s.m, log2_soft, kSums != kOne ? __builtin_amdgcn_logf(s.s1) : log2_soft);
 }
 
 // The columns a row's targets correct.  Entries with the same column are taken together by the
@@ -442,7 +458,7 @@ __device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Tea
 }
 
 // Writes the corrected columns, behind a barrier that follows list_picks and the plain columns.
-template <typename T, bool kTwo, int kBlock>
+template <typename T, int kSums, int kBlock>
 __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T* z, T* out) {
   const bool twice = *p.twice != 0;
   for (int j = threadIdx.x; j < p.n; j += kBlock) {
@@ -456,7 +472,7 @@ __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T
       for (int i = j + 1; i < p.n; ++i)
         if (p.at[i] == at) minus += p.minus[i];
     }
-    Wide<T>::put(out + at, g.template at<kTwo>(Wide<T>::one(z + at)) - minus);
+    Wide<T>::put(out + at, g.template at<kSums>(Wide<T>::one(z + at)) - minus);
   }
 }
 
@@ -472,7 +488,7 @@ constexpr int kGradBlock = 256;
 
 // Columns [split * per_split, ...) of a row.  With `parts` the row's sums are joined from them and
 // the first split writes the loss; otherwise they come from `stats`.
-template <typename T, bool kTwo>
+template <typename T, int kSums>
 __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per_split, const float* dloss, int dloss_step,
                                                        const float* stats, const float* parts, float* loss, T* dlogits,
                                                        int64_t out_width, int log2_slots) {
@@ -491,11 +507,11 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   if ((int)blockIdx.x == splits - 1) put_zeros<T, kGradBlock>(out_row + a.vocab, out_width - a.vocab);
   Grad g;
   if (parts) {
-    const Sums<kTwo> s = join_parts<kTwo>(parts, row, splits, c0);
-    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, s);
+    const Exps<kSums> s = join_parts<kSums>(parts, row, splits, c0);
+    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, s);
     if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, nullptr);
   } else {
-    g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
+    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
   }
   if (!t.any && label < 0) {
     put_zeros<T, kGradBlock>(out_row + from, count);
@@ -518,7 +534,7 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
       if (w < s.words) {
         float v[kWide];
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) v[j] = g.template at<kTwo>(Wide<T>::get(raw[u], j));
+        for (int j = 0; j < kWide; ++j) v[j] = g.template at<kSums>(Wide<T>::get(raw[u], j));
         Wide<T>::store(out + s.head + (int64_t)w * kWide, v);
       }
     }
@@ -526,17 +542,18 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   const int i = (int)threadIdx.x;
   if (i < s.head + s.tail) {
     const int c = i < s.head ? i : s.tail_at + i - s.head;
-    Wide<T>::put(out + c, g.template at<kTwo>(Wide<T>::one(z + c)));
+    Wide<T>::put(out + c, g.template at<kSums>(Wide<T>::one(z + c)));
   }
   __syncthreads();
-  put_picks<T, kTwo, kGradBlock>(picks, g, z_row, out_row);
+  put_picks<T, kSums, kGradBlock>(picks, g, z_row, out_row);
 }
 
 constexpr int kStepBlock = 1024;
 constexpr int kStepMaxWords16 = 16, kStepMaxWords32 = 8;  // words per thread that stay in registers
+constexpr int kOneByOne = 8, kStepWords = 4;  // there are kernels for 1 to 8 words, and for 12 and 16
 
 // Loss and gradient of a row that fits kWords words per thread.
-template <typename T, bool kTwo, int kWords>
+template <typename T, int kSums, int kWords>
 __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 : 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
                                                        T* dlogits, int64_t out_width, int log2_slots) {
   constexpr int kWaves = kStepBlock / kLanes;
@@ -559,12 +576,20 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
     if (i == 0) loss[row] = 0.f;
     return;
   }
+  // Word u of a thread lies a fixed distance behind word 0, so one register of offset serves them all.
+  // The first kSure words exist in every thread (words_per_thread).
+  constexpr int kPitch = kStepBlock * kWide, kSure = kWords <= kOneByOne ? kWords - 1 : kWords - kStepWords;
+  auto exists = [&](int u) { return u < kSure || i + u * kStepBlock < s.words; };
+  const uint32_t off = (uint32_t)i * (kWide * sizeof(T));
+  const T* z0 = z + s.head;
+  T* out0 = out + s.head;
+  auto word_of = [&](const T* base, int u) { return (const T*)((const char*)(base + u * kPitch) + off); };
   typename Wide<T>::Raw raw[kWords];
   if (s.words > 0) {
 #pragma unroll
     for (int u = 0; u < kWords; ++u) {
-      const int w = i + u * kStepBlock < s.words ? i + u * kStepBlock : s.words - 1;
-      raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
+      const int w = i + u * kStepBlock;
+      raw[u] = Wide<T>::load(u < kSure ? word_of(z0, u) : z0 + (int64_t)(w < s.words ? w : s.words - 1) * kWide);
     }
   } else {
 #pragma unroll
@@ -588,19 +613,19 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   // phases they leave room for two workgroups per CU.
 #pragma unroll
   for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
-  Sums<kTwo> sums;
+  Exps<kSums> sums;
   sums.m = top;
-  const float b = Sums<kTwo>::base(top);
+  const float b = Exps<kSums>::base(top);
 #pragma unroll
   for (int u = 0; u < kWords; ++u) {
-    if (i + u * kStepBlock < s.words) {
+    if (exists(u)) {
 #pragma unroll
       for (int j = 0; j < kWide; ++j) sums.term(Wide<T>::get(raw[u], j), b, c0);
     }
   }
   if (single) sums.term(x1, b, c0);
   sums.s0 = wave_add(sums.s0);
-  if constexpr (kTwo) sums.s1 = wave_add(sums.s1);
+  if constexpr (kSums != kOne) sums.s1 = wave_add(sums.s1);
   if ((i & (kLanes - 1)) == 0) {
     red[1][i / kLanes][0] = sums.s0;
     red[1][i / kLanes][1] = sums.s1;
@@ -614,27 +639,26 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   }
 #pragma unroll
   for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
-  const Grad g = grad_of<kTwo>(a, c0, dl, t.any, label >= 0, sums);
+  const Grad g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, sums);
 #pragma unroll
   for (int u = 0; u < kWords; ++u) {
-    const int w = i + u * kStepBlock;
-    if (w < s.words) {
+    if (exists(u)) {
       float v[kWide];
 #pragma unroll
-      for (int j = 0; j < kWide; ++j) v[j] = g.template at<kTwo>(Wide<T>::get(raw[u], j));
-      Wide<T>::store(out + s.head + (int64_t)w * kWide, v);
+      for (int j = 0; j < kWide; ++j) v[j] = g.template at<kSums>(Wide<T>::get(raw[u], j));
+      Wide<T>::store(const_cast<T*>(word_of(out0, u)), v);
     }
   }
-  if (single) Wide<T>::put(out + single_at, g.template at<kTwo>(x1));
+  if (single) Wide<T>::put(out + single_at, g.template at<kSums>(x1));
   if (i < kLanes) finish_row<T>(a, row, t, label, row_sums_of(sums), loss, nullptr);
   __syncthreads();
-  put_picks<T, kTwo, kStepBlock>(picks, g, z, out);
+  put_picks<T, kSums, kStepBlock>(picks, g, z, out);
 }
 
 // ---------------------------------------------------------------------------------------- host
 constexpr int kWantBlocks = 1024;     // four workgroups for each of 256 CUs
 constexpr int kMinPerSplit = 4096;    // columns below which another workgroup does not pay
-constexpr int kGradColumns = 16384;   // columns of a row_grad workgroup where rows are plenty
+constexpr int kGradColumns = 8192;    // columns of a row_grad workgroup where rows are plenty
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -651,6 +675,9 @@ int columns_per_split(int64_t rows, int64_t vocab, int64_t most) {
 bool rows_are_split(int64_t rows, int64_t vocab) { return rows < kWantBlocks / 2 && vocab > kMinPerSplit; }
 int splits_of(int64_t rows, int64_t vocab) { return (int)ceil_div(vocab, columns_per_split(rows, vocab, vocab)); }
 
+// Words of a thread in row_step.  All but the last exist in every thread, whether or not the row starts
+// with a single element: vocab / kWide is at least (result - 1) * kStepBlock + 1, and a row has that
+// many words or one less.
 int words_per_thread(int64_t vocab) { return (int)ceil_div(vocab / kWide, kStepBlock); }
 bool row_fits(int64_t vocab, int32_t dtype) {
   return words_per_thread(vocab) <= (dtype == RAFHIP_F32 ? kStepMaxWords32 : kStepMaxWords16);
@@ -704,7 +731,7 @@ int check_gradient(const char* who, const rafhip_topk_distill_args& a, const flo
 }
 
 // A term that cannot matter is dropped here, so that the kernels neither read for it nor sum for it.
-Task task_of(const rafhip_topk_distill_args& a, bool* two, float* c0) {
+Task task_of(const rafhip_topk_distill_args& a, int* mode, float* c0) {
   Task t;
   t.logits = a.logits;
   t.indices = a.topk_indices;
@@ -721,17 +748,24 @@ Task task_of(const rafhip_topk_distill_args& a, bool* two, float* c0) {
   t.hard = a.hard_weight;
   t.c_soft = (float)(1.44269504088896340736 / (double)a.temperature);
   const bool soft = t.topk > 0, hard = t.labels != nullptr;
-  *two = soft && hard && a.temperature != 1.f;
+  *mode = !soft || !hard || a.temperature == 1.f ? kOne
+          : a.temperature == 2.f                    ? kSquare
+          : a.temperature == 4.f                    ? kFourth
+                                                    : kBoth;
   *c0 = soft ? t.c_soft : kLog2e;
   return t;
 }
 
 template <typename F>
-void with_flag(bool flag, F&& f) {
-  if (flag)
-    f(std::true_type{});
+void with_sums(int mode, F&& f) {
+  if (mode == kOne)
+    f(std::integral_constant<int, kOne>{});
+  else if (mode == kBoth)
+    f(std::integral_constant<int, kBoth>{});
+  else if (mode == kSquare)
+    f(std::integral_constant<int, kSquare>{});
   else
-    f(std::false_type{});
+    f(std::integral_constant<int, kFourth>{});
 }
 
 constexpr int64_t kMaxGridY = 65535;
@@ -779,23 +813,23 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
   const bool split = rows_are_split(a.rows, a.vocab);
   const int64_t need = split ? rafhip_topk_distill_workspace_bytes(args) : 0;
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
-  bool two;
+  int sums;
   float c0;
-  const Task t = task_of(a, &two, &c0);
+  const Task t = task_of(a, &sums, &c0);
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_element(a.logits_dtype, [&](auto e) {
-    with_flag(two, [&](auto flag) {
+    with_sums(sums, [&](auto mode) {
       using T = decltype(e);
-      constexpr bool kTwo = decltype(flag)::value;
+      constexpr int kSums = decltype(mode)::value;
       if (!split) {
-        hipLaunchKernelGGL((row_loss<T, kTwo>), dim3((unsigned)a.rows), dim3(kLossBlock), 0, s, t, c0, loss, stats);
+        hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)a.rows), dim3(kLossBlock), 0, s, t, c0, loss, stats);
         return;
       }
       float* parts = static_cast<float*>(workspace);
       const int splits = splits_of(a.rows, a.vocab);
-      hipLaunchKernelGGL((row_part<T, kTwo>), dim3((unsigned)splits, (unsigned)a.rows), dim3(kPartBlock), 0, s, t, c0,
+      hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)a.rows), dim3(kPartBlock), 0, s, t, c0,
                          columns_per_split(a.rows, a.vocab, a.vocab), parts);
-      hipLaunchKernelGGL((join_loss<T, kTwo>), dim3((unsigned)a.rows), dim3(kLanes), 0, s, t, c0, parts, splits, loss, stats);
+      hipLaunchKernelGGL((join_loss<T, kSums>), dim3((unsigned)a.rows), dim3(kLanes), 0, s, t, c0, parts, splits, loss, stats);
     });
   });
   RAFHIP_HIP_TRY(hipGetLastError());
@@ -813,19 +847,19 @@ extern "C" int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, cons
   if (a.rows == 0 || out_width == 0) return RAFHIP_OK;
   if (int st = check_pointers(who, a)) return st;
   if (!stats || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: stats %p", who, (const void*)stats);
-  bool two;
+  int sums;
   float c0;
-  const Task t = task_of(a, &two, &c0);
+  const Task t = task_of(a, &sums, &c0);
   const int per = columns_per_split(a.rows, a.vocab, kGradColumns);
   const unsigned splits = (unsigned)(a.vocab > 0 ? ceil_div(a.vocab, per) : 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_element(a.logits_dtype, [&](auto e) {
-    with_flag(two, [&](auto flag) {
+    with_sums(sums, [&](auto mode) {
       using T = decltype(e);
-      constexpr bool kTwo = decltype(flag)::value;
+      constexpr int kSums = decltype(mode)::value;
       for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
         const int step = dloss_count == 1 ? 0 : 1;
-        hipLaunchKernelGGL((row_grad<T, kTwo>), dim3(splits, (unsigned)part.rows), dim3(kGradBlock),
+        hipLaunchKernelGGL((row_grad<T, kSums>), dim3(splits, (unsigned)part.rows), dim3(kGradBlock),
                            picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, stats + r0 * 3,
                            (const float*)nullptr, (float*)nullptr, static_cast<T*>(dlogits) + r0 * out_width, out_width,
                            picks_log2_slots(t.topk));
@@ -850,15 +884,15 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
   if (!loss || !is_aligned(loss, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss %p", who, (const void*)loss);
   const int64_t need = rafhip_topk_distill_workspace_bytes(args);
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
-  bool two;
+  int sums;
   float c0;
-  const Task t = task_of(a, &two, &c0);
+  const Task t = task_of(a, &sums, &c0);
   const int step = dloss_count == 1 ? 0 : 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_element(a.logits_dtype, [&](auto e) {
-    with_flag(two, [&](auto flag) {
+    with_sums(sums, [&](auto mode) {
       using T = decltype(e);
-      constexpr bool kTwo = decltype(flag)::value;
+      constexpr int kSums = decltype(mode)::value;
       if (need == 0) {
         auto go = [&](auto kernel) {
           hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(kStepBlock), picks_bytes(t.topk), s, t, c0, dloss, step,
@@ -867,20 +901,20 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
         const int words = words_per_thread(a.vocab);
         switch (words) {
           case 0:
-          case 1: go(row_step<T, kTwo, 1>); break;
-          case 2: go(row_step<T, kTwo, 2>); break;
-          case 3: go(row_step<T, kTwo, 3>); break;
-          case 4: go(row_step<T, kTwo, 4>); break;
-          case 5: go(row_step<T, kTwo, 5>); break;
-          case 6: go(row_step<T, kTwo, 6>); break;
-          case 7: go(row_step<T, kTwo, 7>); break;
-          case 8: go(row_step<T, kTwo, 8>); break;
+          case 1: go(row_step<T, kSums, 1>); break;
+          case 2: go(row_step<T, kSums, 2>); break;
+          case 3: go(row_step<T, kSums, 3>); break;
+          case 4: go(row_step<T, kSums, 4>); break;
+          case 5: go(row_step<T, kSums, 5>); break;
+          case 6: go(row_step<T, kSums, 6>); break;
+          case 7: go(row_step<T, kSums, 7>); break;
+          case 8: go(row_step<T, kSums, 8>); break;
           default:
             if constexpr (sizeof(T) == 2) {
               if (words <= 12)
-                go(row_step<T, kTwo, 12>);
+                go(row_step<T, kSums, 12>);
               else
-                go(row_step<T, kTwo, 16>);
+                go(row_step<T, kSums, 16>);
             }
         }
         return;
@@ -888,9 +922,9 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
       const int splits = splits_of(a.rows, a.vocab), per = columns_per_split(a.rows, a.vocab, a.vocab);
       for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
         float* parts = static_cast<float*>(workspace) + r0 * splits * 4;
-        hipLaunchKernelGGL((row_part<T, kTwo>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
+        hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
                            per, parts);
-        hipLaunchKernelGGL((row_grad<T, kTwo>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kGradBlock),
+        hipLaunchKernelGGL((row_grad<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kGradBlock),
                            picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, (const float*)nullptr,
                            (const float*)parts, loss + r0, static_cast<T*>(dlogits) + r0 * out_width, out_width,
                            picks_log2_slots(t.topk));
