@@ -114,11 +114,22 @@ __device__ __forceinline__ Teacher teacher_of(const Task& a, int64_t row) {
   return r;
 }
 
+// Whether a row has any teacher entry, found by a wavefront (the same in all lanes): one round trip
+// where the first 64 have one, before anything else of the row is read.
+__device__ __forceinline__ bool any_entry(const Task& a, int64_t row) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  for (int j0 = 0; j0 < a.topk; j0 += kLanes) {
+    float t;
+    if (__any(j0 + lane < a.topk && a.entry(row, j0 + lane, &t) >= 0)) return true;
+  }
+  return false;
+}
+
 // Which sums a row needs.  kOne: a single factor serves whatever is wanted -- T == 1, or only one of the
 // two terms.  Else both exp((z - m)/T) and exp(z - m); for the temperatures 2 and 4 the second is a
 // power of the first, which saves an exponential (a quarter-rate instruction) per element and pass:
-// 8192 rows of 50257 in 16 bits, loss and gradient at once, take SQUARE_US with the square and
-// 460 us with two exponentials, which is then what bounds them.
+// of 8192 rows of 50257 in 16 bits the loss takes 144 us with the square and 153 with two exponentials,
+// the gradient 312 and 320, both at once 360 and 367.
 enum { kOne = 0, kBoth, kSquare, kFourth };
 
 // Running maximum and sums over the columns a lane has seen.  c0 is log2(e)/T, or log2(e) if only the
@@ -164,7 +175,7 @@ struct Exps {
 };
 
 // Joined over the workgroup, the same in every thread; `red` holds three floats per wavefront.
-template <int kWaves, int kSums>
+template <int kSums>
 __device__ __forceinline__ void block_merge(Exps<kSums>& a, float (*red)[3], float c0) {
   a.wave_merge(c0);
   if ((threadIdx.x & (kLanes - 1)) == 0) {
@@ -175,8 +186,8 @@ __device__ __forceinline__ void block_merge(Exps<kSums>& a, float (*red)[3], flo
   }
   __syncthreads();
   Exps<kSums> all;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) all.merge(red[w][0], red[w][1], red[w][2], c0);
+  const int waves = (int)blockDim.x / kLanes;
+  for (int w = 0; w < waves; ++w) all.merge(red[w][0], red[w][1], red[w][2], c0);
   a = all;
 }
 
@@ -196,18 +207,19 @@ __device__ __forceinline__ Stretch stretch_of(const T* at, int count) {
   return s;
 }
 
-// The sums over `count` columns at z, by kBlock threads.
-template <typename T, int kSums, int kBlock>
+// The sums over `count` columns at z, by the workgroup.
+template <typename T, int kSums>
 __device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int count, float c0) {
   constexpr int kInFlight = 4;
+  const int block = (int)blockDim.x;
   const Stretch s = stretch_of(z, count);
-  for (int w0 = threadIdx.x; w0 < s.words; w0 += kBlock * kInFlight) {
+  for (int w0 = threadIdx.x; w0 < s.words; w0 += block * kInFlight) {
     typename Wide<T>::Raw raw[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       // Without a condition, the last word again behind the last: the compiler puts a wait for all
       // earlier loads in front of every load in a branch.
-      const int w = w0 + u * kBlock < s.words ? w0 + u * kBlock : s.words - 1;
+      const int w = w0 + u * block < s.words ? w0 + u * block : s.words - 1;
       raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
     }
     float top = a.m;
@@ -220,7 +232,7 @@ __device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int coun
     const float b = Exps<kSums>::base(top);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      if (w0 + u * kBlock < s.words) {
+      if (w0 + u * block < s.words) {
 #pragma unroll
         for (int j = 0; j < kWide; ++j) a.term(Wide<T>::get(raw[u], j), b, c0);
       }
@@ -283,19 +295,18 @@ __device__ __forceinline__ void finish_row(const Task& a, int64_t row, const Tea
   }
 }
 
-constexpr int kLossBlock = 256;
+constexpr int kMaxBlock = 1024;
 
 template <typename T, int kSums>
-__global__ __launch_bounds__(kLossBlock) void row_loss(Task a, float c0, float* loss, float* stats) {
-  constexpr int kWaves = kLossBlock / kLanes;
-  __shared__ float red[kWaves][3];
+__global__ __launch_bounds__(kMaxBlock, 8) void row_loss(Task a, float c0, float* loss, float* stats) {
+  __shared__ float red[kMaxBlock / kLanes][3];
   const int64_t row = blockIdx.x;
   const Teacher t = teacher_of(a, row);
   const int label = a.label(row);
   Exps<kSums> s;
   if (t.any || label >= 0) {  // the same in all threads
-    add_columns<T, kSums, kLossBlock>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
-    block_merge<kWaves>(s, red, c0);
+    add_columns<T, kSums>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
+    block_merge(s, red, c0);
   }
   if (threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, stats);
 }
@@ -305,20 +316,14 @@ constexpr int kPartBlock = 256;
 // Columns [split * per_split, ...) of a row: partial sums to parts[row][split][4].
 template <typename T, int kSums>
 __global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per_split, float* parts) {
-  constexpr int kWaves = kPartBlock / kLanes;
-  __shared__ float red[kWaves][3];
+  __shared__ float red[kPartBlock / kLanes][3];
   const int64_t row = blockIdx.y;
   const int from = (int)blockIdx.x * per_split;
   const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
-  bool any = a.label(row) >= 0;  // a row without targets is not read
-  for (int j = threadIdx.x & (kLanes - 1); j < a.topk && !any; j += kLanes) {
-    float t;
-    any = a.entry(row, j, &t) >= 0;
-  }
   Exps<kSums> s;
-  if (__any(any)) {
-    add_columns<T, kSums, kPartBlock>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
-    block_merge<kWaves>(s, red, c0);
+  if (a.label(row) >= 0 || any_entry(a, row)) {  // a row without targets is not read
+    add_columns<T, kSums>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
+    block_merge(s, red, c0);
   }
   if (threadIdx.x == 0) {
     float* p = parts + (row * gridDim.x + blockIdx.x) * 4;
@@ -421,14 +426,17 @@ inline size_t picks_bytes(int topk) {
   return 4 * (1 + 2 * ((size_t)topk + 1) + ((size_t)1 << picks_log2_slots(topk)));
 }
 
-// Fills in the targets of a row that lie in [from, from + count); a barrier must follow.
-template <int kBlock>
+// In steps: empty the table; list the targets of a row that lie in [from, from + count); enter them into
+// the table, behind a barrier after the first step; put_picks, behind another after all.
+__device__ __forceinline__ void clear_picks(const Picks& p) {
+  for (int i = threadIdx.x; i < p.n_slots; i += (int)blockDim.x) p.slots[i] = -1;
+  if (threadIdx.x == 0) *p.twice = 0;
+}
+
 __device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Teacher& t, int label, float dloss, int from,
                                            int count, const Picks& p) {
-  for (int i = threadIdx.x; i < p.n_slots; i += kBlock) p.slots[i] = -1;
-  if (threadIdx.x == 0) *p.twice = 0;
   const float scale = dloss * a.soft * a.temperature;
-  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+  for (int j = threadIdx.x; j < p.n; j += (int)blockDim.x) {
     int at = -1;
     float minus = 0.f;
     if (j == a.topk) {
@@ -439,11 +447,15 @@ __device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Tea
       at = a.entry(row, j, &tj);
       minus = scale * (exp2_hw((tj - t.top) * a.c_soft) / t.sum);
     }
-    p.at[j] = at >= from && at < from + count ? at : -1;
+    at = at >= from && at < from + count ? at : -1;
+    p.at[j] = at;
     p.minus[j] = minus;
   }
-  __syncthreads();
-  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+}
+
+// Each thread enters what it has listed.
+__device__ __forceinline__ void enter_picks(const Picks& p) {
+  for (int j = threadIdx.x; j < p.n; j += (int)blockDim.x) {
     const int at = p.at[j];
     if (at < 0) continue;
     for (int h = at & (p.n_slots - 1);; h = (h + 1) & (p.n_slots - 1)) {  // half of the slots stay free
@@ -457,11 +469,10 @@ __device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Tea
   }
 }
 
-// Writes the corrected columns, behind a barrier that follows list_picks and the plain columns.
-template <typename T, int kSums, int kBlock>
+template <typename T, int kSums>
 __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T* z, T* out) {
   const bool twice = *p.twice != 0;
-  for (int j = threadIdx.x; j < p.n; j += kBlock) {
+  for (int j = threadIdx.x; j < p.n; j += (int)blockDim.x) {
     const int at = p.at[j];
     if (at < 0) continue;
     float minus = p.minus[j];
@@ -476,12 +487,12 @@ __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T
   }
 }
 
-template <typename T, int kBlock>
+template <typename T>
 __device__ __forceinline__ void put_zeros(T* out, int64_t count) {
   const float none[kWide] = {};
   const int64_t words = count / kWide;
-  for (int64_t w = threadIdx.x; w < words; w += kBlock) Wide<T>::store(out + w * kWide, none);
-  for (int64_t i = words * kWide + threadIdx.x; i < count; i += kBlock) Wide<T>::put(out + i, 0.f);
+  for (int64_t w = threadIdx.x; w < words; w += (int)blockDim.x) Wide<T>::store(out + w * kWide, none);
+  for (int64_t i = words * kWide + threadIdx.x; i < count; i += (int)blockDim.x) Wide<T>::put(out + i, 0.f);
 }
 
 constexpr int kGradBlock = 256;
@@ -490,44 +501,51 @@ constexpr int kGradBlock = 256;
 // the first split writes the loss; otherwise they come from `stats`.
 template <typename T, int kSums>
 __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per_split, const float* dloss, int dloss_step,
-                                                       const float* stats, const float* parts, float* loss, T* dlogits,
-                                                       int64_t out_width, int log2_slots) {
+                                                       const float* stats, const float* parts, int n_parts, float* loss,
+                                                       T* dlogits, int64_t out_width, int log2_slots) {
   constexpr int kInFlight = 4;
   extern __shared__ int lds[];
   const Picks picks(a.topk, log2_slots, lds);
   const int64_t row = blockIdx.y;
-  const int splits = (int)gridDim.x;
   const int from = (int)blockIdx.x * per_split;
   const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
-  const Teacher t = teacher_of(a, row);
   const int label = a.label(row);
   const float dl = dloss[row * dloss_step];
   T* out_row = dlogits + row * out_width;
   const T* z_row = (const T*)a.logits + row * a.row_stride;
-  if ((int)blockIdx.x == splits - 1) put_zeros<T, kGradBlock>(out_row + a.vocab, out_width - a.vocab);
-  Grad g;
-  if (parts) {
-    const Exps<kSums> s = join_parts<kSums>(parts, row, splits, c0);
-    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, s);
-    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, nullptr);
-  } else {
-    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
-  }
-  if (!t.any && label < 0) {
-    put_zeros<T, kGradBlock>(out_row + from, count);
-    return;
-  }
-  list_picks<kGradBlock>(a, row, t, label, dl, from, count, picks);
   const T* z = z_row + from;
   T* out = out_row + from;
+  if (blockIdx.x == gridDim.x - 1) put_zeros<T>(out_row + a.vocab, out_width - a.vocab);
+  if (!any_entry(a, row) && label < 0) {
+    put_zeros<T>(out, count);
+    if (parts && blockIdx.x == 0 && threadIdx.x == 0) loss[row] = 0.f;
+    return;
+  }
+  // The first words are requested before the targets are looked at.
   const Stretch s = stretch_of(out, count);
-  for (int w0 = threadIdx.x; w0 < s.words; w0 += kGradBlock * kInFlight) {
-    typename Wide<T>::Raw raw[kInFlight];
+  typename Wide<T>::Raw raw[kInFlight];
+  auto request = [&](int w0) {
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       const int w = w0 + u * kGradBlock < s.words ? w0 + u * kGradBlock : s.words - 1;
       raw[u] = Wide<T>::load(z + s.head + (int64_t)w * kWide);
     }
+  };
+  if (s.words > 0) request(threadIdx.x);
+  const Teacher t = teacher_of(a, row);
+  clear_picks(picks);
+  list_picks(a, row, t, label, dl, from, count, picks);
+  __syncthreads();
+  enter_picks(picks);
+  Grad g;
+  if (parts) {
+    const Exps<kSums> sums = join_parts<kSums>(parts, row, n_parts, c0);
+    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, sums);
+    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(sums), loss, nullptr);
+  } else {
+    g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
+  }
+  for (int w0 = threadIdx.x; w0 < s.words; w0 += kGradBlock * kInFlight) {
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       const int w = w0 + u * kGradBlock;
@@ -538,6 +556,7 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
         Wide<T>::store(out + s.head + (int64_t)w * kWide, v);
       }
     }
+    if (w0 + kGradBlock * kInFlight < s.words) request(w0 + kGradBlock * kInFlight);
   }
   const int i = (int)threadIdx.x;
   if (i < s.head + s.tail) {
@@ -545,21 +564,35 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
     Wide<T>::put(out + c, g.template at<kSums>(Wide<T>::one(z + c)));
   }
   __syncthreads();
-  put_picks<T, kSums, kGradBlock>(picks, g, z_row, out_row);
+  put_picks<T, kSums>(picks, g, z_row, out_row);
 }
 
-constexpr int kStepBlock = 1024;
-constexpr int kStepMaxWords16 = 16, kStepMaxWords32 = 8;  // words per thread that stay in registers
-constexpr int kOneByOne = 8, kStepWords = 4;  // there are kernels for 1 to 8 words, and for 12 and 16
+// Words of a thread for which there are kernels; the first of a kernel's words that may not exist.
+template <typename T>
+struct StepWords;
+template <>
+struct StepWords<float> {
+  static constexpr int kCount = 6, kList[kCount] = {1, 2, 4, 6, 9, 12}, kMostAtMaxBlock = 12;
+};
+template <>
+struct StepWords<_Float16> {
+  static constexpr int kCount = 8, kList[kCount] = {1, 2, 4, 8, 12, 16, 20, 25}, kMostAtMaxBlock = 20;
+};
+template <>
+struct StepWords<Bf16> : StepWords<_Float16> {};
 
-// Loss and gradient of a row that fits kWords words per thread.
-template <typename T, int kSums, int kWords>
-__global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 : 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
-                                                       T* dlogits, int64_t out_width, int log2_slots) {
-  constexpr int kWaves = kStepBlock / kLanes;
-  __shared__ float red[2][kWaves][3];
+// Loss and gradient of a row whose words stay in the registers of a workgroup, kWords a thread, so that
+// each logit is read once.  With many rows the workgroup is the smallest that holds a row: four of 256
+// threads share a CU, and while one waits for its row or for the others' sums the rest read, compute
+// and write (8192 rows of 50257 in 16 bits, T = 2 with labels: 360 us, with two of 1024 threads 410;
+// T = 1 without labels 348 and 331).
+template <typename T, int kSums, int kWords, int kSure>
+__global__ __launch_bounds__(kMaxBlock, 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
+                                                            T* dlogits, int64_t out_width, int log2_slots) {
+  __shared__ float red[2][kMaxBlock / kLanes][2];
   extern __shared__ int lds[];
   const Picks picks(a.topk, log2_slots, lds);
+  const int block = (int)blockDim.x, waves = block / kLanes;
   const int64_t row = blockIdx.x;
   const T* z = (const T*)a.logits + row * a.row_stride;
   T* out = dlogits + row * out_width;
@@ -567,28 +600,26 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   const int i = (int)threadIdx.x;
   const bool single = i < s.head + s.tail;
   const int single_at = i < s.head ? i : s.tail_at + i - s.head;
-  const Teacher t = teacher_of(a, row);
   const int label = a.label(row);
   const float dl = dloss[row * dloss_step];
-  put_zeros<T, kStepBlock>(out + a.vocab, out_width - a.vocab);
+  put_zeros<T>(out + a.vocab, out_width - a.vocab);
+  const Teacher t = teacher_of(a, row);
   if (!t.any && label < 0) {
-    put_zeros<T, kStepBlock>(out, a.vocab);
+    put_zeros<T>(out, a.vocab);
     if (i == 0) loss[row] = 0.f;
     return;
   }
   // Word u of a thread lies a fixed distance behind word 0, so one register of offset serves them all.
-  // The first kSure words exist in every thread (words_per_thread).
-  constexpr int kPitch = kStepBlock * kWide, kSure = kWords <= kOneByOne ? kWords - 1 : kWords - kStepWords;
-  auto exists = [&](int u) { return u < kSure || i + u * kStepBlock < s.words; };
+  auto exists = [&](int u) { return u < kSure || i + u * block < s.words; };
   const uint32_t off = (uint32_t)i * (kWide * sizeof(T));
   const T* z0 = z + s.head;
   T* out0 = out + s.head;
-  auto word_of = [&](const T* base, int u) { return (const T*)((const char*)(base + u * kPitch) + off); };
+  auto word_of = [&](const T* base, int u) { return (const T*)((const char*)(base + u * block * kWide) + off); };
   typename Wide<T>::Raw raw[kWords];
   if (s.words > 0) {
 #pragma unroll
     for (int u = 0; u < kWords; ++u) {
-      const int w = i + u * kStepBlock;
+      const int w = i + u * block;
       raw[u] = Wide<T>::load(u < kSure ? word_of(z0, u) : z0 + (int64_t)(w < s.words ? w : s.words - 1) * kWide);
     }
   } else {
@@ -596,7 +627,7 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
     for (int u = 0; u < kWords; ++u) raw[u] = Wide<T>::fill(-INFINITY);
   }
   const float x1 = single ? Wide<T>::one(z + single_at) : -INFINITY;
-  list_picks<kStepBlock>(a, row, t, label, dl, 0, a.vocab, picks);
+  clear_picks(picks);
   // The row's maximum first: the sums then need no rescaling.
   float top = x1;
 #pragma unroll
@@ -607,10 +638,9 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   top = wave_max(top);
   if ((i & (kLanes - 1)) == 0) red[0][i / kLanes][0] = top;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red[0][w][0]);
-  // The words are widened again for the sums and for the gradient: kept in 16 bits between the
-  // phases they leave room for two workgroups per CU.
+  for (int w = 0; w < waves; ++w) top = fmaxf(top, red[0][w][0]);
+  // The words are widened again for the sums and for the gradient: as fp32 numbers the row would not
+  // fit.
 #pragma unroll
   for (int u = 0; u < kWords; ++u) Wide<T>::keep_narrow(raw[u]);
   Exps<kSums> sums;
@@ -632,8 +662,7 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   }
   __syncthreads();
   sums.s0 = sums.s1 = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < waves; ++w) {
     sums.s0 += red[1][w][0];
     sums.s1 += red[1][w][1];
   }
@@ -651,36 +680,71 @@ __global__ __launch_bounds__(kStepBlock, kWords <= (sizeof(T) == 2 ? 8 : 2) ? 8 
   }
   if (single) Wide<T>::put(out + single_at, g.template at<kSums>(x1));
   if (i < kLanes) finish_row<T>(a, row, t, label, row_sums_of(sums), loss, nullptr);
+  list_picks(a, row, t, label, dl, 0, a.vocab, picks);  // now that the row's registers are free
+  enter_picks(picks);
   __syncthreads();
-  put_picks<T, kSums, kStepBlock>(picks, g, z, out);
+  put_picks<T, kSums>(picks, g, z, out);
 }
 
 // ---------------------------------------------------------------------------------------- host
-constexpr int kWantBlocks = 1024;     // four workgroups for each of 256 CUs
+constexpr int64_t kManyRows = 512;  // rows that keep the GPU busy with a workgroup of 256 threads each
+constexpr int64_t kFewRows = 64;    // rows that leave most CUs idle with one workgroup each
+constexpr int kWantBlocks = 1024;   // four workgroups for each of 256 CUs
 constexpr int kMinPerSplit = 4096;    // columns below which another workgroup does not pay
-constexpr int kGradColumns = 8192;    // columns of a row_grad workgroup where rows are plenty
+constexpr int kGradColumns = 8192;    // of a row_grad workgroup: four words a thread, requested at once
+constexpr int kPartColumns = 32768;   // of a row_part workgroup at most
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Columns per workgroup so that `rows` rows make kWantBlocks workgroups, a multiple of a word.
 int columns_per_split(int64_t rows, int64_t vocab, int64_t most) {
-  const int64_t splits = ceil_div(kWantBlocks, rows < 1 ? 1 : rows);
-  int64_t per = ceil_div(vocab, splits);
+  int64_t per = ceil_div(vocab, ceil_div(kWantBlocks, rows < 1 ? 1 : rows));
   if (per > most) per = ceil_div(vocab, ceil_div(vocab, most));
   if (per < kMinPerSplit) per = kMinPerSplit;
   return (int)((per + kWide - 1) / kWide * kWide);
 }
 
-// One workgroup per row, or several with their partial sums in the workspace.
-bool rows_are_split(int64_t rows, int64_t vocab) { return rows < kWantBlocks / 2 && vocab > kMinPerSplit; }
-int splits_of(int64_t rows, int64_t vocab) { return (int)ceil_div(vocab, columns_per_split(rows, vocab, vocab)); }
+// The forward call.  A few long rows are read by several workgroups each, whose partial sums a second
+// launch joins (16 bits, us split and whole: 8 rows of 65536 7.9 and 9.0, of 100000 8.2 and 10.7; 64 rows
+// of 65536 9.3 and 9.1, of 256000 13.8 and 20.3; 256 rows of 65536 13.9 and 11.2).
+bool loss_is_split(int64_t rows, int64_t vocab) { return rows <= kFewRows && vocab > 65536; }
 
-// Words of a thread in row_step.  All but the last exist in every thread, whether or not the row starts
-// with a single element: vocab / kWide is at least (result - 1) * kStepBlock + 1, and a row has that
-// many words or one less.
-int words_per_thread(int64_t vocab) { return (int)ceil_div(vocab / kWide, kStepBlock); }
-bool row_fits(int64_t vocab, int32_t dtype) {
-  return words_per_thread(vocab) <= (dtype == RAFHIP_F32 ? kStepMaxWords32 : kStepMaxWords16);
+// Otherwise a workgroup reads a row, a larger one where there are not many and they are long (16 bits, us
+// with 256 and 512 threads: 256 rows of 8192 5.6 and 6.5; 8 rows of 50257 9.2 and 8.3, 256 11.5 and 10.0).
+int loss_block(int64_t rows, int64_t vocab) { return rows < kManyRows && vocab > 16384 ? 512 : 256; }
+
+// Threads of row_step for a row, the fewest whose registers hold it, from 256 with many rows and from 512
+// with fewer, or 0: then row_part and row_grad read it twice, with workgroups for every CU.  So are a few
+// rows (16 bits, us twice and once: 8 rows of 8192 14.3 and 12.1, of 32000 12.6 and 14.4, of 160000 13
+// and 29; 64 rows of 32000 15.2 and 15.0, of 50257 16.2 and 17.6; 256 rows of 50257 26 and 22), and rows
+// for which a CU's registers spill (2048 rows of 160000 374 and 334, of 200000 437 and 465).
+template <typename T>
+int block_for_row(int64_t rows, int64_t vocab) {
+  using W = StepWords<T>;
+  const int64_t words = vocab / kWide;
+  if (rows <= kFewRows && vocab > 24576) return 0;
+  for (int block = rows < kManyRows ? 512 : 256; block < kMaxBlock; block *= 2)
+    if (words <= (int64_t)block * W::kList[W::kCount - 1]) return block;
+  return words <= (int64_t)kMaxBlock * W::kMostAtMaxBlock ? kMaxBlock : 0;
+}
+int step_block(int64_t rows, int64_t vocab, int32_t dtype) {
+  return dtype == RAFHIP_F32 ? block_for_row<float>(rows, vocab) : block_for_row<_Float16>(rows, vocab);
+}
+
+int64_t parts_bytes(int64_t rows, int64_t vocab) {
+  return rows * ceil_div(vocab, columns_per_split(rows, vocab, kPartColumns)) * 16;
+}
+
+// Calls f with the kernel for `words` words a thread: the next larger of the list.  All words that the
+// kernel before it has exist in every thread, whether or not the row starts with a single element:
+// a row has vocab / kWide words or one less, and vocab / kWide exceeds theirs by one at least.
+template <typename T, int kSums, int kAt = 0, typename F>
+void with_step_kernel(int words, F&& f) {
+  constexpr int kWords = StepWords<T>::kList[kAt], kSure = kAt > 0 ? StepWords<T>::kList[kAt > 0 ? kAt - 1 : 0] : 0;
+  if constexpr (kAt + 1 < StepWords<T>::kCount) {
+    if (words > kWords) return with_step_kernel<T, kSums, kAt + 1>(words, f);
+  }
+  f(row_step<T, kSums, kWords, kSure>);
 }
 
 int check_args(const char* who, const rafhip_topk_distill_args* p) {
@@ -794,9 +858,8 @@ extern "C" int64_t rafhip_topk_distill_workspace_bytes(const rafhip_topk_distill
   if (check_args("rafhip_topk_distill_workspace_bytes", args) != RAFHIP_OK) return -1;
   const rafhip_topk_distill_args& a = *args;
   if (a.rows == 0 || a.vocab == 0) return 0;
-  // The combined call splits long rows too, whatever their number.
-  if (!rows_are_split(a.rows, a.vocab) && row_fits(a.vocab, a.logits_dtype)) return 0;
-  return a.rows * splits_of(a.rows, a.vocab) * 16;
+  if (!loss_is_split(a.rows, a.vocab) && step_block(a.rows, a.vocab, a.logits_dtype) > 0) return 0;
+  return parts_bytes(a.rows, a.vocab);
 }
 
 extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* loss, float* stats, void* workspace,
@@ -810,8 +873,8 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
   if (int st = check_pointers(who, a)) return st;
   if (!loss) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss is NULL", who);
   if (!is_aligned(loss, 4) || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
-  const bool split = rows_are_split(a.rows, a.vocab);
-  const int64_t need = split ? rafhip_topk_distill_workspace_bytes(args) : 0;
+  const bool split = loss_is_split(a.rows, a.vocab);
+  const int64_t need = split ? parts_bytes(a.rows, a.vocab) : 0;
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
   int sums;
   float c0;
@@ -822,13 +885,14 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
       using T = decltype(e);
       constexpr int kSums = decltype(mode)::value;
       if (!split) {
-        hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)a.rows), dim3(kLossBlock), 0, s, t, c0, loss, stats);
+        hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)a.rows), dim3((unsigned)loss_block(a.rows, a.vocab)), 0, s,
+                           t, c0, loss, stats);
         return;
       }
       float* parts = static_cast<float*>(workspace);
-      const int splits = splits_of(a.rows, a.vocab);
+      const int per = columns_per_split(a.rows, a.vocab, kPartColumns), splits = (int)ceil_div(a.vocab, per);
       hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)a.rows), dim3(kPartBlock), 0, s, t, c0,
-                         columns_per_split(a.rows, a.vocab, a.vocab), parts);
+                         per, parts);
       hipLaunchKernelGGL((join_loss<T, kSums>), dim3((unsigned)a.rows), dim3(kLanes), 0, s, t, c0, parts, splits, loss, stats);
     });
   });
@@ -861,7 +925,7 @@ extern "C" int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, cons
         const int step = dloss_count == 1 ? 0 : 1;
         hipLaunchKernelGGL((row_grad<T, kSums>), dim3(splits, (unsigned)part.rows), dim3(kGradBlock),
                            picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, stats + r0 * 3,
-                           (const float*)nullptr, (float*)nullptr, static_cast<T*>(dlogits) + r0 * out_width, out_width,
+                           (const float*)nullptr, 0, (float*)nullptr, static_cast<T*>(dlogits) + r0 * out_width, out_width,
                            picks_log2_slots(t.topk));
       });
     });
@@ -882,7 +946,8 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
   if (a.rows == 0) return RAFHIP_OK;
   if (int st = check_pointers(who, a)) return st;
   if (!loss || !is_aligned(loss, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss %p", who, (const void*)loss);
-  const int64_t need = rafhip_topk_distill_workspace_bytes(args);
+  const int block = step_block(a.rows, a.vocab, a.logits_dtype);
+  const int64_t need = block > 0 ? 0 : parts_bytes(a.rows, a.vocab);
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
   int sums;
   float c0;
@@ -893,41 +958,23 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
     with_sums(sums, [&](auto mode) {
       using T = decltype(e);
       constexpr int kSums = decltype(mode)::value;
-      if (need == 0) {
-        auto go = [&](auto kernel) {
-          hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(kStepBlock), picks_bytes(t.topk), s, t, c0, dloss, step,
+      if (block > 0) {
+        with_step_kernel<T, kSums>((int)ceil_div(a.vocab / kWide, block), [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3((unsigned)block), picks_bytes(t.topk), s, t, c0, dloss, step,
                              loss, static_cast<T*>(dlogits), out_width, picks_log2_slots(t.topk));
-        };
-        const int words = words_per_thread(a.vocab);
-        switch (words) {
-          case 0:
-          case 1: go(row_step<T, kSums, 1>); break;
-          case 2: go(row_step<T, kSums, 2>); break;
-          case 3: go(row_step<T, kSums, 3>); break;
-          case 4: go(row_step<T, kSums, 4>); break;
-          case 5: go(row_step<T, kSums, 5>); break;
-          case 6: go(row_step<T, kSums, 6>); break;
-          case 7: go(row_step<T, kSums, 7>); break;
-          case 8: go(row_step<T, kSums, 8>); break;
-          default:
-            if constexpr (sizeof(T) == 2) {
-              if (words <= 12)
-                go(row_step<T, kSums, 12>);
-              else
-                go(row_step<T, kSums, 16>);
-            }
-        }
+        });
         return;
       }
-      const int splits = splits_of(a.rows, a.vocab), per = columns_per_split(a.rows, a.vocab, a.vocab);
+      const int per = columns_per_split(a.rows, a.vocab, kPartColumns), splits = (int)ceil_div(a.vocab, per);
+      const int per_grad = columns_per_split(a.rows, a.vocab, kGradColumns);
       for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
         float* parts = static_cast<float*>(workspace) + r0 * splits * 4;
         hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
                            per, parts);
-        hipLaunchKernelGGL((row_grad<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kGradBlock),
-                           picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, (const float*)nullptr,
-                           (const float*)parts, loss + r0, static_cast<T*>(dlogits) + r0 * out_width, out_width,
-                           picks_log2_slots(t.topk));
+        hipLaunchKernelGGL((row_grad<T, kSums>), dim3((unsigned)ceil_div(a.vocab, per_grad), (unsigned)part.rows),
+                           dim3(kGradBlock), picks_bytes(t.topk), s, part, c0, per_grad, dloss + r0 * step, step,
+                           (const float*)nullptr, (const float*)parts, splits, loss + r0,
+                           static_cast<T*>(dlogits) + r0 * out_width, out_width, picks_log2_slots(t.topk));
       });
     });
   });

@@ -49,6 +49,9 @@ def _want(z, idx, t, dloss, vocab, temperature, soft, labels, hard):
         finite = np.where(np.isfinite(zz), zz, np.nan)
         spread = (np.nanmax(finite, 1, initial=-1e30) - np.nanmin(finite, 1, initial=1e30)) * max(1.0, 1.0 / temperature) * 1.4427
         spread = np.clip(spread, 0, 160)  # what lies further down is below the smallest number
+    # An exponential below 2^-126 becomes 0 before its factor dloss soft T / S_T (or dloss hard / S_1; S >= 1)
+    # enters: its element of the gradient is off by 2^-126 times that factor, not by 2^-126.
+    r["factor"] = np.maximum(1.0, np.abs(dloss.double().numpy()) * (abs(soft) * temperature + abs(hard)))[:, None]
     r["E"] = 300 + 8 * (spread + np.log2(max(vocab, 2)))
     return r
 
@@ -78,7 +81,7 @@ def _check_grad(grad, r, vocab):
     assert np.array_equal(np.isnan(got), np.isnan(want))
     with np.errstate(all="ignore"):
         bound = U * r["E"][:, None] * (r["soft"] + r["p"] + r["hard"])
-        bound += 1.01 * HALF_STEP[out] * (np.abs(want) + bound) + TINY[out]
+        bound += 1.01 * HALF_STEP[out] * (np.abs(want) + bound) + TINY[out] + 2.0 ** -126 * r["factor"]
         worst = np.max(np.nan_to_num(np.abs(got - want) / bound, nan=0), initial=0)
     assert worst <= 1, f"gradient: {worst:.3f} of the bound"
 
@@ -123,6 +126,15 @@ def test_weights_and_temperatures(native_libs, temperature, soft, hard, labelled
     _all(z, idx, t, labels if labelled else None, dloss, temperature=temperature, soft=soft, hard=hard)
 
 
+@pytest.mark.parametrize("rows, vocab", [(21, 900), (600, 300), (3, 40_000), (70, 30_000)])
+@pytest.mark.parametrize("temperature", [2.0, 4.0, 2.5])
+def test_both_terms(native_libs, temperature, rows, vocab):
+    """Two sums of one pass; at 2 and 4 the second is a power of the first.  The rows' ranges differ widely."""
+    z, idx, t, labels, dloss = _case(rows, vocab, 5, F32)
+    z *= torch.logspace(-3, 2, rows)[:, None]
+    _all(z, idx, t, labels, dloss, temperature=temperature, hard=0.75)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,vocab", [
     (5, 1), (5, 2), (3, 7), (3, 8), (4, 9), (9, 63), (600, 65), (7, 4096), (7, 4097), (1, 8191), (2, 8193), (1, 50257),
@@ -138,6 +150,15 @@ def test_sizes(native_libs, rows, vocab, dtype):
 def test_teacher_lengths(native_libs, k, rows):
     z, idx, t, labels, dloss = _case(rows, 1500 if rows > 3 else 9000, k, F16)
     _all(z, idx, t, labels, dloss, temperature=1.5, hard=0.5)
+
+
+@pytest.mark.parametrize("rows, vocab, dtype", [(520, 100_000, F32), (520, 90_001, F32), (100, 90_001, F32),
+                                                (520, 165_003, BF16), (520, 163_847, F16), (520, 102_407, BF16), (65, 170_001, F16),
+                                                (64, 70_001, F32), (64, 25_000, BF16), (64, 24_576, F16)])
+def test_long_rows(native_libs, rows, vocab, dtype):
+    """Rows that 256, 512 and 1024 threads hold in registers, the longest of each, and ones that none hold."""
+    z, idx, t, labels, dloss = _case(rows, vocab, 4, dtype, masked=0.3)
+    _all(z, idx, t, labels, dloss, temperature=2.0, hard=0.5)
 
 
 def test_a_row_too_long_for_registers_among_many(native_libs):

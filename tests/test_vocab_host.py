@@ -94,7 +94,7 @@ def test_distill_argument_validation(native_libs):
     lib = L.optim()
     ws = lambda a: lib.rafhip_topk_distill_workspace_bytes(ctypes.byref(a))
     assert ws(_args(L)) > 0 and ws(_args(L, rows=4096)) == 0 and ws(_args(L, rows=0)) == 0
-    assert ws(_args(L, rows=4096, vocab=140_000, row_stride=140_000)) == 4096 * 16  # longer than the registers hold
+    assert ws(_args(L, rows=4096, vocab=170_000, row_stride=170_000)) == 4096 * 16 * 6  # longer than the registers hold
     assert lib.rafhip_topk_distill_workspace_bytes(None) == -1
 
     def all_three(a, loss=ONE, stats=ONE, dloss=ONE, count=4, out=ONE, width=50304, space=ONE, nbytes=1 << 20):
@@ -116,7 +116,7 @@ def test_distill_argument_validation(native_libs):
                    dict(vocab=1 << 28, row_stride=1 << 28), dict(row_stride=1 << 28)):
         assert all_three(_args(L, **change)) == (no, no, no), change
     assert all_three(_args(L, rows=0), count=0) == (0, 0, 0)
-    p = ctypes.byref(_args(L))
+    p = ctypes.byref(_args(L, vocab=70_000, row_stride=70_000))  # four rows, read in parts
     assert lib.rafhip_topk_distill(p, None, ONE, ONE, 1 << 20, None) == bad
     assert lib.rafhip_topk_distill(p, ONE, ONE, None, 0, None) == space
     assert lib.rafhip_topk_distill(p, ONE, ONE, ONE, 64, None) == space
@@ -124,8 +124,8 @@ def test_distill_argument_validation(native_libs):
     for kw in (dict(count=3), dict(count=0), dict(dloss=None), dict(out=None), dict(width=50256), dict(out=ONE + 1),
                dict(dloss=ONE + 2)):
         assert all_three(_args(L), loss=None, **kw)[1:] == (bad, bad), kw
-    assert lib.rafhip_topk_distill_dx(p, ONE, 4, None, ONE, 50304, None) == bad
-    assert lib.rafhip_topk_distill_step(p, ONE, 4, ONE, ONE, 50304, None, 0, None) == space
+    assert lib.rafhip_topk_distill_dx(p, ONE, 4, None, ONE, 70_016, None) == bad
+    assert lib.rafhip_topk_distill_step(p, ONE, 4, ONE, ONE, 70_016, None, 0, None) == space
     for fn in (lib.rafhip_topk_distill, lib.rafhip_topk_distill_dx, lib.rafhip_topk_distill_step):
         assert fn(None, *[None if t is ctypes.c_void_p else 0 for t in fn.argtypes[1:]]) == bad
 
