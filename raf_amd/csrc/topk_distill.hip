@@ -516,12 +516,12 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   const T* z = z_row + from;
   T* out = out_row + from;
   if (blockIdx.x == gridDim.x - 1) put_zeros<T>(out_row + a.vocab, out_width - a.vocab);
-  if (!any_entry(a, row) && label < 0) {
+  const Teacher t = teacher_of(a, row);
+  if (!t.any && label < 0) {
     put_zeros<T>(out, count);
     if (parts && blockIdx.x == 0 && threadIdx.x == 0) loss[row] = 0.f;
     return;
   }
-  // The first words are requested before the targets are looked at.
   const Stretch s = stretch_of(out, count);
   typename Wide<T>::Raw raw[kInFlight];
   auto request = [&](int w0) {
@@ -532,7 +532,6 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
     }
   };
   if (s.words > 0) request(threadIdx.x);
-  const Teacher t = teacher_of(a, row);
   clear_picks(picks);
   list_picks(a, row, t, label, dl, from, count, picks);
   __syncthreads();
