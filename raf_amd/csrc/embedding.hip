@@ -5,11 +5,12 @@
 //
 // Gradient: dx[r] = scale * sum over the tokens of row r of dy[t].  A sum by floating-point atomics
 // would depend on the order in which they arrive, so tokens are sorted by row first:
-//   1. tile_sort   sorts each tile of tokens by (row, position);
+//   1. tile_sort   sorts each tile of tokens by (row, position)
+//                  (meanwhile the gradient is zeroed, if most rows will have no tokens);
 //   2. find_rows   looks every row up in all sorted tiles at once (a binary search per lane and
-//                  tile), writes zeros for rows without tokens, and lists the others: the tokens of
+//                  tile), else writes zeros for rows without tokens, and lists the others: the tokens of
 //                  rows of up to kDirect, and chunks of kChunk tokens of longer rows;
-//   3. sum_rows    sums what is listed, a chunk per workgroup and the short rows by wavefronts, so
+//   3. sum_rows    sums what is listed, a wavefront for 64 words of a chunk or of eight short rows, so
 //                  that a token that fills half the batch is spread over the GPU;
 //   4. join_chunks adds the chunks of a row in order.
 // Runs of a row are visited in tile order and sorted inside a tile, so every sum runs over
@@ -101,6 +102,7 @@ constexpr int kMaxTiles = 512;
 constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens have a lane each
 constexpr int kSmallSort = 512, kSort = 1024;  // threads of a tile of 2^10 tokens, of more
 constexpr int kInFlight = 8;  // words in flight per lane
+constexpr int kChunkInFlight = 16;  // of a chunk: its four or two round trips are what a batch of 3003 waits for (33.3 and 31.3 us)
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr int kSlotShift = 28;  // an entry: a token (23 bits: kMaxTiles tiles of 2^14) and its row's slot
 
@@ -126,7 +128,7 @@ struct Run {
   uint32_t at, before;  // first key of the run; tokens of the row in earlier runs
 };
 // How much of each list is taken, in one word: a wavefront reserves all it needs with one atomic
-// (with four, 800 wavefronts queued for some 60 us).
+// (with four, 800 wavefronts queued for 60 us).
 typedef unsigned long long Taken;
 constexpr int kRunBits = 24, kSingleBits = 21;  // up to 2^23 runs, 2^23 / 9 rows of one chunk, 2^23 / 16 chunks
 __device__ __forceinline__ Taken take(uint32_t runs, uint32_t chunks) {
@@ -215,14 +217,28 @@ __device__ __forceinline__ void exchange_lanes(uint32_t (&v)[kEach], int tid, in
   }
 }
 
+// Zeros to `bytes` bytes, of which a multiple of 16 of a 2-byte aligned address, by `block` of `blocks` workgroups.
+__device__ __forceinline__ void fill_zeros(char* at, int64_t bytes, int64_t block, int64_t blocks) {
+  typedef uint32_t Sixteen __attribute__((ext_vector_type(4)));
+  int64_t head = (int64_t)(-(intptr_t)at & 15);
+  head = head < bytes ? head : bytes;
+  const int64_t pieces = (bytes - head) / 16, done = head + pieces * 16;
+  RAFHIP_GLOBAL Sixteen* out = (RAFHIP_GLOBAL Sixteen*)(at + head);
+  for (int64_t i = block * blockDim.x + threadIdx.x; i < pieces; i += blocks * blockDim.x) out[i] = Sixteen{};
+  const int64_t i = 2 * (int64_t)threadIdx.x;  // the ends, fewer than 16 bytes each
+  if (block == 0 && i < head) *(RAFHIP_GLOBAL uint16_t*)(at + i) = 0;
+  if (block == 0 && i < bytes - done) *(RAFHIP_GLOBAL uint16_t*)(at + done + i) = 0;
+}
+
 // Sorts one tile by a bitonic network over (row << tile_bits | position), kEach keys in the registers
 // of each thread: key i sits in register i % kEach of thread i / kEach, so of the 55 stages of 1024
 // keys 10 stay inside a thread, 39 inside a wavefront and 6 go through LDS.  Then the index: for every
-// bucket of rows the first key that is not below it.
+// bucket of rows the first key that is not below it.  Workgroups behind the tiles write fill_bytes of zeros.
 template <typename Id, int kThreads, int kEach>
 __global__ __launch_bounds__(kThreads) void tile_sort(const Id* ids, int64_t n, Which which, int tile_bits,
                                                       int bucket_bits, int buckets, uint32_t* keys, uint16_t* index,
-                                                      Taken* taken) {
+                                                      Taken* taken, int tiles, char* fill, int64_t fill_bytes) {
+  if ((int)blockIdx.x >= tiles) return fill_zeros(fill, fill_bytes, (int)blockIdx.x - tiles, (int)gridDim.x - tiles);
   constexpr int kSize = kEach * kThreads;
   __shared__ uint32_t lds[kSize];
   const int tid = threadIdx.x;
@@ -453,7 +469,7 @@ __device__ __forceinline__ T element(const T* base, uint32_t i) {
 template <typename TO, int kSlots, int kRounds>
 __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const uint16_t* index, int tiles, int tile_bits,
                                                     int bucket_bits, int buckets, int64_t rows, int64_t width,
-                                                    int accumulate, TO* dx, Taken* taken, uint32_t* entries,
+                                                    int write_zeros, TO* dx, Taken* taken, uint32_t* entries,
                                                     uint32_t* counts, Item* singles, Item* items, uint32_t* long_rows, Run* runs) {
   constexpr int kSpread = kLanes / kSlots;
   const int lane = threadIdx.x & (kLanes - 1);
@@ -551,7 +567,7 @@ __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const 
       if (row >= rows) break;
       const int count = __builtin_amdgcn_readlane(total, i * kSpread);
       if (count <= kDirect) {
-        if (count == 0 && !accumulate) zero_row(dx + row * width, width);
+        if (count == 0 && write_zeros) zero_row(dx + row * width, width);
         continue;
       }
       int n_runs = 0;
@@ -690,7 +706,7 @@ __device__ __forceinline__ void sum_chunk(const TD* dy, const uint32_t* keys, in
   const int64_t word = (int64_t)slice * kLanes + lane;
   if ((int64_t)slice * kLanes < words) {
     float acc[1][kWide] = {};
-    add_words<TD, 1, kInFlight>(dy, width, word, words, token, count, acc);
+    add_words<TD, 1, kChunkInFlight>(dy, width, word, words, token, count, acc);
     if (word < words) {
       if (part)
         Wide<float>::store(part + word * kWide, acc[0]);
@@ -780,7 +796,13 @@ __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale
 
 constexpr int kFewRowsPerWave = 8;
 // Eight workgroups per CU; a launch of more would only take longer to start.
-constexpr int64_t kMaxFindBlocks = 2048, kMaxSumBlocks = 2048;
+constexpr int64_t kMaxFindBlocks = 2048, kMaxSumBlocks = 2048, kMaxFillBlocks = 512;
+
+// Whether the whole gradient is zeroed while the tiles are sorted, which keep few CUs busy, rather than
+// the rows without tokens when they are known (us, first and later: 300 tokens over 25128 x 513 rows of
+// fp32 24 and 28, 3003 33 and 35, 16384 42.5 and 42.9; over 50257 x 1600 of 16 bits 300 44 and 48, 3003 50
+// and 52, 16384 66 and 65, 65536 130 and 118).
+bool fill_first(int64_t n, int64_t rows) { return n <= rows / 8; }
 
 template <typename TD, typename TO, typename Id>
 void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64_t width, float scale, int accumulate,
@@ -802,9 +824,14 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   auto* long_rows = reinterpret_cast<uint32_t*>(ws + l.long_at);
   auto* runs = reinterpret_cast<Run*>(ws + l.runs_at);
   auto* parts = reinterpret_cast<float*>(ws + l.parts_at);
+  const bool fill = !accumulate && fill_first(n, rows);
+  const int64_t fill_bytes = fill ? rows * width * (int64_t)sizeof(TO) : 0;
+  const int threads = l.tile_bits == kMinTileBits ? kSmallSort : kSort;
+  const int64_t fill_blocks = (fill_bytes + threads * 64 - 1) / (threads * 64);
+  const unsigned sort_blocks = (unsigned)(l.tiles + (fill_blocks < kMaxFillBlocks ? fill_blocks : kMaxFillBlocks));
   auto sort = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)l.tiles), dim3(l.tile_bits == kMinTileBits ? kSmallSort : kSort), 0, s, ids, n, which, l.tile_bits, l.bucket_bits,
-                       l.buckets, keys, index, taken);
+    hipLaunchKernelGGL(kernel, dim3(sort_blocks), dim3(threads), 0, s, ids, n, which, l.tile_bits, l.bucket_bits, l.buckets,
+                       keys, index, taken, l.tiles, reinterpret_cast<char*>(dx), fill_bytes);
   };
   switch (l.tile_bits) {
     case kMinTileBits: sort(tile_sort<Id, kSmallSort, 2>); break;
@@ -818,7 +845,7 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   const unsigned find_blocks = (unsigned)(max_blocks < kMaxFindBlocks ? max_blocks : kMaxFindBlocks);
   auto find = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(find_blocks), dim3(kBlock), 0, s, keys, index, l.tiles, l.tile_bits, l.bucket_bits,
-                       l.buckets, rows, width, accumulate, dx, taken, entries, counts, singles, items, long_rows, runs);
+                       l.buckets, rows, width, !accumulate && !fill, dx, taken, entries, counts, singles, items, long_rows, runs);
   };
   if (l.tiles <= 8)
     find(find_rows<TO, kGroup, 1>);

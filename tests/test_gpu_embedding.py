@@ -204,6 +204,26 @@ def test_gradient_leaves_out_what_takes_no_part(native_libs):
         assert torch.equal(op.embedding_dx(dy.to(DEV), all_dead, rows, padding_idx=120, first_row=first, grad=old.clone()), old)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 13, 520])
+def test_gradient_of_few_rows_of_many(native_libs, width, dtype):
+    """The gradient is zeroed as a whole first: from any element on, to the last, and nothing beside it."""
+    from raf_amd import kernels
+
+    n, rows = 300, 2411
+    ids = _ids(n, rows, "zipf")
+    dy = _randn(n, width, dtype=dtype)
+    want, size, count = vocab_f64.embedding_dx(dy.float().numpy(), ids.numpy(), rows)
+    for shift in range(0, 9, 2 if width > 8 else 1):
+        room = torch.full((rows * width + 16,), float("nan"), dtype=dtype, device=DEV)
+        out = room[shift:shift + rows * width].view(rows, width)
+        kernels.embedding_dx(dy.to(DEV), ids.to(DEV), out)
+        got = out.double().cpu().numpy()
+        bound = count[:, None] * U * size + 1.01 * HALF_STEP[dtype] * (np.abs(want) + count[:, None] * U * size) + TINY[dtype]
+        assert (np.abs(got - want) <= bound).all() and not got[count == 0].any()
+        assert room[:shift].isnan().all() and room[shift + rows * width:].isnan().all()
+
+
 def test_gradient_of_nothing(native_libs):
     from raf_amd import op
 
