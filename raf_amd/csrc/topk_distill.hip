@@ -47,13 +47,21 @@ struct Task {
   float temperature, soft, hard;
   float c_soft;  // log2(e) / T
 
+  // Both without a branch on the type, behind which the compiler would wait for every load: 64 bits or the
+  // low half twice, 32 bits or the low half twice.
   __device__ __forceinline__ int64_t index_at(const void* p, int64_t i) const {
-    return index_bits == 32 ? (int64_t)((const RAFHIP_GLOBAL int32_t*)p)[i] : ((const RAFHIP_GLOBAL int64_t*)p)[i];
+    const bool wide = index_bits != 32;
+    const RAFHIP_GLOBAL int32_t* at = (const RAFHIP_GLOBAL int32_t*)p + (wide ? 2 * i : i);
+    const int32_t low = at[0], high = at[wide ? 1 : 0];
+    return wide ? (int64_t)((uint64_t)(uint32_t)high << 32 | (uint32_t)low) : (int64_t)low;
   }
   __device__ __forceinline__ float teacher_at(int64_t i) const {
-    if (teacher_dtype == RAFHIP_F32) return ((const RAFHIP_GLOBAL float*)teacher)[i];
-    if (teacher_dtype == RAFHIP_F16) return (float)((const RAFHIP_GLOBAL _Float16*)teacher)[i];
-    return bf16_widen(((const RAFHIP_GLOBAL unsigned short*)teacher)[i]);
+    const bool wide = teacher_dtype == RAFHIP_F32;
+    const RAFHIP_GLOBAL unsigned short* at = (const RAFHIP_GLOBAL unsigned short*)teacher + (wide ? 2 * i : i);
+    const unsigned short low = at[0], high = at[wide ? 1 : 0];
+    const float half = (float)__builtin_bit_cast(_Float16, low);
+    const float other = __uint_as_float(wide ? (uint32_t)high << 16 | low : (uint32_t)low << 16);
+    return teacher_dtype == RAFHIP_F16 ? half : other;
   }
   // Column of teacher entry j of a row, -1 if it is absent; *t is its logit.
   __device__ __forceinline__ int entry(int64_t row, int j, float* t) const {
@@ -92,23 +100,34 @@ struct Teacher {
   bool any;
 };
 __device__ __forceinline__ Teacher teacher_of(const Task& a, int64_t row) {
+  constexpr int kHeld = 2;  // entries of a lane that are requested at once, and kept where there are no more
   const int lane = threadIdx.x & (kLanes - 1);
   Teacher r;
+  float held[kHeld];
   float top = -INFINITY;
   bool any = false;
-  for (int j = lane; j < a.topk; j += kLanes) {
-    float t;
-    if (a.entry(row, j, &t) >= 0) {
-      top = fmaxf(top, t);
-      any = true;
+  auto request = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int j = j0 + u * kLanes + lane;
+      const int at = a.entry(row, j < a.topk ? j : a.topk - 1, &held[u]);
+      if (j >= a.topk || at < 0) held[u] = -INFINITY;  // as an entry that is absent
+      any |= j < a.topk && at >= 0;
     }
+  };
+  for (int j0 = 0; j0 < a.topk; j0 += kHeld * kLanes) {
+    request(j0);
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) top = fmaxf(top, held[u]);
   }
   r.any = __any(any);
   r.top = wave_max(top);
   float sum = 0.f;
-  for (int j = lane; j < a.topk; j += kLanes) {
-    float t;
-    if (a.entry(row, j, &t) >= 0) sum += exp2_hw((t - r.top) * a.c_soft);
+  for (int j0 = 0; j0 < a.topk; j0 += kHeld * kLanes) {
+    if (a.topk > kHeld * kLanes) request(j0);
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (held[u] != -INFINITY) sum += exp2_hw((held[u] - r.top) * a.c_soft);
   }
   r.sum = wave_add(sum);
   return r;
@@ -497,8 +516,8 @@ __device__ __forceinline__ void put_zeros(T* out, int64_t count) {
 
 constexpr int kGradBlock = 256;
 
-// Columns [split * per_split, ...) of a row.  With `parts` the row's sums are joined from them and
-// the first split writes the loss; otherwise they come from `stats`.
+// Columns [split * per_split, ...) of a row.  With `parts` the row's sums are joined from them and one more
+// workgroup, without columns, writes the loss; otherwise they come from `stats`.
 template <typename T, int kSums>
 __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per_split, const float* dloss, int dloss_step,
                                                        const float* stats, const float* parts, int n_parts, float* loss,
@@ -508,7 +527,7 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   const Picks picks(a.topk, log2_slots, lds);
   const int64_t row = blockIdx.y;
   const int from = (int)blockIdx.x * per_split;
-  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
+  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;  // <= 0: the workgroup of the loss
   const int label = a.label(row);
   const float dl = dloss[row * dloss_step];
   T* out_row = dlogits + row * out_width;
@@ -517,11 +536,12 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   T* out = out_row + from;
   if (blockIdx.x == gridDim.x - 1) put_zeros<T>(out_row + a.vocab, out_width - a.vocab);
   const Teacher t = teacher_of(a, row);
-  if (!t.any && label < 0) {
-    put_zeros<T>(out, count);
-    if (parts && blockIdx.x == 0 && threadIdx.x == 0) loss[row] = 0.f;
+  if (count <= 0) {
+    if (threadIdx.x < kLanes)
+      finish_row<T>(a, row, t, label, row_sums_of(join_parts<kSums>(parts, row, n_parts, c0)), loss, nullptr);
     return;
   }
+  if (!t.any && label < 0) return put_zeros<T>(out, count);
   const Stretch s = stretch_of(out, count);
   typename Wide<T>::Raw raw[kInFlight];
   auto request = [&](int w0) {
@@ -540,7 +560,6 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   if (parts) {
     const Exps<kSums> sums = join_parts<kSums>(parts, row, n_parts, c0);
     g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, sums);
-    if (blockIdx.x == 0 && threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(sums), loss, nullptr);
   } else {
     g = grad_of<kSums>(a, c0, dl, t.any, label >= 0, stats[row * 3], stats[row * 3 + 1] * kLog2e, stats[row * 3 + 2] * kLog2e);
   }
@@ -970,7 +989,7 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
         float* parts = static_cast<float*>(workspace) + r0 * splits * 4;
         hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
                            per, parts);
-        hipLaunchKernelGGL((row_grad<T, kSums>), dim3((unsigned)ceil_div(a.vocab, per_grad), (unsigned)part.rows),
+        hipLaunchKernelGGL((row_grad<T, kSums>), dim3((unsigned)ceil_div(a.vocab, per_grad) + 1, (unsigned)part.rows),
                            dim3(kGradBlock), picks_bytes(t.topk), s, part, c0, per_grad, dloss + r0 * step, step,
                            (const float*)nullptr, (const float*)parts, splits, loss + r0,
                            static_cast<T*>(dlogits) + r0 * out_width, out_width, picks_log2_slots(t.topk));
