@@ -934,9 +934,13 @@ extern "C" int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, in
 
 extern "C" int64_t rafhip_embedding_dx_workspace_bytes(int64_t n, int64_t rows, int64_t width) {
   using namespace rafhip;
-  if (n < 0 || rows < 0 || width < 0 || width >= (1LL << 24)) return -1;
+  clear_error();
   Layout l;
-  if (!layout_of(n, rows, width, &l)) return -1;
+  if (n < 0 || rows < 0 || width < 0 || width >= (1LL << 24) || !layout_of(n, rows, width, &l)) {
+    fail(RAFHIP_ERR_UNSUPPORTED, "rafhip_embedding_dx: %lld tokens over %lld rows of width %lld", (long long)n, (long long)rows,
+         (long long)width);
+    return -1;
+  }
   return n <= kFewTokens || rows == 0 || width == 0 ? 0 : l.bytes;
 }
 
@@ -949,8 +953,7 @@ extern "C" int rafhip_embedding_dx(const void* dy, int32_t dy_dtype, const void*
   const char* who = "rafhip_embedding_dx";
   if (int st = check_common(who, dy_dtype, dx_dtype, rows, width, index_bits, n, first_row)) return st;
   const int64_t need = rafhip_embedding_dx_workspace_bytes(n, rows, width);
-  if (need < 0)
-    return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %lld tokens over %lld rows", who, (long long)n, (long long)rows);
+  if (need < 0) return RAFHIP_ERR_UNSUPPORTED;  // and the message says why
   if (rows == 0 || width == 0) return RAFHIP_OK;
   if (!dx || (n > 0 && (!dy || !indices))) return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
   if (!is_aligned(dy, element_bytes(dy_dtype)) || !is_aligned(dx, element_bytes(dx_dtype)) || !is_aligned(indices, index_bits / 8))

@@ -777,7 +777,7 @@ int check_args(const char* who, const rafhip_topk_distill_args* p) {
   if (a.vocab >= (1LL << 28) || a.row_stride >= (1LL << 28) || a.rows >= (1LL << 31) || a.topk > kMaxTop)
     return fail(RAFHIP_ERR_UNSUPPORTED, "%s: rows = %lld, vocab = %lld, row_stride = %lld, topk = %d", who, (long long)a.rows,
                 (long long)a.vocab, (long long)a.row_stride, a.topk);
-  if (!(a.temperature > 0.f) || !std::isfinite(a.temperature) || !std::isfinite(1.f / a.temperature))
+  if (!(a.temperature > 0.f) || !std::isfinite(a.temperature) || !std::isfinite(kLog2e / a.temperature))
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: temperature = %g", who, (double)a.temperature);
   if (!std::isfinite(a.soft_weight) || !std::isfinite(a.hard_weight))
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: soft_weight = %g, hard_weight = %g", who, (double)a.soft_weight, (double)a.hard_weight);

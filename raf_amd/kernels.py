@@ -159,6 +159,17 @@ def _vocab_tensor(t: torch.Tensor, name: str, dtypes, device=None) -> torch.Tens
     return t
 
 
+def _apart(out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """The kernels read their inputs while they write ``out``."""
+    def extent(t):
+        last = sum((n - 1) * stride for n, stride in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    for t in inputs:
+        if out.numel() and t.numel() and extent(out)[0] < extent(t)[1] and extent(t)[0] < extent(out)[1]:
+            raise ValueError("out: overlaps an input")
+
+
 def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
@@ -175,6 +186,8 @@ def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_
         out = torch.empty(*indices.shape, x.shape[1], dtype=x.dtype, device=x.device)
     elif tuple(_vocab_tensor(out, "out", _DTYPE_CODE, x.device).shape) != (*indices.shape, x.shape[1]):
         raise ValueError(f"out: shape {tuple(out.shape)}")
+    else:
+        _apart(out, x, indices)
     with torch.cuda.device(x.device):
         check(_lib.optim().rafhip_embedding(x.data_ptr(), _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], indices.data_ptr(),
                                             _INDEX_BITS[indices.dtype], indices.numel(), int(first_row), float(scale),
@@ -191,6 +204,7 @@ def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, out: torch.Tensor, sca
     _vocab_tensor(out, "out", _DTYPE_CODE, dy.device)
     if out.dim() != 2 or tuple(dy.shape) != (*indices.shape, out.shape[1]):
         raise ValueError(f"dy {tuple(dy.shape)}, indices {tuple(indices.shape)}, out {tuple(out.shape)}")
+    _apart(out, dy, indices)
     lib = _lib.optim()
     need = lib.rafhip_embedding_dx_workspace_bytes(indices.numel(), *out.shape)
     ws = _scratch(need, dy.device)
@@ -252,6 +266,7 @@ class TopkDistill:
         _vocab_tensor(out, "out", (self.logits.dtype,), self.logits.device)
         if out.dim() != 2 or out.shape[0] != self.rows or out.shape[1] < self.vocab:
             raise ValueError(f"out: shape {tuple(out.shape)}")
+        _apart(out, self.logits, *(t for t in self._keep if t is not None))
         return out
 
     def loss(self):

@@ -392,3 +392,7 @@ def test_refusals_on_the_device(native_libs):
         kernels.TopkDistill(z, idx, t, labels=labels[:3])
     with pytest.raises(ValueError, match="dloss"):
         kernels.TopkDistill(z, idx, t).step(dloss[:3])
+    room = torch.zeros(4, 128, device=DEV)
+    for out in (room, room.view(-1)[40:440].view(4, 100)):  # the logits' own memory, and part of it
+        with pytest.raises(ValueError, match="overlaps"):
+            kernels.TopkDistill(room[:, 50:100], idx, t).step(dloss, out=out)

@@ -47,7 +47,9 @@ def test_embedding_dx_workspace(native_libs):
     assert last < 8_388_608 * (4 * 64 / 16 + 24)
     assert ws(8_388_609, 50257, 64) == -1 and ws(8_388_608, 262_143, 64) > 0 and ws(8_388_608, 262_144, 64) == -1
     assert ws(1 << 20, (1 << 21) - 1, 1) > 0 and ws((1 << 20) + 1, (1 << 21) - 1, 1) == -1
-    assert ws(1, 1 << 21, 1) == -1 and ws(-1, 1, 1) == -1 and ws(1, -1, 1) == -1 and ws(1, 1, 1 << 24) == -1
+    assert ws(1, 1 << 21, 1) == -1 and b"1 tokens over 2097152 rows of width 1" in native_libs.optim().rafhip_last_error()
+    assert ws(1, 1, 1) == 0 and native_libs.optim().rafhip_last_error() == b""  # nor is an older message left
+    assert ws(-1, 1, 1) == -1 and ws(1, -1, 1) == -1 and ws(1, 1, 1 << 24) == -1
 
 
 def test_embedding_argument_validation(native_libs):
@@ -106,7 +108,7 @@ def test_distill_argument_validation(native_libs):
     bad, no, space = L.RAFHIP_ERR_INVALID_ARG, L.RAFHIP_ERR_UNSUPPORTED, L.RAFHIP_ERR_WORKSPACE
     for change in (dict(rows=-1), dict(vocab=-1), dict(topk=-1), dict(row_stride=50256), dict(temperature=0.0),
                    dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
-                   dict(temperature=1e-40), dict(soft_weight=float("nan")), dict(hard_weight=float("inf")),
+                   dict(temperature=1e-40), dict(temperature=3.5e-39), dict(soft_weight=float("nan")), dict(hard_weight=float("inf")),
                    dict(logits=None), dict(topk_indices=None), dict(topk_logits=None), dict(logits=ONE + 1),
                    dict(topk_indices=ONE + 4), dict(topk_logits=ONE + 2), dict(labels=ONE + 4)):
         assert all_three(_args(L, **change)) == (bad, bad, bad), change
