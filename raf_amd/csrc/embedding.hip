@@ -393,23 +393,77 @@ __device__ __forceinline__ void for_words(int64_t words, F&& f) {
   if (words > w) f(std::integral_constant<int, 1>{}, w);
 }
 
-// All of the gradient for up to kFewTokens tokens: every wavefront looks through the ids for its rows.
+// The tokens of a row among up to kFewTokens, as bits, summed into the row by a wavefront.
+template <typename TD, typename TO, int kRounds>
+__device__ __forceinline__ void sum_hits(const TD* dy, int64_t width, const uint64_t (&hits)[kRounds], float scale,
+                                         bool accumulate, TO* at) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  // The set bits in ascending order: lane e learns the position of the e-th.
+  int token[kRounds], count[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const uint64_t m = hits[k];
+    const bool set = m >> lane & 1;
+    const int place = __popcll(m & ((1ull << lane) - 1));
+    count[k] = __popcll(m);
+    // A lane that holds a token sends it to the lane of its rank, the others behind the last.
+    token[k] = __builtin_amdgcn_ds_permute((set ? place : count[k] + (lane - place)) * 4, k * kLanes + lane);
+  }
+  const int64_t words = width / kWide;
+  for_words(words, [&](auto sweeps, int64_t w) {
+    constexpr int kSweeps = decltype(sweeps)::value;
+    float acc[kSweeps][kWide] = {};
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps, kInFlight / kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
+#pragma unroll
+    for (int s = 0; s < kSweeps; ++s) {
+      const int64_t word = w + lane + s * kLanes;
+      if (word < words) put_row<TO, kWide>(at + word * kWide, acc[s], scale, accumulate);
+    }
+  });
+  const int64_t col = words * kWide + lane;
+  if (words * kWide < width) {
+    float acc[1] = {};
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) acc[0] += add_singles(dy, width, col, token[k], count[k]);
+    if (col < width) put_row<TO, 1>(at + col, acc, scale, accumulate);
+  }
+}
+
+// All of the gradient for up to kFewTokens tokens.  Written anew, a wavefront takes rows_per_wave rows and looks
+// through all the ids for them; added to (rows_per_wave 0), it takes a token and sums those of its
+// row if it is the first of them (37 tokens, 30522 x 768 rows: 8.8 us by rows, 4.4 by tokens).
 template <typename TD, typename TO, typename Id>
 __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids, int n, Which which, int64_t width,
-                                                     float scale, int accumulate, int rows_per_wave, TO* dx) {
+                                                     float scale, int rows_per_wave, TO* dx) {
   constexpr int kRounds = kFewTokens / kLanes;
   const int lane = threadIdx.x & (kLanes - 1);
   const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+  const bool accumulate = rows_per_wave == 0;
   const int64_t r0 = wave * rows_per_wave;
-  if (r0 >= which.rows) return;
+  if (accumulate ? wave >= n : r0 >= which.rows) return;
   const int mine = (int)(which.rows - r0 < rows_per_wave ? which.rows - r0 : rows_per_wave);
   int64_t row[kRounds];
   bool any = false;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     const int t = k * kLanes + lane;
-    row[k] = t < n ? which.row((int64_t)ids[t]) - r0 : -1;
+    const int64_t r = n > 0 ? which.row((int64_t)ids[t < n ? t : n - 1]) : -1;
+    row[k] = t < n && r >= 0 ? r - r0 : -1;
     any |= row[k] >= 0 && row[k] < mine;
+  }
+  if (accumulate) {
+    const int64_t r = which.row((int64_t)ids[wave]);
+    if (r < 0) return;
+    uint64_t hits[kRounds], earlier = 0;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      hits[k] = __ballot(row[k] == r);
+      const int64_t before = wave - k * kLanes;  // of these tokens, those in front of this wavefront's
+      earlier |= before <= 0 ? 0 : before >= kLanes ? hits[k] : hits[k] & ((1ull << before) - 1);
+    }
+    if (earlier == 0) sum_hits<TD, TO, kRounds>(dy, width, hits, scale, true, dx + r * width);
+    return;
   }
   const bool some = __any(any);
   for (int i = 0; i < mine; ++i) {
@@ -420,40 +474,10 @@ __global__ __launch_bounds__(kBlock) void few_tokens(const TD* dy, const Id* ids
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) all |= hits[k] = __ballot(row[k] == i);
     }
-    if (all == 0) {
-      if (!accumulate) zero_row(at, width);
-      continue;
-    }
-    // The set bits in ascending order: lane e learns the position of the e-th.
-    int token[kRounds], count[kRounds];
-#pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-      const uint64_t m = hits[k];
-      const bool set = m >> lane & 1;
-      const int place = __popcll(m & ((1ull << lane) - 1));
-      count[k] = __popcll(m);
-      // A lane that holds a token sends it to the lane of its rank, the others behind the last.
-      token[k] = __builtin_amdgcn_ds_permute((set ? place : count[k] + (lane - place)) * 4, k * kLanes + lane);
-    }
-    const int64_t words = width / kWide;
-    for_words(words, [&](auto sweeps, int64_t w) {
-      constexpr int kSweeps = decltype(sweeps)::value;
-      float acc[kSweeps][kWide] = {};
-#pragma unroll
-      for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps, kInFlight / kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
-#pragma unroll
-      for (int s = 0; s < kSweeps; ++s) {
-        const int64_t word = w + lane + s * kLanes;
-        if (word < words) put_row<TO, kWide>(at + word * kWide, acc[s], scale, accumulate != 0);
-      }
-    });
-    const int64_t col = words * kWide + lane;
-    if (words * kWide < width) {
-      float acc[1] = {};
-#pragma unroll
-      for (int k = 0; k < kRounds; ++k) acc[0] += add_singles(dy, width, col, token[k], count[k]);
-      if (col < width) put_row<TO, 1>(at + col, acc, scale, accumulate != 0);
-    }
+    if (all == 0)
+      zero_row(at, width);
+    else
+      sum_hits<TD, TO, kRounds>(dy, width, hits, scale, false, at);
   }
 }
 
@@ -809,9 +833,9 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
                TO* dx, char* ws, const Layout& l, hipStream_t s) {
   const int64_t rows = which.rows;
   if (n <= kFewTokens) {
-    const int64_t waves = (rows + kFewRowsPerWave - 1) / kFewRowsPerWave;
+    const int64_t waves = accumulate ? n : (rows + kFewRowsPerWave - 1) / kFewRowsPerWave;
     hipLaunchKernelGGL((few_tokens<TD, TO, Id>), dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, dy, ids,
-                       (int)n, which, width, scale, accumulate, kFewRowsPerWave, dx);
+                       (int)n, which, width, scale, accumulate ? 0 : kFewRowsPerWave, dx);
     return;
   }
   auto* taken = reinterpret_cast<Taken*>(ws + l.taken_at);
