@@ -416,9 +416,10 @@ __device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bo
   return grad_of<kSums>(a, c0, dloss, soft, hard, s.m, log2_soft, kSums != kOne ? __builtin_amdgcn_logf(s.s1) : log2_soft);
 }
 
-// The columns a row's targets correct.  Entries with the same column are taken together by the
-// first of them; whether there are any is found by a hash table, since comparing all pairs would
-// cost more than the row for hundreds of entries.
+// The columns a row's targets correct, the label last.  Teacher entries with the same column are taken
+// together by the first of them; whether there are any is found by a hash table, since comparing all
+// pairs would cost more than the row for hundreds of entries.  The label, which is among the teacher's
+// entries more often than not, is only looked up there.
 // In dynamic LDS: picks_bytes(topk) bytes.
 struct Picks {
   int n, n_slots;  // topk and the label; a power of two of at least twice that many
@@ -472,9 +473,9 @@ __device__ __forceinline__ void list_picks(const Task& a, int64_t row, const Tea
   }
 }
 
-// Each thread enters what it has listed.
+// Each thread enters the teacher's entries that it has listed.
 __device__ __forceinline__ void enter_picks(const Picks& p) {
-  for (int j = threadIdx.x; j < p.n; j += (int)blockDim.x) {
+  for (int j = threadIdx.x; j < p.n - 1; j += (int)blockDim.x) {
     const int at = p.at[j];
     if (at < 0) continue;
     for (int h = at & (p.n_slots - 1);; h = (h + 1) & (p.n_slots - 1)) {  // half of the slots stay free
@@ -491,6 +492,7 @@ __device__ __forceinline__ void enter_picks(const Picks& p) {
 template <typename T, int kSums>
 __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T* z, T* out) {
   const bool twice = *p.twice != 0;
+  const int label = p.at[p.n - 1];
   for (int j = threadIdx.x; j < p.n; j += (int)blockDim.x) {
     const int at = p.at[j];
     if (at < 0) continue;
@@ -501,6 +503,12 @@ __device__ __forceinline__ void put_picks(const Picks& p, const Grad& g, const T
       if (!first) continue;
       for (int i = j + 1; i < p.n; ++i)
         if (p.at[i] == at) minus += p.minus[i];
+    } else if (j < p.n - 1) {
+      if (at == label) minus += p.minus[p.n - 1];
+    } else {
+      int h = at & (p.n_slots - 1);
+      while (p.slots[h] != -1 && p.slots[h] != at) h = (h + 1) & (p.n_slots - 1);
+      if (p.slots[h] == at) continue;  // its part is that entry's
     }
     Wide<T>::put(out + at, g.template at<kSums>(Wide<T>::one(z + at)) - minus);
   }
