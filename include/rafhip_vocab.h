@@ -110,7 +110,7 @@ int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, const float* dl
 
 /* Both at once, for a training step that knows the upstream gradient beforehand (a weight per row
  * times the loss scale): each logit is read once from memory where a row fits the registers of a
- * workgroup (163,840 columns of 16 bits, 98,304 of fp32; 24,576 where there are 64 rows or
+ * workgroup (204,800 columns of 16 bits, 98,304 of fp32; 24,576 where there are 64 rows or
  * fewer: several workgroups then read a row twice sooner).  loss and dlogits as above. */
 int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, const float* dloss, int64_t dloss_count,
                              float* loss, void* dlogits, int64_t out_width, void* workspace,

@@ -147,8 +147,8 @@ __device__ __forceinline__ bool any_entry(const Task& a, int64_t row) {
 // Which sums a row needs.  kOne: a single factor serves whatever is wanted -- T == 1, or only one of the
 // two terms.  Else both exp((z - m)/T) and exp(z - m); for the temperatures 2 and 4 the second is a
 // power of the first, which saves an exponential (a quarter-rate instruction) per element and pass:
-// of 8192 rows of 50257 in 16 bits the loss takes 144 us with the square and 153 with two exponentials,
-// the gradient 312 and 320, both at once 360 and 367.
+// of 8192 rows of 50257 in 16 bits the loss takes 144 us with the square and 166 with two exponentials,
+// the gradient 308 and 320, both at once 354 and 383.
 enum { kOne = 0, kBoth, kSquare, kFourth };
 
 // Running maximum and sums over the columns a lane has seen.  c0 is log2(e)/T, or log2(e) if only the
@@ -598,11 +598,11 @@ template <typename T>
 struct StepWords;
 template <>
 struct StepWords<float> {
-  static constexpr int kCount = 6, kList[kCount] = {1, 2, 4, 6, 9, 12}, kMostAtMaxBlock = 12;
+  static constexpr int kCount = 6, kList[kCount] = {1, 2, 4, 6, 9, 12};
 };
 template <>
 struct StepWords<_Float16> {
-  static constexpr int kCount = 8, kList[kCount] = {1, 2, 4, 8, 12, 16, 20, 25}, kMostAtMaxBlock = 20;
+  static constexpr int kCount = 8, kList[kCount] = {1, 2, 4, 8, 12, 16, 20, 25};
 };
 template <>
 struct StepWords<Bf16> : StepWords<_Float16> {};
@@ -610,8 +610,8 @@ struct StepWords<Bf16> : StepWords<_Float16> {};
 // Loss and gradient of a row whose words stay in the registers of a workgroup, kWords a thread, so that
 // each logit is read once.  With many rows the workgroup is the smallest that holds a row: four of 256
 // threads share a CU, and while one waits for its row or for the others' sums the rest read, compute
-// and write (8192 rows of 50257 in 16 bits, T = 2 with labels: 360 us, with two of 1024 threads 410;
-// T = 1 without labels 348 and 331).
+// and write (8192 rows of 50257 in 16 bits, T = 2 with labels: 354 us, with one of 1024 threads 461;
+// T = 1 without labels 350 both).
 template <typename T, int kSums, int kWords, int kSure>
 __global__ __launch_bounds__(kMaxBlock, 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
                                                             T* dlogits, int64_t out_width, int log2_slots) {
@@ -741,17 +741,15 @@ int loss_block(int64_t rows, int64_t vocab) { return rows < kManyRows && vocab >
 
 // Threads of row_step for a row, the fewest whose registers hold it, from 256 with many rows and from 512
 // with fewer, or 0: then row_part and row_grad read it twice, with workgroups for every CU.  So are a few
-// rows (16 bits, us twice and once: 8 rows of 8192 14.3 and 12.1, of 32000 12.6 and 14.4, of 160000 13
-// and 29; 64 rows of 32000 15.2 and 15.0, of 50257 16.2 and 17.6; 256 rows of 50257 26 and 22), and rows
-// for which a CU's registers spill (2048 rows of 160000 374 and 334, of 200000 437 and 465).
+// long rows (16 bits, us twice and once: 8 rows of 8192 12.4 and 11.5, of 32000 12.3 and 14, of 160000 9.5
+// and 24; 64 rows of 16384 12.7 and 12.3, of 32000 13.4 and 14.2; but 256 rows of 50257 24 and 20, 2048
+// of 200000 460 and 409).
 template <typename T>
 int block_for_row(int64_t rows, int64_t vocab) {
-  using W = StepWords<T>;
-  const int64_t words = vocab / kWide;
   if (rows <= kFewRows && vocab > 24576) return 0;
-  for (int block = rows < kManyRows ? 512 : 256; block < kMaxBlock; block *= 2)
-    if (words <= (int64_t)block * W::kList[W::kCount - 1]) return block;
-  return words <= (int64_t)kMaxBlock * W::kMostAtMaxBlock ? kMaxBlock : 0;
+  for (int block = rows < kManyRows ? 512 : 256; block <= kMaxBlock; block *= 2)
+    if (vocab / kWide <= (int64_t)block * StepWords<T>::kList[StepWords<T>::kCount - 1]) return block;
+  return 0;
 }
 int step_block(int64_t rows, int64_t vocab, int32_t dtype) {
   return dtype == RAFHIP_F32 ? block_for_row<float>(rows, vocab) : block_for_row<_Float16>(rows, vocab);

@@ -153,7 +153,7 @@ def test_teacher_lengths(native_libs, k, rows):
 
 
 @pytest.mark.parametrize("rows, vocab, dtype", [(520, 100_000, F32), (520, 90_001, F32), (100, 90_001, F32),
-                                                (520, 165_003, BF16), (520, 163_847, F16), (520, 102_407, BF16), (65, 170_001, F16),
+                                                (520, 204_808, BF16), (520, 204_807, F16), (520, 102_407, BF16), (65, 205_001, F16),
                                                 (64, 70_001, F32), (64, 25_000, BF16), (64, 24_576, F16)])
 def test_long_rows(native_libs, rows, vocab, dtype):
     """Rows that 256, 512 and 1024 threads hold in registers, the longest of each, and ones that none hold."""

@@ -96,7 +96,7 @@ def test_distill_argument_validation(native_libs):
     lib = L.optim()
     ws = lambda a: lib.rafhip_topk_distill_workspace_bytes(ctypes.byref(a))
     assert ws(_args(L)) > 0 and ws(_args(L, rows=4096)) == 0 and ws(_args(L, rows=0)) == 0
-    assert ws(_args(L, rows=4096, vocab=170_000, row_stride=170_000)) == 4096 * 16 * 6  # longer than the registers hold
+    assert ws(_args(L, rows=4096, vocab=210_000, row_stride=210_000)) == 4096 * 16 * 7  # longer than the registers hold
     assert lib.rafhip_topk_distill_workspace_bytes(None) == -1
 
     def all_three(a, loss=ONE, stats=ONE, dloss=ONE, count=4, out=ONE, width=50304, space=ONE, nbytes=1 << 20):
