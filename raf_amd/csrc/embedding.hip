@@ -102,7 +102,8 @@ constexpr int kMaxTiles = 512;
 constexpr int kGroup = kLanes / kDirect;  // rows of a wavefront: their tokens have a lane each
 constexpr int kSmallSort = 512, kSort = 1024;  // threads of a tile of 2^10 tokens, of more
 constexpr int kInFlight = 8;  // words in flight per lane
-constexpr int kChunkInFlight = 16;  // of a chunk: its four or two round trips are what a batch of 3003 waits for (33.3 and 31.3 us)
+// Of a chunk: a short batch waits for its round trips (3003 tokens 31.3 us with two of 16, 33.3 with four of 8).
+constexpr int kChunkInFlight = 16;
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr int kSlotShift = 28;  // an entry: a token (23 bits: kMaxTiles tiles of 2^14) and its row's slot
 
@@ -115,7 +116,8 @@ struct Layout {
   int64_t max_runs = 0;   // runs of them
   int64_t max_long = 0;   // rows of more than one chunk
   int64_t max_parts = 0;  // their chunks
-  int64_t keys_at = 0, index_at = 0, taken_at = 0, entries_at = 0, counts_at = 0, singles_at = 0, items_at = 0, long_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
+  int64_t keys_at = 0, index_at = 0, taken_at = 0, entries_at = 0, counts_at = 0, singles_at = 0, items_at = 0;
+  int64_t long_at = 0, runs_at = 0, parts_at = 0, bytes = 0;
 };
 
 // One chunk of a row of more than kDirect tokens, with all that its sum needs to know.  There are two
@@ -414,7 +416,8 @@ __device__ __forceinline__ void sum_hits(const TD* dy, int64_t width, const uint
     constexpr int kSweeps = decltype(sweeps)::value;
     float acc[kSweeps][kWide] = {};
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k) add_words<TD, kSweeps, kInFlight / kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
+    for (int k = 0; k < kRounds; ++k)
+      add_words<TD, kSweeps, kInFlight / kSweeps>(dy, width, w + lane, words, token[k], count[k], acc);
 #pragma unroll
     for (int s = 0; s < kSweeps; ++s) {
       const int64_t word = w + lane + s * kLanes;
@@ -494,7 +497,8 @@ template <typename TO, int kSlots, int kRounds>
 __global__ __launch_bounds__(kBlock) void find_rows(const uint32_t* keys, const uint16_t* index, int tiles, int tile_bits,
                                                     int bucket_bits, int buckets, int64_t rows, int64_t width,
                                                     int write_zeros, TO* dx, Taken* taken, uint32_t* entries,
-                                                    uint32_t* counts, Item* singles, Item* items, uint32_t* long_rows, Run* runs) {
+                                                    uint32_t* counts, Item* singles, Item* items, uint32_t* long_rows,
+                                                    Run* runs) {
   constexpr int kSpread = kLanes / kSlots;
   const int lane = threadIdx.x & (kLanes - 1);
   const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
@@ -663,7 +667,8 @@ __device__ __forceinline__ void sum_short_rows(const TD* dy, int64_t width, cons
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
       const int e = e0 + u < entries ? e0 + u : entries - 1;
-      raw[u] = Wide<TD>::load(dy + (int64_t)__builtin_amdgcn_readlane(token, e) * width + (word < words ? word : words - 1) * kWide);
+      const TD* row = dy + (int64_t)__builtin_amdgcn_readlane(token, e) * width;
+      raw[u] = Wide<TD>::load(row + (word < words ? word : words - 1) * kWide);
     }
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
@@ -890,8 +895,8 @@ void launch_dx(const TD* dy, const Id* ids, int64_t n, const Which& which, int64
   hipLaunchKernelGGL((sum_rows<TD, TO>), dim3(chunk_blocks + short_blocks), dim3(kBlock), 0, s, dy, keys, l.tile_bits,
                      width, scale, accumulate, dx, taken, entries, counts, stride, rows, singles, items, runs,
                      parts, chunk_blocks, slices);
-  hipLaunchKernelGGL(join_chunks<TO>, dim3((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_long < 128 ? l.max_long : 128)),
-                     dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, long_rows, parts);
+  const dim3 join_blocks((unsigned)((width + kLanes - 1) / kLanes), (unsigned)(l.max_long < 128 ? l.max_long : 128));
+  hipLaunchKernelGGL(join_chunks<TO>, join_blocks, dim3(kBlock), 0, s, width, scale, accumulate, dx, taken, items, long_rows, parts);
 }
 
 int check_common(const char* who, int32_t a_dtype, int32_t b_dtype, int64_t rows, int64_t width, int32_t index_bits, int64_t n,
@@ -900,12 +905,14 @@ int check_common(const char* who, int32_t a_dtype, int32_t b_dtype, int64_t rows
     return fail(RAFHIP_ERR_UNSUPPORTED, "%s: dtypes %d and %d", who, a_dtype, b_dtype);
   if (index_bits != 32 && index_bits != 64) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %d-bit indices", who, index_bits);
   if (n < 0 || rows < 0 || width < 0)
-    return fail(RAFHIP_ERR_INVALID_ARG, "%s: n = %lld, rows = %lld, width = %lld", who, (long long)n, (long long)rows, (long long)width);
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: n = %lld, rows = %lld, width = %lld", who, (long long)n, (long long)rows,
+                (long long)width);
   if (first_row < 0 || first_row > INT64_MAX - rows)
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: first_row = %lld", who, (long long)first_row);
   // Byte offsets stay far inside 63 bits, and the column arithmetic of a workgroup inside 31.
   if (width >= (1LL << 24) || rows >= (1LL << 36) || n >= (1LL << 36))
-    return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %lld rows, %lld tokens of width %lld", who, (long long)rows, (long long)n, (long long)width);
+    return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %lld rows, %lld tokens of width %lld", who, (long long)rows, (long long)n,
+                (long long)width);
   return RAFHIP_OK;
 }
 
@@ -985,7 +992,8 @@ extern "C" int rafhip_embedding_dx(const void* dy, int32_t dy_dtype, const void*
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p of %lld bytes, need %lld", who, workspace, (long long)workspace_bytes,
                 (long long)need);
-  if (need > 0 && !is_aligned(workspace, 16)) return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
+  if (need > 0 && !is_aligned(workspace, 16))
+    return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
   if (n == 0 && accumulate) return RAFHIP_OK;
   Layout l;
   layout_of(n, rows, width, &l);

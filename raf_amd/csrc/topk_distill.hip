@@ -786,7 +786,8 @@ int check_args(const char* who, const rafhip_topk_distill_args* p) {
   if (!(a.temperature > 0.f) || !std::isfinite(a.temperature) || !std::isfinite(kLog2e / a.temperature))
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: temperature = %g", who, (double)a.temperature);
   if (!std::isfinite(a.soft_weight) || !std::isfinite(a.hard_weight))
-    return fail(RAFHIP_ERR_INVALID_ARG, "%s: soft_weight = %g, hard_weight = %g", who, (double)a.soft_weight, (double)a.hard_weight);
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: soft_weight = %g, hard_weight = %g", who, (double)a.soft_weight,
+                (double)a.hard_weight);
   return RAFHIP_OK;
 }
 
@@ -801,15 +802,18 @@ int check_pointers(const char* who, const rafhip_topk_distill_args& a) {
 
 int check_workspace(const char* who, int64_t need, const void* workspace, int64_t bytes) {
   if (need > 0 && (!workspace || bytes < need))
-    return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p of %lld bytes, need %lld", who, workspace, (long long)bytes, (long long)need);
-  if (need > 0 && !is_aligned(workspace, 16)) return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
+    return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p of %lld bytes, need %lld", who, workspace, (long long)bytes,
+                (long long)need);
+  if (need > 0 && !is_aligned(workspace, 16))
+    return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
   return RAFHIP_OK;
 }
 
 int check_gradient(const char* who, const rafhip_topk_distill_args& a, const float* dloss, int64_t dloss_count,
                    const void* dlogits, int64_t out_width) {
   if (dloss_count != a.rows && dloss_count != 1)
-    return fail(RAFHIP_ERR_INVALID_ARG, "%s: dloss has %lld values for %lld rows", who, (long long)dloss_count, (long long)a.rows);
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: dloss has %lld values for %lld rows", who, (long long)dloss_count,
+                (long long)a.rows);
   if (out_width < a.vocab) return fail(RAFHIP_ERR_INVALID_ARG, "%s: out_width = %lld < vocab", who, (long long)out_width);
   if (out_width >= (1LL << 28)) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: out_width = %lld", who, (long long)out_width);
   if (a.rows > 0 && (!dloss || (out_width > 0 && !dlogits))) return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
@@ -896,7 +900,8 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
   if (a.rows == 0) return RAFHIP_OK;
   if (int st = check_pointers(who, a)) return st;
   if (!loss) return fail(RAFHIP_ERR_INVALID_ARG, "%s: loss is NULL", who);
-  if (!is_aligned(loss, 4) || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  if (!is_aligned(loss, 4) || !is_aligned(stats, 4))
+    return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
   const bool split = loss_is_split(a.rows, a.vocab);
   const int64_t need = split ? parts_bytes(a.rows, a.vocab) : 0;
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
