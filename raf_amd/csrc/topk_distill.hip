@@ -535,7 +535,7 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   const Picks picks(a.topk, log2_slots, lds);
   const int64_t row = blockIdx.y;
   const int from = (int)blockIdx.x * per_split;
-  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;  // <= 0: the workgroup of the loss
+  const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
   const int label = a.label(row);
   const float dl = dloss[row * dloss_step];
   T* out_row = dlogits + row * out_width;
@@ -543,8 +543,9 @@ __global__ __launch_bounds__(kGradBlock) void row_grad(Task a, float c0, int per
   const T* z = z_row + from;
   T* out = out_row + from;
   if (blockIdx.x == gridDim.x - 1) put_zeros<T>(out_row + a.vocab, out_width - a.vocab);
+  if (count <= 0 && !parts) return;  // a vocabulary without columns: its padding is all there is
   const Teacher t = teacher_of(a, row);
-  if (count <= 0) {
+  if (count <= 0) {  // the workgroup of the loss
     if (threadIdx.x < kLanes)
       finish_row<T>(a, row, t, label, row_sums_of(join_parts<kSums>(parts, row, n_parts, c0)), loss, nullptr);
     return;

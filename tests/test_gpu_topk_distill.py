@@ -293,6 +293,28 @@ def test_leading_dimensions_and_empty_shapes(native_libs):
     assert not padded[0].any() and not padded[1].any()
 
 
+def test_a_vocabulary_without_columns(native_libs):
+    """Every column is padding: no loss, and a gradient of zeros as wide as it is asked for."""
+    from raf_amd import kernels, op
+
+    for rows in (24, 600):
+        z, idx, t, labels, dloss = (x.to(DEV) for x in _case(rows, 90, 4, F16))
+        more = dict(labels=labels, hard_weight=0.5, vocab_size=0)
+        loss, stats = op.topk_distill(z, idx, t, **more)
+        assert not loss.any() and not stats.any()
+        assert not op.topk_distill_dx(dloss, z, idx, t, stats, **more).any()
+        loss, grad = op.topk_distill_step(z, idx, t, dloss, **more)
+        assert not loss.any() and not grad.any()
+        h = kernels.TopkDistill(z[:, :0], idx, t, 2.0, 1.0, labels, 0.5)
+        loss, stats = h.loss()
+        assert not loss.any() and not stats.any()
+        for width in (0, 1, 9, 515):
+            wide = torch.full((rows, width), 9.0, dtype=F16, device=DEV)
+            assert not h.dx(dloss, stats, out=wide).any()
+            loss, grad = h.step(dloss, out=wide.fill_(9.0))
+            assert not loss.any() and not grad.any()
+
+
 def test_rows_of_a_wider_matrix(native_libs):
     """The direct handle takes rows that lie apart, and an output of another width than the input."""
     from raf_amd import kernels
