@@ -21,6 +21,7 @@
 
 #include <cstdint>
 
+#include "device_table.h"
 #include "rafhip_vocab.h"
 #include "status.h"
 #include "vocab_io.h"
@@ -945,17 +946,19 @@ extern "C" int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, in
   const int64_t per_block = all >= 256 * 8 * 4 * (int64_t)kBlock ? 4 * kBlock : kBlock;
   int64_t tokens = per_block / (words > 0 ? words : 1);
   tokens = tokens < 1 ? 1 : tokens;
-  const int64_t blocks = (n + tokens - 1) / tokens;
-  if (blocks > INT32_MAX) return fail(RAFHIP_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)n);
+  const int64_t most = kMaxGridBlocks * tokens;  // of a launch
   with_element(x_dtype, [&](auto tx) {
     with_element(y_dtype, [&](auto ty) {
       with_index(index_bits, [&](auto id) {
         using TX = decltype(tx);
         using TY = decltype(ty);
         using Id = decltype(id);
-        hipLaunchKernelGGL((embedding_kernel<TX, TY, Id>), dim3((unsigned)blocks), dim3(kBlock), 0, s,
-                           static_cast<const TX*>(x), static_cast<const Id*>(indices), n, rows, first_row, width, words,
-                           (int)tokens, scale, static_cast<TY*>(y));
+        for (int64_t t0 = 0; t0 < n; t0 += most) {
+          const int64_t count = n - t0 < most ? n - t0 : most;
+          hipLaunchKernelGGL((embedding_kernel<TX, TY, Id>), dim3((unsigned)((count + tokens - 1) / tokens)), dim3(kBlock), 0, s,
+                             static_cast<const TX*>(x), static_cast<const Id*>(indices) + t0, count, rows, first_row, width,
+                             words, (int)tokens, scale, static_cast<TY*>(y) + t0 * width);
+        }
       });
     });
   });

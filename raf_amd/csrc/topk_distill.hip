@@ -22,6 +22,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "device_table.h"
 #include "rafhip_vocab.h"
 #include "status.h"
 #include "vocab_io.h"
@@ -862,13 +863,15 @@ void with_sums(int mode, F&& f) {
 }
 
 constexpr int64_t kMaxGridY = 65535;
+// Workgroups of `block` threads in a launch's first dimension.
+int64_t max_grid_x(int block) { return kMaxGridBlocks * 256 / block; }
 
-// Rows beyond what a launch's second dimension holds go into further launches.
+// Rows beyond the `most` that a launch's dimension holds go into further launches.
 template <typename F>
-void for_row_blocks(const Task& t, size_t element, F&& f) {
-  for (int64_t r0 = 0; r0 < t.rows; r0 += kMaxGridY) {
+void for_row_blocks(const Task& t, size_t element, int64_t most, F&& f) {
+  for (int64_t r0 = 0; r0 < t.rows; r0 += most) {
     Task part = t;
-    part.rows = t.rows - r0 < kMaxGridY ? t.rows - r0 : kMaxGridY;
+    part.rows = t.rows - r0 < most ? t.rows - r0 : most;
     part.logits = static_cast<const char*>(t.logits) + (size_t)r0 * (size_t)t.row_stride * element;
     const size_t index = (size_t)t.index_bits / 8, teacher = t.teacher_dtype == RAFHIP_F32 ? 4 : 2;
     part.indices = static_cast<const char*>(t.indices) + (size_t)r0 * (size_t)t.topk * index;
@@ -915,8 +918,11 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
       using T = decltype(e);
       constexpr int kSums = decltype(mode)::value;
       if (!split) {
-        hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)a.rows), dim3((unsigned)loss_block(a.rows, a.vocab)), 0, s,
-                           t, c0, loss, stats);
+        const int block = loss_block(a.rows, a.vocab);
+        for_row_blocks(t, sizeof(T), max_grid_x(block), [&](const Task& part, int64_t r0) {
+          hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)part.rows), dim3((unsigned)block), 0, s, part, c0, loss + r0,
+                             stats ? stats + r0 * 3 : nullptr);
+        });
         return;
       }
       float* parts = static_cast<float*>(workspace);
@@ -951,7 +957,7 @@ extern "C" int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, cons
     with_sums(sums, [&](auto mode) {
       using T = decltype(e);
       constexpr int kSums = decltype(mode)::value;
-      for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
+      for_row_blocks(t, sizeof(T), kMaxGridY, [&](const Task& part, int64_t r0) {
         const int step = dloss_count == 1 ? 0 : 1;
         hipLaunchKernelGGL((row_grad<T, kSums>), dim3(splits, (unsigned)part.rows), dim3(kGradBlock),
                            picks_bytes(t.topk), s, part, c0, per, dloss + r0 * step, step, stats + r0 * 3,
@@ -990,14 +996,17 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
       constexpr int kSums = decltype(mode)::value;
       if (block > 0) {
         with_step_kernel<T, kSums>((int)ceil_div(a.vocab / kWide, block), [&](auto kernel) {
-          hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3((unsigned)block), picks_bytes(t.topk), s, t, c0, dloss, step,
-                             loss, static_cast<T*>(dlogits), out_width, picks_log2_slots(t.topk));
+          for_row_blocks(t, sizeof(T), max_grid_x(block), [&](const Task& part, int64_t r0) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)part.rows), dim3((unsigned)block), picks_bytes(t.topk), s, part, c0,
+                               dloss + r0 * step, step, loss + r0, static_cast<T*>(dlogits) + r0 * out_width, out_width,
+                               picks_log2_slots(t.topk));
+          });
         });
         return;
       }
       const int per = columns_per_split(a.rows, a.vocab, kPartColumns), splits = (int)ceil_div(a.vocab, per);
       const int per_grad = columns_per_split(a.rows, a.vocab, kGradColumns);
-      for_row_blocks(t, sizeof(T), [&](const Task& part, int64_t r0) {
+      for_row_blocks(t, sizeof(T), kMaxGridY, [&](const Task& part, int64_t r0) {
         float* parts = static_cast<float*>(workspace) + r0 * splits * 4;
         hipLaunchKernelGGL((row_part<T, kSums>), dim3((unsigned)splits, (unsigned)part.rows), dim3(kPartBlock), 0, s, part, c0,
                            per, parts);

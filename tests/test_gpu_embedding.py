@@ -114,6 +114,24 @@ def test_lookup_and_gradient_beyond_2_to_31_elements(native_libs):
     assert dx[rows - 1].eq(120).all() and dx[1_048_576].eq(60).all()
 
 
+def test_lookup_of_more_tokens_than_a_launch_holds(native_libs):
+    """Rows of 513 words are a workgroup each, and 2^24 workgroups one more than a launch may have: the last
+    tokens are another launch's."""
+    from raf_amd import op
+
+    n, rows, width = (1 << 24) + 5, 3, 4104
+    if torch.cuda.mem_get_info()[0] < 2.2 * n * width:
+        pytest.skip("needs 138 GB of free memory")
+    x = _randn(rows, width, dtype=BF16).to(DEV)
+    ids = torch.arange(n, device=DEV, dtype=I32) % 4  # 3 is outside
+    y = op.embedding(x, ids)
+    zero = torch.cat([x, torch.zeros(1, width, dtype=BF16, device=DEV)])
+    for at in (0, 4_000_000, (1 << 24) - 1028, n - 1024):
+        assert torch.equal(y[at:at + 1024], zero[ids[at:at + 1024].long()])
+    del y
+    torch.cuda.empty_cache()
+
+
 def _check_dx(got, dy, ids, rows, scale=1.0, padding=None, first=0, old=None):
     want, size, count = vocab_f64.embedding_dx(dy.float().numpy(), ids.numpy(), rows, np.float32(scale), padding, first)
     out = got.dtype

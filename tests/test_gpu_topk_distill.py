@@ -171,6 +171,34 @@ def test_more_rows_than_a_grid_dimension_holds(native_libs):
     _all(z, idx, t, labels, dloss, temperature=2.0, hard=1.0)
 
 
+def test_more_rows_than_a_launch_holds(native_libs):
+    """2^24 workgroups of 256 threads are one more than a launch may have: the loss and the combined call go on
+    in another.  Two columns, so that the definition is a formula; each rounding is at most 2^-24 of
+    values below 16, and there are fewer than 64 of them."""
+    from raf_amd import op
+
+    rows = (1 << 24) + 77
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    z = torch.randn(rows, 2, device=DEV, generator=gen)
+    idx = torch.randint(-1, 2, (rows, 1), device=DEV, generator=gen, dtype=I32)
+    idx[-77:] = torch.arange(77, device=DEV, dtype=I32)[:, None] % 2
+    t = torch.randn(rows, 1, device=DEV, generator=gen)
+    dloss = torch.rand(rows, device=DEV, generator=gen) + 0.5
+    live = (idx >= 0).flatten()
+    z64 = z.double()
+    logq = torch.log_softmax(z64, 1)
+    hot = torch.nn.functional.one_hot(idx.flatten().clamp(min=0).long(), 2)
+    want = -(logq * hot).sum(1) * live
+    grad = ((logq.exp() - hot) * dloss.double()[:, None]) * live[:, None]
+    loss, stats = op.topk_distill(z, idx, t)
+    assert ((loss - want).abs() <= 64 * U * 16).all() and not loss[~live].any()
+    assert torch.equal(stats[:, 0], z.max(1).values * live)
+    loss2, got = op.topk_distill_step(z, idx, t, dloss)
+    assert ((loss2 - want).abs() <= 64 * U * 16).all() and ((got - grad).abs() <= 64 * U * 16).all()
+    got = op.topk_distill_dx(dloss, z, idx, t, stats)
+    assert ((got - grad).abs() <= 64 * U * 16).all()
+
+
 def test_the_same_index_twice(native_libs):
     for rows, vocab in ((40, 300), (2, 20_000)):
         for k in (2, 50, 700):
