@@ -158,7 +158,8 @@ int rafhip_raf_topk_distill_make(int32_t kind, const rafhip_tensor_desc* logits,
                                  double soft_weight, double hard_weight, int64_t vocab_size, rafhip_raf_env** env_out);
 
 /* Execute of the five ops above: the tensors in schema order (an absent one as a descriptor of
- * negative rank) and the outputs.  Calls on one env may come from several threads. */
+ * negative rank) and the outputs, all of the shape, dtype and device that the env was made for; others
+ * are an error.  Calls on one env may come from several threads. */
 int rafhip_raf_execute(rafhip_raf_env* env, int32_t n_in, const rafhip_tensor_desc* inputs, int32_t n_out,
                        const rafhip_tensor_desc* outputs, void* workspace, int64_t workspace_bytes, void* stream);
 

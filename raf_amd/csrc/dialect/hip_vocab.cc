@@ -62,10 +62,15 @@ class VocabHipEnv : public OpEnv {
     workspace_bytes_ = bytes;
     if (bytes > 0) RequestWorkspace(&workspace_, cv->device, bytes);
   }
-  // The inputs and outputs of an Execute have the shapes that the OpEnv was made for.
-  const TensorView& Same(const Value& v, const std::vector<int64_t>& shape, const char* what) const {
+  // The inputs and outputs of an Execute have the shapes, dtypes and devices that the OpEnv was made
+  // for: the kernels take them from there.
+  const TensorView& Same(const Value& v, const TensorView& made_for, const char* what) const {
     const TensorView& t = AsTensor(v)->tensor;
-    RAF_CHECK(t.shape == shape, op_ + ": the shape of " + what + " changed since the OpEnv was made");
+    RAF_CHECK(t.shape == made_for.shape, op_ + ": the shape of " + what + " changed since the OpEnv was made");
+    RAF_CHECK(t.dtype.code == made_for.dtype.code && t.dtype.bits == made_for.dtype.bits,
+              op_ + ": the dtype of " + what + " changed since the OpEnv was made");
+    RAF_CHECK(t.device.device_type() == made_for.device.device_type() && t.device.device_id() == made_for.device.device_id(),
+              op_ + ": the device of " + what + " changed since the OpEnv was made");
     return t;
   }
 
@@ -85,7 +90,7 @@ class EmbeddingHipEnv : public VocabHipEnv {
     arg_indices = {args->FieldIndex("x"), args->FieldIndex("indices")};
     x_ = args->x->tensor;
     ids_ = args->indices->tensor;
-    out_shape_ = AsTensor(cv->out)->tensor.shape;
+    out_ = AsTensor(cv->out)->tensor;
     x_dtype_ = KernelDType(x_.dtype);
     out_dtype_ = KernelDType(args->out_dtype);
     scale_ = (float)args->scale;
@@ -103,19 +108,18 @@ class EmbeddingHipEnv : public VocabHipEnv {
 
   void Execute(const std::vector<Value>& inputs, Value output) override {
     RAF_CHECK(inputs.size() == 2, op_ + " takes x and indices");
-    const TensorView& x = Same(inputs[0], x_.shape, "x");
-    const TensorView& ids = Same(inputs[1], ids_.shape, "indices");
-    const TensorView& out = Same(output, out_shape_, "the output");
+    const TensorView& x = Same(inputs[0], x_, "x");
+    const TensorView& ids = Same(inputs[1], ids_, "indices");
+    const TensorView& out = Same(output, out_, "the output");
     Check("rafhip_embedding",
-          rafhip_embedding(x.data, x_dtype_, x_.shape[0], x_.shape[1], ids.data, ids_.dtype.bits, ids_.numel(), first_row_,
+          rafhip_embedding(x.data, x_dtype_, x.shape[0], x.shape[1], ids.data, ids.dtype.bits, ids.numel(), first_row_,
                            scale_, out.data, out_dtype_, Stream()));
   }
 
   static OpEnv* make(const CallValues& cv) { return new EmbeddingHipEnv(cv); }
 
  private:
-  TensorView x_, ids_;
-  std::vector<int64_t> out_shape_;
+  TensorView x_, ids_, out_;
   int32_t x_dtype_ = -1, out_dtype_ = -1;
   float scale_ = 1.f;
   int64_t first_row_ = 0;
@@ -131,13 +135,15 @@ class EmbeddingDxHipEnv : public VocabHipEnv {
     }
     arg_indices = {args->FieldIndex("dy"), args->FieldIndex("indices"), args->FieldIndex("grad")};
     args_ = *args;
-    out_shape_ = AsTensor(cv->out)->tensor.shape;
+    dy_ = args->dy->tensor;
+    ids_ = args->indices->tensor;
+    out_ = AsTensor(cv->out)->tensor;
     dy_dtype_ = KernelDType(args->dy->tensor.dtype);
     out_dtype_ = KernelDType(args->out_dtype);
     RequireDType(dy_dtype_, "dy");
     RequireDType(out_dtype_, "the output");
     RequireDevice(cv);
-    RequireWorkspace(cv, rafhip_embedding_dx_workspace_bytes(args->indices->tensor.numel(), out_shape_[0], out_shape_[1]));
+    RequireWorkspace(cv, rafhip_embedding_dx_workspace_bytes(args->indices->tensor.numel(), out_.shape[0], out_.shape[1]));
   }
 
   void Execute(const CallValues& cv) override {
@@ -148,13 +154,13 @@ class EmbeddingDxHipEnv : public VocabHipEnv {
 
   void Execute(const std::vector<Value>& inputs, Value output) override {
     RAF_CHECK(inputs.size() == 3, op_ + " takes dy, indices and grad");
-    const TensorView& dy = Same(inputs[0], args_.dy->tensor.shape, "dy");
-    const TensorView& ids = Same(inputs[1], args_.indices->tensor.shape, "indices");
-    const TensorView& out = Same(output, out_shape_, "the output");
+    const TensorView& dy = Same(inputs[0], dy_, "dy");
+    const TensorView& ids = Same(inputs[1], ids_, "indices");
+    const TensorView& out = Same(output, out_, "the output");
     RAF_CHECK((inputs[2] != nullptr) == (args_.grad != nullptr), op_ + ": grad came or went since the OpEnv was made");
-    if (inputs[2]) RAF_CHECK(AsTensor(inputs[2])->tensor.data == out.data, op_ + ": the output of a call with grad is grad");
+    if (inputs[2]) RAF_CHECK(Same(inputs[2], out_, "grad").data == out.data, op_ + ": the output of a call with grad is grad");
     Check("rafhip_embedding_dx",
-          rafhip_embedding_dx(dy.data, dy_dtype_, ids.data, ids.dtype.bits, ids.numel(), out_shape_[0], out_shape_[1],
+          rafhip_embedding_dx(dy.data, dy_dtype_, ids.data, ids.dtype.bits, ids.numel(), out.shape[0], out.shape[1],
                               args_.first_row, args_.has_padding ? 1 : 0, args_.padding_index, (float)args_.scale, out.data,
                               out_dtype_, args_.grad ? 1 : 0, workspace_, workspace_bytes_, Stream()));
   }
@@ -163,7 +169,7 @@ class EmbeddingDxHipEnv : public VocabHipEnv {
 
  private:
   schema::EmbeddingDxArgs args_;
-  std::vector<int64_t> out_shape_;
+  TensorView dy_, ids_, out_;
   int32_t dy_dtype_ = -1, out_dtype_ = -1;
 };
 
@@ -179,7 +185,14 @@ class TopkDistillHipEnv : public VocabHipEnv {
     }
     for (const char* field : {"logits", "topk_indices", "topk_logits", "labels", "dloss", "stats"})
       arg_indices.push_back(args->FieldIndex(field));
-    args_ = *args;
+    for (const auto& t : {args->logits, args->topk_indices, args->topk_logits, args->labels, args->dloss, args->stats})
+      ins_.push_back(t ? t->tensor : TensorView());
+    has_labels_ = args->labels != nullptr;
+    if (kind == kGradient) {
+      outs_ = {AsTensor(cv->out)->tensor};
+    } else {
+      for (const Value& field : AsTuple(cv->out)->fields) outs_.push_back(AsTensor(field)->tensor);
+    }
     const TensorView& z = args->logits->tensor;
     const TensorView& index = args->topk_indices->tensor;
     width_ = z.shape.back();
@@ -217,41 +230,36 @@ class TopkDistillHipEnv : public VocabHipEnv {
   void Execute(const std::vector<Value>& inputs, Value output) override {
     RAF_CHECK(inputs.size() == 6, op_ + " takes logits, topk_indices, topk_logits, labels, dloss and stats");
     rafhip_topk_distill_args call = call_;
-    const std::vector<int64_t>& logits_shape = args_.logits->tensor.shape;
-    const std::vector<int64_t>& index_shape = args_.topk_indices->tensor.shape;
-    const std::vector<int64_t> rows(logits_shape.begin(), logits_shape.end() - 1);
-    call.logits = Same(inputs[0], logits_shape, "logits").data;
-    call.topk_indices = Same(inputs[1], index_shape, "topk_indices").data;
-    call.topk_logits = Same(inputs[2], index_shape, "topk_logits").data;
-    RAF_CHECK((inputs[3] != nullptr) == (args_.labels != nullptr), op_ + ": labels came or went since the OpEnv was made");
-    call.labels = inputs[3] ? Same(inputs[3], rows, "labels").data : nullptr;
+    call.logits = Same(inputs[0], ins_[0], "logits").data;
+    call.topk_indices = Same(inputs[1], ins_[1], "topk_indices").data;
+    call.topk_logits = Same(inputs[2], ins_[2], "topk_logits").data;
+    RAF_CHECK((inputs[3] != nullptr) == has_labels_, op_ + ": labels came or went since the OpEnv was made");
+    call.labels = inputs[3] ? Same(inputs[3], ins_[3], "labels").data : nullptr;
     const float* dloss = nullptr;
     int64_t dloss_count = 0;
     if (kind_ != kLoss) {
-      const TensorView& d = Same(inputs[4], args_.dloss->tensor.shape, "dloss");
+      const TensorView& d = Same(inputs[4], ins_[4], "dloss");
       dloss = static_cast<const float*>(d.data);
       dloss_count = d.numel();
     }
-    std::vector<int64_t> stats_shape = rows;
-    stats_shape.push_back(3);
     if (kind_ == kGradient) {
-      const TensorView& stats = Same(inputs[5], stats_shape, "stats");
+      const TensorView& stats = Same(inputs[5], ins_[5], "stats");
       Check("rafhip_topk_distill_dx",
             rafhip_topk_distill_dx(&call, dloss, dloss_count, static_cast<const float*>(stats.data),
-                                   Same(output, logits_shape, "dlogits").data, width_, Stream()));
+                                   Same(output, outs_[0], "dlogits").data, width_, Stream()));
       return;
     }
     const auto outs = AsTuple(output);
     RAF_CHECK(outs->fields.size() == 2, op_ + " has two outputs");
-    float* loss = static_cast<float*>(Same(outs->fields[0], rows, "loss").data);
+    float* loss = static_cast<float*>(Same(outs->fields[0], outs_[0], "loss").data);
     if (kind_ == kLoss) {
-      float* stats = static_cast<float*>(Same(outs->fields[1], stats_shape, "stats").data);
+      float* stats = static_cast<float*>(Same(outs->fields[1], outs_[1], "stats").data);
       Check("rafhip_topk_distill", rafhip_topk_distill(&call, loss, stats, workspace_, workspace_bytes_, Stream()));
       return;
     }
     Check("rafhip_topk_distill_step",
-          rafhip_topk_distill_step(&call, dloss, dloss_count, loss, Same(outs->fields[1], logits_shape, "dlogits").data,
-                                   width_, workspace_, workspace_bytes_, Stream()));
+          rafhip_topk_distill_step(&call, dloss, dloss_count, loss, Same(outs->fields[1], outs_[1], "dlogits").data, width_,
+                                   workspace_, workspace_bytes_, Stream()));
   }
 
   static OpEnv* make(const CallValues& cv) { return new TopkDistillHipEnv(cv, "raf.op.hip.topk_distill", kLoss); }
@@ -260,7 +268,8 @@ class TopkDistillHipEnv : public VocabHipEnv {
 
  private:
   Kind kind_;
-  schema::TopkDistillArgs args_;
+  std::vector<TensorView> ins_, outs_;  // in the schema's order
+  bool has_labels_ = false;
   rafhip_topk_distill_args call_ = {};
   int64_t width_ = 0;
 };
