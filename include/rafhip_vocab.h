@@ -12,6 +12,10 @@
  * Results do not depend on the launch, the stream or the run: every sum is taken in an order that
  * the data fixes.
  *
+ * An output or workspace that shares bytes with an input, or with another output, is refused
+ * (RAFHIP_ERR_INVALID_ARG): the kernels read while they write.  A matrix of rows that lie apart
+ * counts from its first element to its last.
+ *
  * Element types: RAFHIP_F32, RAFHIP_F16 and RAFHIP_BF16 in any mixture; indices are signed, of
  * index_bits 32 or 64.  Everything is computed in fp32 or wider and rounded once on store.
  * Pointers need their element's alignment only.
@@ -34,7 +38,7 @@ extern "C" {
  * for n indices and a table x of rows x width (contiguous).  An index outside
  * [first_row, first_row + rows) -- another shard's, or a negative one that marks nothing -- gives a
  * row of zeros.  first_row >= 0 places a vocabulary shard.
- * y: n x width of y_dtype, contiguous; it must not overlap x.  n, rows and width may be 0.
+ * y: n x width of y_dtype, contiguous.  n, rows and width may be 0.
  */
 int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, int64_t width, const void* indices,
                      int32_t index_bits, int64_t n, int64_t first_row, float scale, void* y,
@@ -47,7 +51,7 @@ int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, int64_t width
  * order fixed by their positions, so equal inputs give equal bits.  Indices outside the table and,
  * with has_padding, indices equal to padding_index take no part (their dy is not read).  With
  * accumulate, rows without a token keep their bits.
- * dy: n x width of dy_dtype, dx: rows x width of dx_dtype, contiguous, not overlapping.
+ * dy: n x width of dy_dtype, dx: rows x width of dx_dtype, contiguous.
  * workspace: rafhip_embedding_dx_workspace_bytes(n, rows, width) bytes (0 for short calls, then it
  * may be NULL), 16-byte aligned, no initialisation needed.  That function is host arithmetic; it returns -1 for
  * sizes that are not supported: 2^21 rows or more, 2^24 columns or more, or more tokens than 512
@@ -104,7 +108,7 @@ int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* loss, float
 
 /* Gradient from the forward call's stats (same args).  dloss: `dloss_count` fp32 values, rows of
  * them or one for all rows.  dlogits: rows x out_width of the logits' dtype, contiguous,
- * out_width >= vocab; the columns behind vocab are written as zeros.  Must not overlap an input. */
+ * out_width >= vocab; the columns behind vocab are written as zeros. */
 int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, const float* dloss, int64_t dloss_count,
                            const float* stats, void* dlogits, int64_t out_width, void* stream);
 

@@ -931,6 +931,9 @@ extern "C" int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, in
   if ((rows > 0 && !x) || !indices || !y) return fail(RAFHIP_ERR_INVALID_ARG, "%s: null tensor", who);
   if (!is_aligned(x, element_bytes(x_dtype)) || !is_aligned(y, element_bytes(y_dtype)) || !is_aligned(indices, index_bits / 8))
     return fail(RAFHIP_ERR_INVALID_ARG, "%s: a tensor is not element-aligned", who);
+  const Extent ins[] = {{"x", x, rows * width * element_bytes(x_dtype)}, {"indices", indices, n * (index_bits / 8)}};
+  const Extent outs[] = {{"y", y, n * width * element_bytes(y_dtype)}};
+  if (int st = check_apart(who, outs, ins)) return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows == 0) {
     with_element(y_dtype, [&](auto ty) {
@@ -998,6 +1001,9 @@ extern "C" int rafhip_embedding_dx(const void* dy, int32_t dy_dtype, const void*
   if (need > 0 && !is_aligned(workspace, 16))
     return fail(RAFHIP_ERR_WORKSPACE, "%s: workspace %p is not 16-byte aligned", who, workspace);
   if (n == 0 && accumulate) return RAFHIP_OK;
+  const Extent ins[] = {{"dy", dy, n * width * element_bytes(dy_dtype)}, {"indices", indices, n * (index_bits / 8)}};
+  const Extent outs[] = {{"dx", dx, rows * width * element_bytes(dx_dtype)}, {"workspace", workspace, need}};
+  if (int st = check_apart(who, outs, ins)) return st;
   Layout l;
   layout_of(n, rows, width, &l);
   const Which which{rows, first_row, padding_index, has_padding != 0};

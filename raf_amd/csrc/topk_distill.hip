@@ -824,6 +824,21 @@ int check_gradient(const char* who, const rafhip_topk_distill_args& a, const flo
   return RAFHIP_OK;
 }
 
+// Outputs against the inputs of every call, the gradient's own (none: NULL) and each other.
+template <size_t kOuts>
+int check_extents(const char* who, const rafhip_topk_distill_args& a, const Extent (&outs)[kOuts], const float* dloss = nullptr,
+                  int64_t dloss_count = 0, const float* stats = nullptr) {
+  const int64_t entries = a.rows * a.topk, index = a.index_bits / 8;
+  const Extent ins[] = {
+      {"logits", a.logits, a.vocab > 0 ? ((a.rows - 1) * a.row_stride + a.vocab) * element_bytes(a.logits_dtype) : 0},
+      {"topk_indices", a.topk_indices, entries * index},
+      {"topk_logits", a.topk_logits, entries * element_bytes(a.topk_dtype)},
+      {"labels", a.labels, a.rows * index},
+      {"dloss", dloss, dloss_count * 4},
+      {"stats", stats, a.rows * 12}};
+  return check_apart(who, outs, ins);
+}
+
 // A term that cannot matter is dropped here, so that the kernels neither read for it nor sum for it.
 Task task_of(const rafhip_topk_distill_args& a, int* mode, float* c0) {
   Task t;
@@ -909,6 +924,8 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
   const bool split = loss_is_split(a.rows, a.vocab);
   const int64_t need = split ? parts_bytes(a.rows, a.vocab) : 0;
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
+  const Extent outs[] = {{"loss", loss, a.rows * 4}, {"stats", stats, a.rows * 12}, {"workspace", workspace, need}};
+  if (int st = check_extents(who, a, outs)) return st;
   int sums;
   float c0;
   const Task t = task_of(a, &sums, &c0);
@@ -947,6 +964,8 @@ extern "C" int rafhip_topk_distill_dx(const rafhip_topk_distill_args* args, cons
   if (a.rows == 0 || out_width == 0) return RAFHIP_OK;
   if (int st = check_pointers(who, a)) return st;
   if (!stats || !is_aligned(stats, 4)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: stats %p", who, (const void*)stats);
+  const Extent outs[] = {{"dlogits", dlogits, a.rows * out_width * element_bytes(a.logits_dtype)}};
+  if (int st = check_extents(who, a, outs, dloss, dloss_count, stats)) return st;
   int sums;
   float c0;
   const Task t = task_of(a, &sums, &c0);
@@ -985,6 +1004,10 @@ extern "C" int rafhip_topk_distill_step(const rafhip_topk_distill_args* args, co
   const int block = step_block(a.rows, a.vocab, a.logits_dtype);
   const int64_t need = block > 0 ? 0 : parts_bytes(a.rows, a.vocab);
   if (int st = check_workspace(who, need, workspace, workspace_bytes)) return st;
+  const Extent outs[] = {{"loss", loss, a.rows * 4},
+                         {"dlogits", dlogits, a.rows * out_width * element_bytes(a.logits_dtype)},
+                         {"workspace", workspace, need}};
+  if (int st = check_extents(who, a, outs, dloss, dloss_count)) return st;
   int sums;
   float c0;
   const Task t = task_of(a, &sums, &c0);

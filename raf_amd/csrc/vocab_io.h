@@ -14,6 +14,7 @@
 #include <cstdint>
 
 #include "half_types.h"
+#include "status.h"
 
 namespace rafhip {
 
@@ -122,6 +123,29 @@ void with_index(int32_t index_bits, F&& f) {
 }
 
 inline int element_bytes(int32_t dtype) { return dtype == 0 ? 4 : dtype == 1 || dtype == 2 ? 2 : 0; }
+
+// What a call reads or writes.  The kernels read their inputs while they write, so the entry points refuse
+// an output that shares bytes with an input or another output.
+struct Extent {
+  const char* name;
+  const void* at;
+  int64_t bytes;
+};
+inline bool share_bytes(const Extent& a, const Extent& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+template <size_t kOuts, size_t kIns>
+int check_apart(const char* who, const Extent (&outs)[kOuts], const Extent (&ins)[kIns]) {
+  for (size_t i = 0; i < kOuts; ++i) {
+    for (const Extent& in : ins)
+      if (share_bytes(outs[i], in)) return fail(RAFHIP_ERR_INVALID_ARG, "%s: %s overlaps %s", who, outs[i].name, in.name);
+    for (size_t j = 0; j < i; ++j)
+      if (share_bytes(outs[i], outs[j]))
+        return fail(RAFHIP_ERR_INVALID_ARG, "%s: %s overlaps %s", who, outs[i].name, outs[j].name);
+  }
+  return RAFHIP_OK;
+}
 
 inline bool is_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0; }
 

@@ -260,13 +260,13 @@ class TopkDistill:
             raise ValueError(f"{name}: {t.numel()} elements")
         return t
 
-    def _out(self, out):
+    def _out(self, out, *read):
         if out is None:
             return torch.empty(self.rows, self.vocab, dtype=self.logits.dtype, device=self.logits.device)
         _vocab_tensor(out, "out", (self.logits.dtype,), self.logits.device)
         if out.dim() != 2 or out.shape[0] != self.rows or out.shape[1] < self.vocab:
             raise ValueError(f"out: shape {tuple(out.shape)}")
-        _apart(out, self.logits, *(t for t in self._keep if t is not None))
+        _apart(out, self.logits, *(t for t in (*self._keep, *read) if t is not None))
         return out
 
     def loss(self):
@@ -284,7 +284,7 @@ class TopkDistill:
         """``rafhip_topk_distill_dx``: the gradient for the logits; ``out`` may be wider than vocab."""
         self._f32(dloss, "dloss", (1, self.rows))
         self._f32(stats, "stats", (3 * self.rows,))
-        out = self._out(out)
+        out = self._out(out, dloss, stats)
         with torch.cuda.device(self.logits.device):
             check(_lib.optim().rafhip_topk_distill_dx(ctypes.byref(self.args), dloss.data_ptr(), dloss.numel(),
                                                       stats.data_ptr(), out.data_ptr(), out.shape[1],
@@ -294,7 +294,7 @@ class TopkDistill:
     def step(self, dloss, out=None):
         """``rafhip_topk_distill_step``: ``(loss, gradient)`` at once."""
         self._f32(dloss, "dloss", (1, self.rows))
-        out = self._out(out)
+        out = self._out(out, dloss)
         dev = self.logits.device
         loss = torch.empty(self.rows, dtype=torch.float32, device=dev)
         ws, at, nbytes = self._workspace()

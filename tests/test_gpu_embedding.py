@@ -366,3 +366,22 @@ def test_refusals_on_the_device(native_libs):
         op.embedding(x, ids.cpu())
     with pytest.raises(_lib.RafError, match="unsupported sizes"):
         op.embedding_dx(torch.zeros(3, 1, device=DEV), ids, 1 << 21)
+
+
+def test_a_gradient_that_is_its_own_input_is_refused(native_libs):
+    from raf_amd import _lib, kernels, op
+
+    for n in (40, 3000):
+        dy, ids = _randn(n, 16).to(DEV), _ids(n, n, "uniform").to(DEV)
+        with pytest.raises(_lib.RafError, match="dx overlaps dy"):
+            op.embedding_dx(dy, ids, n, grad=dy)
+        room = torch.zeros(2 * n, 16, device=DEV)
+        with pytest.raises(_lib.RafError, match="dx overlaps dy"):  # by one row
+            op.embedding_dx(room[:n], ids, n, grad=room[n - 1:-1])
+        _check_dx(op.embedding_dx(room[:n].copy_(dy), ids, n, grad=room[n:]), dy.cpu(), ids.cpu(), n,
+                  old=torch.zeros(n, 16))  # side by side
+        bits = torch.zeros(n, 16, dtype=I32, device=DEV)  # the gradient within the indices' memory
+        with pytest.raises(_lib.RafError, match="dx overlaps indices"):
+            op.embedding_dx(dy, bits.view(-1)[:n], n, grad=bits.view(F32))
+        with pytest.raises(ValueError, match="overlaps"):
+            kernels.embedding_dx(dy, ids, dy)

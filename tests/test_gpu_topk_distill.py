@@ -446,3 +446,17 @@ def test_refusals_on_the_device(native_libs):
     for out in (room, room.view(-1)[40:440].view(4, 100)):  # the logits' own memory, and part of it
         with pytest.raises(ValueError, match="overlaps"):
             kernels.TopkDistill(room[:, 50:100], idx, t).step(dloss, out=out)
+
+
+def test_gradient_buffers_that_hold_another_input_are_refused(native_libs):
+    from raf_amd import kernels
+
+    for rows, vocab in ((30, 300), (600, 50)):
+        z, idx, t, labels, dloss = (x.to(DEV) for x in _case(rows, vocab, 3))
+        h = kernels.TopkDistill(z, idx, t, 2.0, 1.0, labels, 0.5)
+        loss, stats = h.loss()
+        out = torch.zeros(rows, vocab, device=DEV)
+        of_rows, of_stats = out.view(-1)[5:5 + rows].copy_(dloss), out.view(-1)[-3 * rows:].view(rows, 3)
+        for call in (lambda: h.step(of_rows, out=out), lambda: h.dx(of_rows, stats, out=out), lambda: h.dx(dloss, of_stats, out=out)):
+            with pytest.raises(ValueError, match="overlaps"):
+                call()

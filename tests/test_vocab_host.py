@@ -132,6 +132,53 @@ def test_distill_argument_validation(native_libs):
         assert fn(None, *[None if t is ctypes.c_void_p else 0 for t in fn.argtypes[1:]]) == bad
 
 
+def test_outputs_that_share_bytes_are_refused(native_libs):
+    """Each output against each input and the other outputs: its first byte on the other's last, its last
+    on the other's first, and both in one place."""
+    L = native_libs
+    lib, f32, bf16 = L.optim(), L.RAFHIP_F32, L.RAFHIP_BF16
+    ws = 1 << 24
+
+    def refused(call, sizes, outs):
+        far = {name: (i + 1) << 32 for i, name in enumerate(sizes)}
+        for o in outs:
+            for other in sizes:
+                if other == o or not sizes[o] or not sizes[other]:
+                    continue
+                for at in (far[other] + sizes[other] - 16, far[other] - sizes[o] + 16, far[other]):
+                    at -= at % 16  # the workspace's alignment, and everything's
+                    if not (at < far[other] + sizes[other] and far[other] < at + sizes[o]):
+                        at = far[other]
+                    assert call(**{**far, o: at}) == L.RAFHIP_ERR_INVALID_ARG, (o, other)
+                    message = lib.rafhip_last_error().decode()
+                    assert f"{o} overlaps {other}" in message or f"{other} overlaps {o}" in message, message
+
+    refused(lambda x, indices, y: lib.rafhip_embedding(x, f32, 100, 64, indices, 64, 50, 0, 1.0, y, bf16, None),
+            {"x": 100 * 64 * 4, "indices": 400, "y": 50 * 64 * 2}, ["y"])
+    need = lib.rafhip_embedding_dx_workspace_bytes(5000, 100, 64)
+    refused(lambda dy, indices, dx, workspace: lib.rafhip_embedding_dx(dy, bf16, indices, 32, 5000, 100, 64, 0, 0, 0, 1.0, dx, f32,
+                                                                        1, workspace, need, None),
+            {"dy": 5000 * 64 * 2, "indices": 20000, "dx": 100 * 64 * 4, "workspace": need}, ["dx", "workspace"])
+    refused(lambda dy, indices, dx: lib.rafhip_embedding_dx(dy, bf16, indices, 32, 200, 100, 64, 0, 0, 0, 1.0, dx, f32, 0, None, 0,
+                                                            None),
+            {"dy": 200 * 64 * 2, "indices": 800, "dx": 100 * 64 * 4}, ["dx"])
+
+    def args(logits, topk_indices, topk_logits, labels):
+        return ctypes.byref(_args(L, rows=40, vocab=70_000, row_stride=70_016, topk=8, logits=logits, topk_indices=topk_indices,
+                                  topk_logits=topk_logits, labels=labels))
+
+    ins = {"logits": (39 * 70_016 + 70_000) * 2, "topk_indices": 40 * 64, "topk_logits": 40 * 32, "labels": 320}
+    need = lib.rafhip_topk_distill_workspace_bytes(ctypes.byref(_args(L, rows=40, vocab=70_000, row_stride=70_016)))
+    assert 0 < need < ws
+    refused(lambda loss, stats, workspace, **t: lib.rafhip_topk_distill(args(**t), loss, stats, workspace, ws, None),
+            {**ins, "loss": 160, "stats": 480, "workspace": need}, ["loss", "stats", "workspace"])
+    refused(lambda dloss, stats, dlogits, **t: lib.rafhip_topk_distill_dx(args(**t), dloss, 40, stats, dlogits, 70_001, None),
+            {**ins, "dloss": 160, "stats": 480, "dlogits": 40 * 70_001 * 2}, ["dlogits"])
+    refused(lambda dloss, loss, dlogits, workspace, **t: lib.rafhip_topk_distill_step(args(**t), dloss, 40, loss, dlogits, 70_001,
+                                                                                      workspace, ws, None),
+            {**ins, "dloss": 160, "loss": 160, "dlogits": 40 * 70_001 * 2, "workspace": need}, ["loss", "dlogits", "workspace"])
+
+
 def test_declares_reach_python(native_libs):
     from raf_amd import _lib, op
 
