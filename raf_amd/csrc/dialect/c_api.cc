@@ -495,7 +495,7 @@ int rafhip_raf_sgd_execute(rafhip_raf_env* env, const rafhip_tensor_desc* x,
     if (!env) throw Error("rafhip_raf_sgd_execute: env is NULL");
     std::vector<value::Value> inputs = {FromDesc(x, "x"), FromDesc(dx, "dx"), FromDesc(v, "v")};
     value::Value out = value::MakeTuple({FromDesc(v1, "v1"), FromDesc(x1, "x1")});
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     env->env->Execute(inputs, out);
   });
@@ -556,7 +556,7 @@ int rafhip_raf_lans_execute(rafhip_raf_env* env, int32_t list_len,
       throw Error("rafhip_raf_lans_execute: bad tensor list");
     value::Value tuple = ListTuple(env, list_len, tensor_list, "tensor_list");
     std::vector<value::Value> inputs = {tuple, FromDesc(step, "step")};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), workspace, workspace_bytes);
     env->env->Execute(inputs, tuple);  // output aliases the inputs
   });
@@ -646,7 +646,7 @@ int rafhip_raf_lans_execute_tuple(rafhip_raf_env* env, const rafhip_raf_tuple* t
     if (!env->env) return;  // declared as a no-op
     value::Value tuple = TupleArgument(tensor_list, as_vm, "rafhip_raf_lans_execute_tuple");
     std::vector<value::Value> inputs = {tuple, FromDesc(step, "step")};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), workspace, workspace_bytes);
     env->env->Execute(inputs, tuple);  // output aliases the inputs
   });
@@ -659,7 +659,7 @@ int rafhip_raf_sgd_multi_execute_tuple(rafhip_raf_env* env, const rafhip_raf_tup
     if (!env->env) return;  // declared as a no-op
     value::Value tuple = TupleArgument(tensor_list, as_vm, "rafhip_raf_sgd_multi_execute_tuple");
     std::vector<value::Value> inputs = {tuple};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     env->env->Execute(inputs, tuple);  // output aliases the inputs
   });
@@ -689,7 +689,7 @@ int rafhip_raf_sgd_multi_execute(rafhip_raf_env* env, int32_t list_len,
       throw Error("rafhip_raf_sgd_multi_execute: bad tensor list");
     value::Value tuple = ListTuple(env, list_len, tensor_list, "tensor_list");
     std::vector<value::Value> inputs = {tuple};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     env->env->Execute(inputs, tuple);  // output aliases the inputs
   });
@@ -711,7 +711,7 @@ int rafhip_raf_l2norm_execute(rafhip_raf_env* env, const rafhip_tensor_desc* x,
   return Guard([&] {
     if (!env || !env->env) throw Error("rafhip_raf_l2norm_execute: env is NULL");
     std::vector<value::Value> inputs = {FromDesc(x, "x")};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), workspace, workspace_bytes);
     env->env->Execute(inputs, FromDesc(out, "out"));
   });
@@ -738,7 +738,7 @@ int rafhip_raf_fuse_tensor_execute(rafhip_raf_env* env, int32_t n, const rafhip_
     std::vector<value::Value> fields;
     for (int32_t i = 0; i < n; ++i) fields.push_back(FromDesc(&data[i], "data"));
     std::vector<value::Value> inputs = {value::MakeTuple(std::move(fields))};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     StreamBinding streams(env->env.get(), env->call->device, stream);
     env->env->Execute(inputs, FromDesc(out, "out"));
@@ -771,7 +771,7 @@ int rafhip_raf_defuse_tensor_execute(rafhip_raf_env* env, const rafhip_tensor_de
     std::vector<value::Value> fields;
     for (int32_t i = 0; i < n_out; ++i) fields.push_back(FromDesc(&outs[i], "out"));
     std::vector<value::Value> inputs = {FromDesc(data, "data")};
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     StreamBinding streams(env->env.get(), env->call->device, stream);
     env->env->Execute(inputs, value::MakeTuple(std::move(fields)));
@@ -859,7 +859,7 @@ int rafhip_raf_execute(rafhip_raf_env* env, int32_t n_in, const rafhip_tensor_de
     for (int32_t i = 0; i < n_in; ++i) in.push_back(Optional(&inputs[i], "input"));
     for (int32_t i = 0; i < n_out; ++i) out.push_back(FromDesc(&outputs[i], "output"));
     std::lock_guard<std::mutex> lock(env->executing);
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     WorkspaceBinding bind(env->env.get(), workspace, workspace_bytes);
     env->env->Execute(in, n_out == 1 ? out[0] : value::MakeTuple(out));
   });
@@ -1097,7 +1097,7 @@ int rafhip_raf_traced_sgd_execute(rafhip_raf_env* env, const rafhip_tensor_desc*
     bindings[env->vars[2].get()] = FromDesc(v, "v");
     CallValues call = BindCall(env->fused, bindings, env->call->device);
     call->out = wt;  // out=w: the result shares w's memory (src/op/declare/binary.cc:52-55)
-    OpEnv::SetStreamForAllBackends(call->device, stream);
+    device_api::CallStream on(call->device, stream);
     WorkspaceBinding bind(env->env.get(), nullptr, 0);
     // the executors hand a fused function all of its arguments (arg_indices covers them all)
     env->env->Execute(call->args_as<schema::ListArgs>()->args, call->out);
@@ -1212,7 +1212,7 @@ int rafhip_raf_traced_optimizer_execute(rafhip_raf_env* env, int32_t n, const ra
     if (!env || env->kind < 0) throw Error("rafhip_raf_traced_optimizer_execute: env was not made by rafhip_raf_traced_optimizer_make");
     const rafhip_tensor_desc* all[5] = {g, w, env->kind == 1 ? m : nullptr, v, p};
     auto bindings = BindLists(env, n, all, 5, step);
-    OpEnv::SetStreamForAllBackends(env->call->device, stream);
+    device_api::CallStream on(env->call->device, stream);
     RunGraph(env, bindings, /*make=*/false, allow_partial != 0, workspace, workspace_bytes);
   });
 }

@@ -7,6 +7,7 @@
 //   CPUDeviceAPI   src/device_api/cpu/cpu.cc:18-131: aligned host memory, memcpy, and errors for
 //                  everything that needs a stream or an event.
 //   DeviceAPI::Get / RegisterMaker   src/impl/device_api.cc:18-50.
+#include <atomic>
 #include <cstdlib>
 #include <cstring>
 #include <map>
@@ -44,6 +45,9 @@ void Try(int status, const char* what) {
     throw Error(std::string(what) + " failed with status " + std::to_string(status) + ": " +
                 rafhip_last_error());
 }
+
+thread_local bool t_call_set = false;  // whether the thread is inside a CallStream
+thread_local void* t_call_stream = nullptr;
 
 class CPUDeviceAPI final : public DeviceAPI {
  public:
@@ -155,8 +159,8 @@ class ROCMDeviceAPI final : public DeviceAPI {
   }
   // The reference also forwards the stream to TVM, cuDNN and cuBLAS (cuda.cc:173-178); the hip
   // dialect's OpEnvs read it from here at Execute time.
-  void SetStream(const Device&, void* stream) override { stream_ = stream; }
-  void* GetStream() override { return stream_; }
+  void SetStream(const Device&, void* stream) override { stream_.store(stream); }
+  void* GetStream() override { return t_call_set ? t_call_stream : stream_.load(); }
 
   void* CreateEvent(const Device& dev, uint32_t flags) override {
     RAF_CHECK(dev.device_type() == DevType::kROCM(), "not a rocm device");
@@ -192,15 +196,24 @@ class ROCMDeviceAPI final : public DeviceAPI {
 
  private:
   int device_id_ = 0;
-  // The default stream unless the executor sets one; per thread, so that two threads' calls cannot
-  // exchange their streams between SetStream and Execute.
-  inline static thread_local void* stream_ = nullptr;
+  std::atomic<void*> stream_{nullptr};  // the default stream unless the executor sets one
 };
 
 const bool kCpuRegistered = DeviceAPI::RegisterMaker("cpu", CPUDeviceAPI::make);
 const bool kRocmRegistered = DeviceAPI::RegisterMaker("rocm", ROCMDeviceAPI::make);
 
 }  // namespace
+
+CallStream::CallStream(const Device& dev, void* stream) : outer_set_(t_call_set), outer_(t_call_stream) {
+  op::OpEnv::SetStreamForAllBackends(dev, stream);
+  t_call_set = true;
+  t_call_stream = stream;
+}
+
+CallStream::~CallStream() {
+  t_call_set = outer_set_;
+  t_call_stream = outer_;
+}
 
 bool DeviceAPI::RegisterMaker(const std::string& devtype_name, Maker maker) {
   std::lock_guard<std::mutex> lock(Mu());

@@ -164,6 +164,22 @@ class DeviceAPI {
   static bool RegisterMaker(const std::string& devtype_name, Maker maker);
 };
 
+// The stream of one executor call.  SetStream is the process's setting, as in the reference: whichever
+// thread executes next reads it.  A caller that names the stream with the call itself holds one of
+// these around Execute: GetStream then answers with that stream on this thread, so that two threads'
+// calls cannot exchange their streams between SetStream and Execute.
+class CallStream {
+ public:
+  CallStream(const Device& dev, void* stream);  // also SetStream, as the executors do
+  ~CallStream();
+  CallStream(const CallStream&) = delete;
+  CallStream& operator=(const CallStream&) = delete;
+
+ private:
+  bool outer_set_;
+  void* outer_;
+};
+
 }  // namespace device_api
 
 namespace op {
