@@ -90,12 +90,33 @@ class _Env:
             pass
 
 
-def _workspace(env: "_Env", like: torch.Tensor, stream) -> runtime.Memory:
+class _GraphChunk:
+    """A workspace of the graph that is being captured, from torch's pool of that graph."""
+
+    def __init__(self, nbytes: int, device):
+        self._tensor = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.data = self._tensor.data_ptr()
+
+
+def _capturing(device) -> bool:
+    if device.index not in (None, torch._C._cuda_getDevice()):
+        with torch.cuda.device(device):
+            return torch.cuda.is_current_stream_capturing()
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _workspace(env: "_Env", like: torch.Tensor, stream):
     """The OpEnv's workspace requests as one chunk from the device's memory pool, allocated on the
     call's stream like the VM does around Execute (src/impl/vm/vm.cc:1099-1105, :846-853).  The
     chunk is kept with the OpEnv and reused by later calls on the same stream (which run after this
     one): on ROCm 7.2 a stream-ordered allocation waits for the stream's pending work, which would
-    serialise host and device once per step."""
+    serialise host and device once per step.
+
+    A call that is being captured gets memory of its own that lives and dies with the graph: what the
+    memory pool allocates under capture is the graph's and gone with it, and a kept chunk
+    would be shared by every graph captured on its stream, whose replays need not follow each other."""
+    if _capturing(like.device):
+        return _GraphChunk(env.workspace_bytes, like.device)
     ws = env.workspaces.get(stream)
     if ws is None:
         dev_id = like.device.index if like.device.index is not None else 0
