@@ -85,7 +85,9 @@ class NonOwnedMemory final : public Memory {
   std::shared_ptr<DeviceAPI> api_;
 };
 
-// Stream-ordered: freed on the stream it was allocated on.
+// Stream-ordered: freed on the stream it was allocated on, or, if that is refused because the stream is
+// gone (an OpEnv's workspace may outlive a stream that its caller destroyed, whose work is done
+// then), at once.
 class NonOwnedAsyncMemory final : public Memory {
  public:
   NonOwnedAsyncMemory(void* ptr, void* stream, const Device& dev, std::shared_ptr<DeviceAPI> api)
@@ -94,7 +96,14 @@ class NonOwnedAsyncMemory final : public Memory {
     device = dev;
   }
   ~NonOwnedAsyncMemory() override {
-    if (data != nullptr) Release([&] { api_->FreeMemoryAsync(data, stream_); });
+    if (data == nullptr) return;
+    Release([&] {
+      try {
+        api_->FreeMemoryAsync(data, stream_);
+      } catch (const Error&) {
+        api_->FreeMemory(data);
+      }
+    });
   }
 
  private:

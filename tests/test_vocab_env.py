@@ -1,6 +1,7 @@
 """OpEnvs and the C window against recording stand-ins for the kernel library, without a GPU, built with
 AddressSanitizer and UndefinedBehaviorSanitizer: what Execute refuses (tests/cpp/test_vocab_env.cc)
-and the stream that a call runs on (test_call_stream.cc)."""
+the stream that a call runs on (test_call_stream.cc) and the end of stream-ordered memory
+(test_memory_release.cc)."""
 import os
 import subprocess
 from concurrent.futures import ThreadPoolExecutor
@@ -25,7 +26,7 @@ def build(tmp_path_factory):
     with ThreadPoolExecutor(max_workers=4) as pool:
         layer = list(pool.map(compile_one, [DIALECT / s for s in (*SOURCES, "hip_vocab.cc")]))
 
-    def run(program, own):
+    def run(program, own, quiet=True):
         stub = out / f"{program}_stub.cc"
         write_stub(stub, leave_out=own)
         exe = out / program
@@ -36,6 +37,7 @@ def build(tmp_path_factory):
         r = subprocess.run([str(exe)], capture_output=True, text=True, env=env, timeout=300)
         assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-6000:]
         assert "ALL OK" in r.stdout
+        assert not quiet or not r.stderr
         assert "runtime error" not in r.stderr and "AddressSanitizer" not in r.stderr and "LeakSanitizer" not in r.stderr
 
     return run
@@ -47,3 +49,8 @@ def test_execute_takes_only_what_the_op_env_was_made_for(build):
 
 def test_streams_of_the_process_and_of_a_call(build):
     build("test_call_stream", {"rafhip_device_count", "rafhip_last_error", "rafhip_sgd"})
+
+
+def test_stream_ordered_memory_that_outlives_its_stream(build):
+    build("test_memory_release", {"rafhip_dev_set", "rafhip_dev_alloc_async", "rafhip_dev_free_async", "rafhip_dev_free"},
+          quiet=False)
