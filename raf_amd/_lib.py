@@ -339,6 +339,14 @@ def last_error() -> str:
     return optim().rafhip_last_error().decode("utf-8", "replace")
 
 
+def as_int64(value, name: str) -> int:
+    """An integer for an int64_t argument; ctypes would cut a larger one to its low bits in silence."""
+    value = int(value)
+    if not -(1 << 63) <= value < 1 << 63:
+        raise ValueError(f"{name}: {value} does not fit 64 bits")
+    return value
+
+
 def check(status: int) -> None:
     if status != RAFHIP_OK:
         raise RafHipError(status, last_error())

@@ -12,7 +12,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import LansHParams, RAFHIP_BF16, RAFHIP_F16, RAFHIP_F32, RAFHIP_F64, check
+from ._lib import LansHParams, RAFHIP_BF16, RAFHIP_F16, RAFHIP_F32, RAFHIP_F64, as_int64, check
 
 
 def _current_stream(device) -> int:
@@ -190,8 +190,8 @@ def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_
         _apart(out, x, indices)
     with torch.cuda.device(x.device):
         check(_lib.optim().rafhip_embedding(x.data_ptr(), _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], indices.data_ptr(),
-                                            _INDEX_BITS[indices.dtype], indices.numel(), int(first_row), float(scale),
-                                            out.data_ptr(), _DTYPE_CODE[out.dtype], _current_stream(x.device)))
+                                            _INDEX_BITS[indices.dtype], indices.numel(), as_int64(first_row, "first_row"),
+                                            float(scale), out.data_ptr(), _DTYPE_CODE[out.dtype], _current_stream(x.device)))
     return out
 
 
@@ -210,10 +210,10 @@ def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, out: torch.Tensor, sca
     ws = _scratch(need, dy.device)
     with torch.cuda.device(dy.device):
         check(lib.rafhip_embedding_dx(dy.data_ptr(), _DTYPE_CODE[dy.dtype], indices.data_ptr(), _INDEX_BITS[indices.dtype],
-                                      indices.numel(), out.shape[0], out.shape[1], int(first_row),
-                                      int(padding_idx is not None), int(padding_idx or 0), float(scale), out.data_ptr(),
-                                      _DTYPE_CODE[out.dtype], int(bool(accumulate)), ws.data_ptr() if ws is not None else None,
-                                      max(need, 0), _current_stream(dy.device)))
+                                      indices.numel(), out.shape[0], out.shape[1], as_int64(first_row, "first_row"),
+                                      int(padding_idx is not None), as_int64(padding_idx or 0, "padding_idx"), float(scale),
+                                      out.data_ptr(), _DTYPE_CODE[out.dtype], int(bool(accumulate)),
+                                      ws.data_ptr() if ws is not None else None, max(need, 0), _current_stream(dy.device)))
     return out
 
 

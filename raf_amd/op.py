@@ -19,7 +19,7 @@ from typing import Dict, List, Sequence, Tuple
 import torch
 
 from . import _lib, runtime
-from ._lib import TensorDesc, check_raf
+from ._lib import TensorDesc, as_int64, check_raf
 
 DEV_CPU, DEV_CUDA, DEV_ROCM = 1, 2, 10  # include/raf/device.h:37-50
 
@@ -781,8 +781,8 @@ def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_
     env = _vocab_envs.get(key)
     if env is None:
         code, bits = _out_dtype(x.dtype if out_dtype is None else out_dtype)
-        env = _make_vocab_env(key, x.device, _lib.dialect().rafhip_raf_embedding_make, (x, indices), scale, first_row,
-                              code, bits)
+        env = _make_vocab_env(key, x.device, _lib.dialect().rafhip_raf_embedding_make, (x, indices), scale,
+                              as_int64(first_row, "first_row"), code, bits)
     return _run_vocab(env, (x, indices))[0]
 
 
@@ -806,7 +806,8 @@ def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, num_weight: int, scale
     if env is None:
         code, bits = _out_dtype(out_dtype)
         env = _make_vocab_env(key, dy.device, _lib.dialect().rafhip_raf_embedding_dx_make, (dy, indices, grad),
-                              num_weight, scale, first_row, int(padding_idx is not None), padding_idx or 0, code, bits)
+                              as_int64(num_weight, "num_weight"), scale, as_int64(first_row, "first_row"),
+                              int(padding_idx is not None), as_int64(padding_idx or 0, "padding_idx"), code, bits)
     return _run_vocab(env, (dy, indices, grad), (grad,) if grad is not None else None)[0]
 
 
@@ -822,7 +823,7 @@ def _topk_distill(kind, logits, topk_indices, topk_logits, labels, dloss, stats,
             raise ValueError("logits must have a vocabulary dimension")
         make = lambda *a: _lib.dialect().rafhip_raf_topk_distill_make(kind, *a)
         env = _make_vocab_env(key, logits.device, make, inputs, temperature, soft_weight, hard_weight,
-                              logits.shape[-1] if vocab_size is None else vocab_size)
+                              logits.shape[-1] if vocab_size is None else as_int64(vocab_size, "vocab_size"))
     return _run_vocab(env, inputs)
 
 

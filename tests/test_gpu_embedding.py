@@ -385,3 +385,14 @@ def test_a_gradient_that_is_its_own_input_is_refused(native_libs):
             op.embedding_dx(dy, bits.view(-1)[:n], n, grad=bits.view(F32))
         with pytest.raises(ValueError, match="overlaps"):
             kernels.embedding_dx(dy, ids, dy)
+
+
+def test_direct_handles_refuse_integers_beyond_64_bits(native_libs):
+    from raf_amd import kernels
+
+    x, ids, dx = _randn(5, 8).to(DEV), torch.zeros(3, dtype=I64, device=DEV), torch.zeros(5, 8, device=DEV)
+    for call in (lambda: kernels.embedding(x, ids, first_row=1 << 64),
+                 lambda: kernels.embedding_dx(x[:3], ids, dx, first_row=1 << 64),
+                 lambda: kernels.embedding_dx(x[:3], ids, dx, padding_idx=1 << 64)):
+        with pytest.raises(ValueError, match="does not fit 64 bits"):
+            call()

@@ -221,6 +221,22 @@ def test_declares_reach_python(native_libs):
         op.embedding(x, ids, out_dtype=torch.complex64)
 
 
+def test_integers_beyond_64_bits_are_refused_not_cut(native_libs):
+    from raf_amd import op
+
+    x, ids = torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
+    z, top, t = torch.zeros(4, 9), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    dy, wraps = torch.zeros(3, 8), 1 << 64
+    for name, call in (("first_row", lambda: op.embedding(x, ids, first_row=wraps)),
+                       ("first_row", lambda: op.embedding_dx(dy, ids, 5, first_row=wraps + 1)),
+                       ("num_weight", lambda: op.embedding_dx(dy, ids, wraps + 5)),
+                       ("padding_idx", lambda: op.embedding_dx(dy, ids, 5, padding_idx=1 - wraps)),
+                       ("vocab_size", lambda: op.topk_distill(z, top, t, vocab_size=wraps + 9)),
+                       ("vocab_size", lambda: op.topk_distill_step(z, top, t, torch.zeros(4), vocab_size=wraps))):
+        with pytest.raises(ValueError, match=f"{name}: .* does not fit 64 bits"):
+            call()
+
+
 def test_direct_handles_refuse_cpu_tensors():
     from raf_amd import kernels
 
