@@ -76,7 +76,8 @@ int rafhip_embedding_dx(const void* dy, int32_t dy_dtype, const void* indices, i
  * whose label is missing (labels NULL, or outside [0, vocab)) no hard term; a row with neither has
  * loss 0 and a gradient of zeros, and its logits are not read, so padded rows may hold anything.
  * Logits of -inf have probability zero; a row of nothing else, +inf and NaN give NaN.
- * Column sums are fp32, row values fp64, the gradient is rounded once.
+ * Columns are summed in fp32, at most 256 one after the other, and these sums and the row's values in
+ * fp32 or fp64; the gradient is rounded once.
  */
 typedef struct rafhip_topk_distill_args {
   const void* logits;       /* rows x vocab, rows `row_stride` elements apart                  */

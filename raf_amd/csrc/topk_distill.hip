@@ -152,7 +152,7 @@ __device__ __forceinline__ bool any_entry(const Task& a, int64_t row) {
 // the gradient 308 and 320, both at once 354 and 383.
 enum { kOne = 0, kBoth, kSquare, kFourth };
 
-// Running maximum and sums over the columns a lane has seen.  c0 is log2(e)/T, or log2(e) if only the
+// Maximum and sums over the columns a lane has seen.  c0 is log2(e)/T, or log2(e) if only the
 // hard term is wanted.
 template <int kSums>
 struct Exps {
@@ -227,12 +227,16 @@ __device__ __forceinline__ Stretch stretch_of(const T* at, int count) {
   return s;
 }
 
-// The sums over `count` columns at z, by the workgroup.
-template <typename T, int kSums>
+// The sums over `count` columns at z, by the workgroup.  With kLong a thread adds the 32 columns that it has in
+// flight in fp32 and these sums in fp64: in fp32 throughout, each of the thousands of columns that a
+// thread has of a long row would be rounded to the step of the sum so far (65 rows of 2^24 columns: log S
+// off by 2e-4).
+template <typename T, int kSums, bool kLong>
 __device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int count, float c0) {
   constexpr int kInFlight = 4;
   const int block = (int)blockDim.x;
   const Stretch s = stretch_of(z, count);
+  double s0 = 0.0, s1 = 0.0;  // relative to a.m
   for (int w0 = threadIdx.x; w0 < s.words; w0 += block * kInFlight) {
     typename Wide<T>::Raw raw[kInFlight];
 #pragma unroll
@@ -248,8 +252,16 @@ __device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int coun
 #pragma unroll
       for (int j = 0; j < kWide; ++j) top = fmaxf(top, Wide<T>::get(raw[u], j));
     }
-    a.rescale(top, c0);
     const float b = Exps<kSums>::base(top);
+    if constexpr (kLong) {
+      const float d = a.m - b, e = exp2_hw(d * c0);
+      s0 *= e;
+      if constexpr (kSums != kOne) s1 *= Exps<kSums>::hard(d, e);
+      a.m = top;
+      a.s0 = a.s1 = 0.f;
+    } else {
+      a.rescale(top, c0);
+    }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (w0 + u * block < s.words) {
@@ -257,6 +269,14 @@ __device__ __forceinline__ void add_columns(Exps<kSums>& a, const T* z, int coun
         for (int j = 0; j < kWide; ++j) a.term(Wide<T>::get(raw[u], j), b, c0);
       }
     }
+    if constexpr (kLong) {
+      s0 += a.s0;
+      if constexpr (kSums != kOne) s1 += a.s1;
+    }
+  }
+  if constexpr (kLong) {
+    a.s0 = (float)s0;
+    a.s1 = (float)s1;
   }
   // The single elements: the first and the last few, one per thread.
   const int i = (int)threadIdx.x;
@@ -317,15 +337,15 @@ __device__ __forceinline__ void finish_row(const Task& a, int64_t row, const Tea
 
 constexpr int kMaxBlock = 1024;
 
-template <typename T, int kSums>
-__global__ __launch_bounds__(kMaxBlock, 8) void row_loss(Task a, float c0, float* loss, float* stats) {
+template <typename T, int kSums, bool kLong>
+__global__ __launch_bounds__(kMaxBlock, kLong ? 7 : 8) void row_loss(Task a, float c0, float* loss, float* stats) {
   __shared__ float red[kMaxBlock / kLanes][3];
   const int64_t row = blockIdx.x;
   const Teacher t = teacher_of(a, row);
   const int label = a.label(row);
   Exps<kSums> s;
   if (t.any || label >= 0) {  // the same in all threads
-    add_columns<T, kSums>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
+    add_columns<T, kSums, kLong>(s, (const T*)a.logits + row * a.row_stride, a.vocab, c0);
     block_merge(s, red, c0);
   }
   if (threadIdx.x < kLanes) finish_row<T>(a, row, t, label, row_sums_of(s), loss, stats);
@@ -342,7 +362,7 @@ __global__ __launch_bounds__(kPartBlock) void row_part(Task a, float c0, int per
   const int count = a.vocab - from < per_split ? a.vocab - from : per_split;
   Exps<kSums> s;
   if (a.label(row) >= 0 || any_entry(a, row)) {  // a row without targets is not read
-    add_columns<T, kSums>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
+    add_columns<T, kSums, false>(s, (const T*)a.logits + row * a.row_stride + from, count, c0);
     block_merge(s, red, c0);
   }
   if (threadIdx.x == 0) {
@@ -741,6 +761,11 @@ bool loss_is_split(int64_t rows, int64_t vocab) { return rows <= kFewRows && voc
 // with 256 and 512 threads: 256 rows of 8192 5.6 and 6.5; 8 rows of 50257 9.2 and 8.3, 256 11.5 and 10.0).
 int loss_block(int64_t rows, int64_t vocab) { return rows < kManyRows && vocab > 16384 ? 512 : 256; }
 
+// Columns of a thread whose sum fp32 takes one after the other; row_part's threads have 128 at most, row_step's
+// 200.  Rows beyond pay for the fp64 sums (16 bits, us without and with: 2048 rows of 131072 97.3 and 97.2 at T = 1,
+// 103.1 and 104 at T = 1.5 with labels, 100.4 and 105.9 at T = 4; 4096 rows of 50257 at T = 4 80 and 85).
+constexpr int kMaxChain = 224;
+
 // Threads of row_step for a row, the fewest whose registers hold it, from 256 with many rows and from 512
 // with fewer, or 0: then row_part and row_grad read it twice, with workgroups for every CU.  So are a few
 // long rows (16 bits, us twice and once: 8 rows of 8192 12.4 and 11.5, of 32000 12.3 and 14, of 160000 9.5
@@ -936,10 +961,16 @@ extern "C" int rafhip_topk_distill(const rafhip_topk_distill_args* args, float* 
       constexpr int kSums = decltype(mode)::value;
       if (!split) {
         const int block = loss_block(a.rows, a.vocab);
-        for_row_blocks(t, sizeof(T), max_grid_x(block), [&](const Task& part, int64_t r0) {
-          hipLaunchKernelGGL((row_loss<T, kSums>), dim3((unsigned)part.rows), dim3((unsigned)block), 0, s, part, c0, loss + r0,
-                             stats ? stats + r0 * 3 : nullptr);
-        });
+        auto launch = [&](auto kernel) {
+          for_row_blocks(t, sizeof(T), max_grid_x(block), [&](const Task& part, int64_t r0) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)part.rows), dim3((unsigned)block), 0, s, part, c0, loss + r0,
+                               stats ? stats + r0 * 3 : nullptr);
+          });
+        };
+        if (a.vocab > (int64_t)block * kMaxChain)
+          launch(row_loss<T, kSums, true>);
+        else
+          launch(row_loss<T, kSums, false>);
         return;
       }
       float* parts = static_cast<float*>(workspace);

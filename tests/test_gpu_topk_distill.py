@@ -166,6 +166,30 @@ def test_a_row_too_long_for_registers_among_many(native_libs):
     _all(z, idx, t, labels, dloss, temperature=2.0)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, temperature", [(65, 2.0), (65, 1.5), (65, 1.0), (520, 2.0), (3, 2.0)])
+def test_sums_over_very_many_columns(native_libs, rows, temperature, dtype):
+    """Rows of millions of equal columns behind larger ones (which every thread meets first, so that the others
+    count less than one each): no thread's chain of additions grows with the row beyond what the bound
+    above counts."""
+    from raf_amd import op
+
+    vocab, first = 1 << (24 if rows < 100 else 21), 1 << 15
+    low = torch.tensor(-1.2).to(dtype)
+    z = torch.full((rows, vocab), float(low), dtype=dtype, device=DEV)
+    z[:, :first] = 0.0
+    at = torch.arange(rows, device=DEV)
+    more = dict(temperature=temperature, labels=at, hard_weight=1.0)
+    loss, stats = op.topk_distill(z, at[:, None], torch.zeros(rows, 1, device=DEV), **more)
+    want = [np.log(first + (vocab - first) * np.exp(float(low.double()) / t)) for t in (temperature, 1.0)]
+    bound = U * (300 + 8 * (1.21 * 1.4427 + np.log2(vocab)))
+    assert not stats[:, 0].any()
+    for k in range(2):
+        assert ((stats[:, k + 1].double() - want[k]).abs() <= bound + 1.01 * U * want[k]).all()
+    total = temperature ** 2 * want[0] + want[1]
+    assert ((loss.double() - total).abs() <= bound * (temperature ** 2 + 1) + 1.01 * U * total).all()
+
+
 def test_more_rows_than_a_grid_dimension_holds(native_libs):
     z, idx, t, labels, dloss = _case(66_000, 3, 2, F32)
     _all(z, idx, t, labels, dloss, temperature=2.0, hard=1.0)
