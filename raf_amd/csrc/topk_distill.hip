@@ -396,7 +396,9 @@ __global__ __launch_bounds__(kLanes) void join_loss(Task a, float c0, const floa
 
 // ------------------------------------------------------------------------------------ gradient
 // g(z) = a0 exp2((z - m) c0 - l0) [+ a1 exp2((z - m) log2(e) - l1)], before the corrections.  Where the
-// second exponential is a power of the first, a1 holds the factor of that power.
+// second exponential is a power of the first, l0 is taken so that this power is the label's softmax
+// itself, and a0 makes up for it.  That factor is at most 1, since S_1 is at most the power of S_T (the other way round
+// a1 would have to hold up to vocab^3, beyond fp32 for large dloss).
 struct Grad {
   float m, c0, l0, a0, l1, a1;
   template <int kSums>
@@ -421,8 +423,10 @@ __device__ __forceinline__ Grad grad_of(const Task& a, float c0, float dloss, bo
     g.a0 = as;
     g.l1 = log2_hard;
     g.a1 = ah;
-    if constexpr (kSums == kSquare || kSums == kFourth)
-      g.a1 = hard ? ah * exp2_hw((kSums == kSquare ? 2.f : 4.f) * log2_soft - log2_hard) : 0.f;
+    if constexpr (kSums == kSquare || kSums == kFourth) {
+      g.l0 = (kSums == kSquare ? 0.5f : 0.25f) * log2_hard;
+      g.a0 = soft ? as * exp2_hw(g.l0 - log2_soft) : 0.f;
+    }
   } else {
     g.l0 = soft ? log2_soft : log2_hard;
     g.a0 = as + ah;

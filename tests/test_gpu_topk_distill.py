@@ -309,6 +309,22 @@ def test_upstream_gradient_of_one_element_and_of_zero(native_libs):
     assert not op.topk_distill_step(zd, idxd, td, zero, temperature=2.0)[1].any()
 
 
+@pytest.mark.parametrize("rows, vocab", [(37, 3000), (600, 3000), (5, 30_000)])
+@pytest.mark.parametrize("temperature", [1.0, 1.5, 2.0, 4.0])
+def test_upstream_gradient_of_any_magnitude(native_libs, temperature, rows, vocab):
+    """A power of two in dloss changes nothing but the exponents, as long as the gradient is within fp32's range."""
+    from raf_amd import op
+
+    z, idx, t, labels, dloss = (x.to(DEV) for x in _case(rows, vocab, 6, F32))
+    more = dict(temperature=temperature, labels=labels, hard_weight=0.5)
+    loss, stats = op.topk_distill(z, idx, t, **more)
+    for grad in (lambda dl: op.topk_distill_dx(dl, z, idx, t, stats, **more), lambda dl: op.topk_distill_step(z, idx, t, dl, **more)[1]):
+        want = grad(dloss)
+        for scale in (2.0 ** 118, 2.0 ** -40):
+            got = grad(dloss * scale)
+            assert torch.isfinite(got).all() and torch.equal(got / scale, want)
+
+
 def test_gradient_against_differences(native_libs):
     """The row losses of the kernel itself, moved by a step in single logits."""
     from raf_amd import op
