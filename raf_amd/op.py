@@ -136,12 +136,18 @@ class _EnvCache(collections.OrderedDict):
     def get(self, key, default=None):
         env = super().get(key, default)
         if env is not default:
-            self.move_to_end(key)
+            self._used(key)
         return env
+
+    def _used(self, key):
+        try:
+            self.move_to_end(key)
+        except KeyError:  # another thread has pushed it out meanwhile; this one holds the OpEnv itself
+            pass
 
     def __setitem__(self, key, env):
         super().__setitem__(key, env)
-        self.move_to_end(key)
+        self._used(key)
         while len(self) > self.capacity:
             self.popitem(last=False)
 
