@@ -84,9 +84,9 @@ typedef struct rafhip_topk_distill_args {
   const void* topk_indices; /* rows x topk, contiguous                                         */
   const void* topk_logits;  /* rows x topk, contiguous                                         */
   const void* labels;       /* rows, or NULL                                                   */
-  int64_t rows;
+  int64_t rows;             /* below 2^31                                                      */
   int64_t vocab;            /* columns that take part: fewer than 2^28                         */
-  int64_t row_stride;       /* >= vocab                                                        */
+  int64_t row_stride;       /* >= vocab, below 2^28                                            */
   int32_t topk;             /* 0 .. RAFHIP_MAX_TOPK                                            */
   int32_t logits_dtype;
   int32_t topk_dtype;

@@ -637,7 +637,9 @@ struct StepWords<Bf16> : StepWords<_Float16> {};
 // each logit is read once.  With many rows the workgroup is the smallest that holds a row: four of 256
 // threads share a CU, and while one waits for its row or for the others' sums the rest read, compute
 // and write (8192 rows of 50257 in 16 bits, T = 2 with labels: 354 us, with one of 1024 threads 461;
-// T = 1 without labels 350 both).
+// T = 1 without labels 350 both).  The most words per thread do not quite fit beside the rest: of the variants
+// of 25 words the compiler keeps 3 registers in scratch with one sum, 13 at T = 2 and 4, 22 (bf16) or 40 (fp16) at other
+// temperatures with labels, and of those of 12 fp32 words 6 to 8 with two sums; no other variant has any.
 template <typename T, int kSums, int kWords, int kSure>
 __global__ __launch_bounds__(kMaxBlock, 4) void row_step(Task a, float c0, const float* dloss, int dloss_step, float* loss,
                                                             T* dlogits, int64_t out_width, int log2_slots) {
@@ -757,8 +759,12 @@ int columns_per_split(int64_t rows, int64_t vocab, int64_t most) {
 }
 
 // The forward call.  A few long rows are read by several workgroups each, whose partial sums a second
-// launch joins (16 bits, us split and whole: 8 rows of 65536 7.9 and 9.0, of 100000 8.2 and 10.7; 64 rows
-// of 65536 9.3 and 9.1, of 256000 13.8 and 20.3; 256 rows of 65536 13.9 and 11.2).
+// launch joins.  Columns count rather than bytes, since a thread waits for its chain of exponentials as much as
+// for its words (T = 2 with labels, us whole and split: 8 rows of 50257 8.6 and 8.1 in fp32, 8.5 and 8.1 in 16 bits,
+// of 160000 15.2 and 8.3, 15.1 and 8.2; 64 rows of 50257 8.7 and 9.4, 8.5 and 9.3, of 65536 9.6 and 9.4, 9.4 and
+// 9.2, of 160000 17.5 and 14.1, 15.2 and 11.5; 256 rows of 160000 29.6 and 31.4, 19 and 22).  Between 64 and
+// 256 rows the two cross, in 16 bits later than in fp32, and the rule leaves up to a quarter there (65 rows of
+// 160000 17.5 and 14.3, 15.2 and 11.7; 100 rows 18.2 and 18.4, 16.7 and 13.7; 150 rows 20.2 and 22.6, 18.2 both).
 bool loss_is_split(int64_t rows, int64_t vocab) { return rows <= kFewRows && vocab > 65536; }
 
 // Otherwise a workgroup reads a row, a larger one where there are not many and they are long (16 bits, us
@@ -772,9 +778,13 @@ constexpr int kMaxChain = 224;
 
 // Threads of row_step for a row, the fewest whose registers hold it, from 256 with many rows and from 512
 // with fewer, or 0: then row_part and row_grad read it twice, with workgroups for every CU.  So are a few
-// long rows (16 bits, us twice and once: 8 rows of 8192 12.4 and 11.5, of 32000 12.3 and 14, of 160000 9.5
-// and 24; 64 rows of 16384 12.7 and 12.3, of 32000 13.4 and 14.2; but 256 rows of 50257 24 and 20, 2048
-// of 200000 460 and 409).
+// long rows (T = 2 with labels, us once and twice: 8 rows of 16384 8.2 and 8.5 in fp32, 8.4 both in 16 bits, of 32000
+// 10.7 and 8.8, 10 and 8.6, of 98000 18.4 and 8.9, 17.4 and 8.7; 64 rows of 16384 12.9 and 12.5, 12.7 and 12.9, of 32000
+// 15.7 and 14, 14.2 and 12.2, of 98000 25.8 and 21.7, 19.5 and 14.9; but 256 rows of 50257 28.5 and 34.4, 20.7 and 25;
+// 2048 of 98000 in fp32 395 and 442, of 200000 in 16 bits 436 and 468).  From 65 to about 100 rows twice is still the
+// faster of the two for long ones (65 rows of 98000 23.3 and 21.6, 19.8 and 15.1; 100 rows 28.7 and 30.2, 23.5 and
+// 21), and so it is for the longest at other temperatures with labels, whose words spill (2048 of 200000 at
+// T = 1.5 496 and 480 in bf16, 516 and 485 in fp16).
 template <typename T>
 int block_for_row(int64_t rows, int64_t vocab) {
   if (rows <= kFewRows && vocab > 24576) return 0;

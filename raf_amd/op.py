@@ -709,6 +709,8 @@ def defuse_tensor(data: torch.Tensor, sizes, shapes, shape_indices):
 
 
 # ------------------------------------------------------------------- the operators at the vocabulary
+# Like the rest of this module they are RAF's imperative operators, not autograd functions: what they return
+# does not require a gradient, whatever their inputs do.
 class _VocabEnvCache(_EnvCache):
     """Theirs are kept apart: batches of ever new lengths should not push the optimizers' OpEnvs out,
     and these own no device memory."""
@@ -781,7 +783,8 @@ def embedding(x: torch.Tensor, indices: torch.Tensor, scale: float = 1.0, first_
     unless given), so an fp32 master table can feed a 16-bit model directly.  ``first_row`` is the
     index of the table's first row, for a table that is one shard of a vocabulary.  An index outside
     the table (another shard's, or a negative one for padding) gives zeros, not an error: the host
-    does not look at the indices."""
+    does not look at the indices.  The result is no node of an autograd graph: its gradient is the
+    caller's ``embedding_dx``."""
     scale, first_row = float(scale), int(first_row)
     key = ("embedding", _lib.glue().key((x, indices)), scale, first_row, out_dtype)
     env = _vocab_envs.get(key)
@@ -801,8 +804,9 @@ def embedding_dx(dy: torch.Tensor, indices: torch.Tensor, num_weight: int, scale
     rounded once to ``out_dtype`` (dy's unless given).  Indices outside the table and those equal to
     ``padding_idx`` take no part.  With ``grad`` the result is added to it in place and ``grad`` is
     returned (of ``out_dtype``, if both are given): the gradient of a table that an output projection
-    shares, or of a batch in several parts.  Equal inputs give equal bits, however often an index
-    occurs."""
+    shares, or of a batch in several parts.  It must share no memory with ``dy`` or ``indices``; autograd
+    is not told that it changed (its version counter stays).  Equal inputs give equal bits, however
+    often an index occurs."""
     if out_dtype is None:
         out_dtype = dy.dtype if grad is None else grad.dtype
     num_weight, scale, first_row = int(num_weight), float(scale), int(first_row)
@@ -845,7 +849,8 @@ def topk_distill(logits: torch.Tensor, topk_indices: torch.Tensor, topk_logits: 
     ``topk_distill_dx`` needs.  A teacher entry whose index is outside the vocabulary (-1, say) or
     whose logit is -inf is absent, and so is a label outside it (-100, say); a row without any has
     loss 0 and no gradient, whatever its logits hold.  ``vocab_size`` leaves out the padding columns
-    of a widened output projection.  ``labels`` have the dtype of ``topk_indices``."""
+    of a widened output projection.  ``labels`` have the dtype of ``topk_indices``.  The loss is no
+    node of an autograd graph: its gradient is the caller's ``topk_distill_dx``."""
     return _topk_distill(0, logits, topk_indices, topk_logits, labels, None, None, temperature, soft_weight, hard_weight,
                          vocab_size)
 
