@@ -47,8 +47,9 @@ int rafhip_embedding(const void* x, int32_t x_dtype, int64_t rows, int64_t width
 /*
  * Its gradient for the table,
  *     dx[r, :] = (accumulate ? dx[r, :] : 0) + scale * sum of dy[t, :] over t with indices[t] - first_row == r,
- * over all rows x width of dx.  Tokens are sorted by row and each row's are added in fp32 in an
- * order fixed by their positions, so equal inputs give equal bits.  Indices outside the table and,
+ * over all rows x width of dx.  Tokens are sorted by row and each row's are added in an order
+ * fixed by their positions, 32 (up to 256 tokens: all) in fp32 and these sums in fp64, so equal inputs give
+ * equal bits.  Indices outside the table and,
  * with has_padding, indices equal to padding_index take no part (their dy is not read).  With
  * accumulate, rows without a token keep their bits.
  * dy: n x width of dy_dtype, dx: rows x width of dx_dtype, contiguous.

@@ -785,12 +785,14 @@ __global__ __launch_bounds__(kBlock) void sum_rows(const TD* dy, const uint32_t*
   }
 }
 
-// The chunks of a long row added in order: 64 columns per workgroup, four stretches of chunks.
+// The chunks of a long row added in order: 64 columns per workgroup, four stretches of chunks.  In fp64, so that a
+// row's error is that of its chunks' 32 fp32 additions however many there are (in fp32 a row of 2^22 equal
+// tokens was off by 3e-4).
 template <typename TO>
 __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale, int accumulate, TO* dx,
                                                      const Taken* taken, const Item* items, const uint32_t* long_rows,
                                                       const float* parts) {
-  __shared__ float sums[kWaves][kLanes];
+  __shared__ double sums[kWaves][kLanes];
   const int lane = threadIdx.x & (kLanes - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
   const int64_t col = (int64_t)blockIdx.x * kLanes + lane;
@@ -801,7 +803,7 @@ __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale
     const int chunks = (int)((row.tokens + kChunk - 1) / kChunk);
     const int per = (chunks + kWaves - 1) / kWaves;
     const int from = wave * per, to = from + per < chunks ? from + per : chunks;
-    float acc = 0.f;
+    double acc = 0.0;
     if (col < width) {
       const float* p = parts + (int64_t)it * width + col;
       for (int c0 = from; c0 < to; c0 += kInFlight) {
@@ -818,7 +820,7 @@ __global__ __launch_bounds__(kBlock) void join_chunks(int64_t width, float scale
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave == 0 && col < width) {
-      float total[1] = {((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]};
+      const float total[1] = {(float)(((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane])};
       put_row<TO, 1>(dx + (int64_t)row.row * width + col, total, scale, accumulate != 0);
     }
   }

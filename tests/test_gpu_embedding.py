@@ -204,6 +204,68 @@ def test_gradient_of_many_rows_takes_many_tiles(native_libs):
     assert k.max() > 30_000
 
 
+@pytest.mark.parametrize("n", [1 << 16, 1 << 20, 1 << 22, 8_388_608])
+def test_gradient_of_a_token_that_occurs_millions_of_times(native_libs, n):
+    """A token's sum is off by the 31 additions of a chunk and its last rounding, however often it occurs;
+    8,388,608 tokens are the most that are taken."""
+    from raf_amd import op
+
+    rows, value = 1000, torch.tensor([0.3, 0.7, 0.11, 1.3, -0.9])
+    dy = value.expand(n, 5).contiguous().to(DEV)
+    ids = torch.full((n,), 500, dtype=I32, device=DEV)
+    ids[5::1000] = 3
+    ids[7::1000] = -1
+    got = op.embedding_dx(dy, ids, rows).cpu().double()
+    for row in (3, 500):
+        want = value.double() * int((ids == row).sum())
+        assert ((got[row] - want).abs() <= 33 * U * want.abs()).all(), row
+    got[[3, 500]] = 0
+    assert not got.any()
+
+
+def test_gradient_of_the_largest_batch(native_libs):
+    from raf_amd import op
+
+    n, rows, width = 8_388_608, 262_143, 3
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    ids = (torch.exp(torch.rand(n, device=DEV, generator=gen, dtype=torch.float64) * np.log(rows)).long() - 1) % rows
+    ids[::7] = torch.randint(0, rows, (len(ids[::7]),), device=DEV, generator=gen)
+    dy = (torch.randn(n, width, device=DEV, generator=gen) * 1024).round() / 1024
+    got = op.embedding_dx(dy, ids, rows).double()
+    in_order, order = torch.sort(ids)
+    ends = torch.searchsorted(in_order, torch.arange(rows + 1, device=DEV))
+
+    def by_rows(x):  # differences of running sums, which are exact: multiples of 2^-10 below 2^26
+        running = torch.cat([torch.zeros(1, width, device=DEV, dtype=torch.float64), x[order].double().cumsum(0)])
+        return running[ends[1:]] - running[ends[:-1]]
+
+    assert ((got - by_rows(dy)).abs() <= 33 * U * by_rows(dy.abs())).all()
+
+
+def test_the_widest_rows(native_libs):
+    """2^24 - 1 columns, a row beyond the reach of 32-bit byte offsets behind a few others."""
+    from raf_amd import op
+
+    rows, width = 70, (1 << 24) - 1
+    x = torch.zeros(rows, width, dtype=F16, device=DEV)
+    x[:, ::1_000_003] = _randn(rows, 17, dtype=F16).to(DEV)
+    x[:, -1] = torch.arange(rows, dtype=F16, device=DEV) + 1
+    for n in (3, 300):
+        ids = torch.arange(n, dtype=I32, device=DEV) * 23 % (rows + 1)  # the last is outside
+        y = op.embedding(x, ids)
+        inside = ids < rows
+        for at in range(0, n, max(n // 7, 1)):
+            assert torch.equal(y[at], x[ids[at]]) if inside[at] else not y[at].any()
+        dx = op.embedding_dx(y, ids, rows)
+        count = torch.bincount(ids.long(), minlength=rows)[:rows]
+        for row in range(0, rows, 9):  # sums of equal halves, a few of them: exact in fp32
+            assert torch.equal(dx[row], (x[row].float() * count[row]).to(F16)), row
+        assert torch.equal(dx[:, -1], ((torch.arange(rows, device=DEV) + 1) * count).to(F16))
+        del y, dx
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_gradient_leaves_out_what_takes_no_part(native_libs):
     """Tokens of padding and of other shards: their gradients may hold anything."""
     from raf_amd import op
