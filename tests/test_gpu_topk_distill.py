@@ -195,6 +195,41 @@ def test_more_rows_than_a_grid_dimension_holds(native_libs):
     _all(z, idx, t, labels, dloss, temperature=2.0, hard=1.0)
 
 
+@pytest.mark.parametrize("rows", [1, 65])
+def test_the_longest_rows(native_libs, rows):
+    """2^28 - 1 columns, read in parts and whole: a uniform student, a teacher with the last column."""
+    from raf_amd import op
+
+    vocab = (1 << 28) - 1
+    if torch.cuda.mem_get_info()[0] < 5 * rows * vocab:
+        pytest.skip("needs 87 GB of free memory")
+    z = torch.zeros(rows, vocab, dtype=BF16, device=DEV)
+    idx = torch.tensor([[vocab - 1, 0, vocab]], dtype=I32, device=DEV).repeat(rows, 1)  # the third is outside
+    t = torch.tensor([[2.0, 0.0, 9.0]], device=DEV).repeat(rows, 1)
+    labels = torch.full((rows,), vocab - 2, dtype=I32, device=DEV)
+    p = torch.softmax(t[0, :2].double() / 2, 0).cpu()
+    more = dict(temperature=2.0, labels=labels, hard_weight=0.5)
+    bound = U * (300 + 8 * 28)
+    want = 4 * (float((p * p.log()).sum()) + np.log(vocab)) + 0.5 * np.log(vocab)
+    loss, stats = op.topk_distill(z, idx, t, **more)
+    assert ((loss.double() - want).abs() <= bound * 5 + 2 * U * want).all()
+    assert ((stats[:, 1:].double() - np.log(vocab)).abs() <= bound + U * 20).all() and not stats[:, 0].any()
+    one = torch.ones(1, device=DEV)
+
+    def check(grad):
+        for at, value in ((vocab - 1, -2 * p[0]), (0, -2 * p[1]), (vocab - 2, -0.5), (vocab // 2, 2.5 / vocab), (1, 2.5 / vocab)):
+            near = 1.01 * HALF_STEP[BF16] * abs(float(value)) + 3 / vocab  # the two softmaxes where a target is
+            assert ((grad[:, at].double() - float(value)).abs() <= near).all(), at
+        assert (grad[:, 1:vocab - 2] == grad[0, 1]).all() and grad[0, 1] > 0
+
+    check(op.topk_distill_dx(one, z, idx, t, stats, **more))
+    loss2, grad = op.topk_distill_step(z, idx, t, one, **more)
+    assert ((loss2.double() - want).abs() <= bound * 5 + 2 * U * want).all()
+    check(grad)
+    del z, grad
+    torch.cuda.empty_cache()
+
+
 def test_more_rows_than_a_launch_holds(native_libs):
     """2^24 workgroups of 256 threads are one more than a launch may have: the loss and the combined call go on
     in another.  Two columns, so that the definition is a formula; each rounding is at most 2^-24 of
